@@ -18,6 +18,12 @@ from .interface import (  # noqa: F401
     ssta_lists,
     sta_lists,
 )
+from .window import (  # noqa: F401
+    SlidingWindowAttnFunc,
+    backward_with_window,
+    forward_with_window,
+    sliding_window_attn_func,
+)
 
 __all__ = [
     "flex_block_attn_func",
@@ -36,4 +42,8 @@ __all__ = [
     "Fp8KVCache",
     "quantize_kv",
     "flex_block_attn_fp8kv",
+    "sliding_window_attn_func",
+    "SlidingWindowAttnFunc",
+    "forward_with_window",
+    "backward_with_window",
 ]

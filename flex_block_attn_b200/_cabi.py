@@ -45,6 +45,9 @@ EXPORTED_SYMBOLS = (
     "fba_bwd_partial_bytes",
     "fba_bwd_split",
     "fba_set_bwd_kernel",
+    "fba_window_fwd",
+    "fba_window_partial_bytes",
+    "fba_window_bwd",
     "fba_bwd_static_scratch_max_rows",
     "fba_bwd_static_scratch",
     "fba_peer_alloc",
@@ -151,6 +154,12 @@ def lib() -> ctypes.CDLL:
                                                         vp, vp, vp, ctypes.c_uint64, vp, vp]
     L.fba_set_bwd_kernel.restype = i32
     L.fba_set_bwd_kernel.argtypes = [i32]
+    L.fba_window_fwd.restype = i32
+    L.fba_window_fwd.argtypes = [vp] * 5 + [i32] * 7 + [ctypes.c_float, vp, vp]
+    L.fba_window_partial_bytes.restype = i32
+    L.fba_window_partial_bytes.argtypes = [i32] * 7 + [ctypes.POINTER(ctypes.c_uint64)]
+    L.fba_window_bwd.restype = i32
+    L.fba_window_bwd.argtypes = [vp] * 9 + [i32] * 7 + [ctypes.c_float, vp, vp, vp, ctypes.c_uint64, vp, vp]
     L.fba_bwd_static_scratch_max_rows.restype = ctypes.c_uint64
     L.fba_bwd_static_scratch_max_rows.argtypes = []
     L.fba_bwd_static_scratch.restype = i32

@@ -1,10 +1,11 @@
 // Error reporting, version query and TMA tensor-map construction for libfba_b200.so.
+#include <math.h>
 #include <stdio.h>
 #include <string.h>
 
 #include <nvtx3/nvToolsExt.h>
 
-#include "fba_internal.cuh"
+#include "fba_common.cuh"
 
 namespace fba {
 
@@ -146,6 +147,28 @@ int make_tmap_u8(CUtensorMap* out, const void* base, long long inner, long long 
         snprintf(buf, sizeof(buf), "cuTensorMapEncodeTiled (8-bit) failed with CUresult %d", (int)r);
         return set_error(FBA_ERR_DRIVER, buf);
     }
+    return FBA_OK;
+}
+
+int window_args(const char* who, int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks, float softmax_scale,
+                WindowDev* win) {
+    char buf[160];
+    const char* why = nullptr;
+    int code = FBA_ERR_BAD_ARG;
+    constexpr int kMaxLen = 1 << 29;   // sums of a position, a window and a tile or two stay below 2^31
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0) why = "non-positive size";
+    else if (Hq % Hkv != 0) why = "Hq must be a multiple of Hkv";
+    else if (window < 0 || sinks < 0) why = "window and sinks must not be negative";
+    else if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY)) why = "softmax_scale must be positive and finite";
+    else if (Sq > kMaxLen || Skv > kMaxLen) code = FBA_ERR_TOO_LARGE, why = "more than 2^29 rows";
+    else if (static_cast<long long>(B) * Hq > 65535) code = FBA_ERR_TOO_LARGE, why = "B * Hq exceeds 65535";
+    if (why) {
+        snprintf(buf, sizeof(buf), "%s: %s", who, why);
+        return set_error(code, buf);
+    }
+    win->q_off = Skv - Sq;
+    win->window = window == 0 || window > Skv ? Skv : window;
+    win->sinks = sinks > Skv ? Skv : sinks;
     return FBA_OK;
 }
 

@@ -104,6 +104,8 @@ struct BwdParams {
     int parts;             // 1: one CTA per (key tile, kv head); else the last tiles are split into this many CTAs each:
     int split_from;        //   those from this one on (kv head * n_ntiles + tile),
     int n_whole;           //   behind this many CTAs with whole groups
+    WindowDev win;         // fba_window_bwd alone (n_whole: its key tiles with sinks, which are split into `parts`)
+    int Sq;
 };
 
 // ------------------------------------------------------------------------------------------
@@ -259,7 +261,11 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
 // kWithDq = false: the dK / dV-only variant that runs beside the query-major dQ pass
 // (fba_bwd_dq.cu): no dQ GEMM, no drain, no reductions.  kSplit: some key tiles are split by query heads (SplitPlan);
 // decided at run time it cost every CTA some 200 clocks, 2 % of a call with lists of one entry.
-template <bool kWithDq, bool kSplit>
+// kWindow: the query tiles of a key tile follow from a sliding window and sinks and are one range, the same for every head;
+// probabilities outside the mask become zero one by one.  A key tile with sinks is seen by every query behind it, and so
+// has a list many times the others' length: with kSplit its steps (query heads one after the other, query tiles in
+// order) are divided over `parts` CTAs at the front of the grid.
+template <bool kWithDq, bool kSplit, bool kWindow = false>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -282,7 +288,17 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const int group = p.Hq / p.Hkv;
     int bhk = blockIdx.y, nt = blockIdx.x, part0 = 0, hr = group;   // bhk: b * Hkv + kv head
     float* partial = nullptr;
-    if (kSplit) {
+    if constexpr (kWindow && kSplit) {
+        const int split_ctas = p.n_whole * p.parts;
+        if (nt < split_ctas) {
+            const int cta = nt;
+            nt = cta / p.parts;
+            part0 = cta - nt * p.parts;
+            partial = p.partial + (static_cast<long long>(bhk) * split_ctas + cta) * 32768;
+        } else {
+            nt -= split_ctas - p.n_whole;
+        }
+    } else if (kSplit) {
         const int cta = nt - p.n_whole;
         if (cta < 0) {
             bhk = nt / p.n_ntiles;
@@ -296,12 +312,12 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             partial = p.partial + cta * 32768LL;
         }
     }
-    if (partial == nullptr) {
+    if (!kWindow && partial == nullptr) {
         if (p.list.order) nt = p.list.order[static_cast<long long>(p.list.bh_stride ? bhk : 0) * p.n_ntiles + nt];
         if (kSplit && bhk * p.n_ntiles + nt >= p.split_from) return;   // its parts are at the end of the grid
     }
-    const int bq0 = (bhk / p.Hkv) * p.Hq + (bhk % p.Hkv) * group + part0;
-    const int sub = p.list.sub;
+    const int bq0 = (bhk / p.Hkv) * p.Hq + (bhk % p.Hkv) * group + (kWindow ? 0 : part0);
+    const int sub = kWindow ? 1 : p.list.sub;
 
     if ((base & 1023u) != 0u) {
         // The swizzled operand panels need a 1024-byte aligned base; report instead of computing garbage.
@@ -314,7 +330,24 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         return static_cast<long long>(bq0 + r) * p.list.bh_stride + nt / p.list.rows_div;
     };
     int n_total = 0;
-    for (int r = 0; r < hr; ++r) n_total += p.list.cnt[list_row(r)] * sub;
+    // Under a window: query tiles win_first .. win_first + win_cnt - 1 of every head; this CTA's steps begin at win_step0.
+    int win_first = 0, win_cnt = 1, win_step0 = 0;
+    if constexpr (kWindow) {
+        const int key = nt * 128, last_key = key + 127;
+        const int lo = max(0, key - p.win.q_off);                               // first and last row that sees the tile
+        const int hi = key < p.win.sinks ? p.Sq - 1 : min(p.Sq - 1, last_key + p.win.window - 1 - p.win.q_off);
+        win_first = lo / 128;
+        const int cnt = hi < lo ? 0 : hi / 128 - win_first + 1;
+        n_total = cnt * group;
+        win_cnt = max(cnt, 1);
+        if (kSplit && partial != nullptr) {
+            win_step0 = static_cast<int>(static_cast<long long>(part0) * n_total / p.parts);
+            n_total = static_cast<int>(static_cast<long long>(part0 + 1) * n_total / p.parts) - win_step0;
+        }
+        hr = 1;   // one loop over all steps
+    } else {
+        for (int r = 0; r < hr; ++r) n_total += p.list.cnt[list_row(r)] * sub;
+    }
     n_total = warp_uniform(n_total);
 
     if (threadIdx.x == 0) {
@@ -397,12 +430,20 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 if (c.r < hr) c.q0 = p.list.idx[c.lr * p.list.stride + c.e] * sub;
             };
             Cursor cur;
-            cur_init(cur);
+            if constexpr (!kWindow) cur_init(cur);
             bool ok = true;
             for (int it = 0; it < n_total && ok; ++it) {
-                if (it > 0) cur_next(cur);
                 const uint32_t sq = q_slot(it), sd = do_slot(it), parity = ((it >> 1) & 1u) ^ 1u;
-                const int qt = cur.q0 + cur.u, bq = bq0 + cur.r;
+                int qt, bq;
+                if constexpr (kWindow) {
+                    const int r = (win_step0 + it) / win_cnt;
+                    qt = win_first + win_step0 + it - r * win_cnt;
+                    bq = bq0 + r;
+                } else {
+                    if (it > 0) cur_next(cur);
+                    qt = cur.q0 + cur.u;
+                    bq = bq0 + cur.r;
+                }
                 if (!mbar_wait(bar(kBEmpty + sq), parity, abort_flag)) {
                     report_timeout(p.status, 2, 13, it, 100);
                     ok = false;
@@ -504,11 +545,18 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         int it = 0;
         bool ok = true;
         for (int r = 0; r < hr && ok && kWithDq; ++r) {
-            const long long lr = list_row(r);
-            const int cnt = p.list.cnt[lr];
-            const long long bq = bq0 + r;
+            const long long lr = kWindow ? 0 : list_row(r);
+            const int cnt = kWindow ? n_total : p.list.cnt[lr];
+            long long bq = bq0 + r;
             for (int e = 0; e < cnt && ok; ++e) {
-                const int q0 = p.list.idx[lr * p.list.stride + e] * sub;
+                int q0;
+                if constexpr (kWindow) {
+                    const int head = (win_step0 + e) / win_cnt;
+                    q0 = win_first + win_step0 + e - head * win_cnt;
+                    bq = bq0 + head;
+                } else {
+                    q0 = p.list.idx[lr * p.list.stride + e] * sub;
+                }
                 for (int u = 0; u < sub && ok; ++u, ++it) {
                     if (!mbar_wait(bar(kBDqFull), it & 1u, abort_flag)) {
                         if (lane == 0) report_timeout(p.status, 2, static_cast<uint32_t>(warp), it, 300);
@@ -563,10 +611,10 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         int it = 0;
         bool ok = true;
         for (int r = 0; r < hr && ok; ++r) {
-            const long long lr = list_row(r);
-            const int cnt = p.list.cnt[lr];
+            const long long lr = kWindow ? 0 : list_row(r);
+            const int cnt = kWindow ? n_total : p.list.cnt[lr];
             for (int e = 0; e < cnt && ok; ++e) {
-                const uint32_t w = p.list.msk ? p.list.msk[lr * p.list.stride + e] : 0xffffu;
+                const uint32_t w = !kWindow && p.list.msk ? p.list.msk[lr * p.list.stride + e] : 0xffffu;
                 for (int u = 0; u < sub && ok; ++u, ++it) {
                     const int st = it & 1;
                     const float2* lse2 = reinterpret_cast<const float2*>(base_ptr + kBwdSmemLD + st * 1024) + 32 * h + q4;
@@ -601,7 +649,27 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                             }
                         }
                     }
-                    if (w != 0xffffu) {
+                    if constexpr (kWindow) {
+                        // Distance of the query of column 0 from key row 0; the tile is seen whole unless some key
+                        // lies ahead of a query, or behind its window and the sinks.
+                        const int step = win_step0 + it;
+                        const int d0 = (win_first + step % win_cnt - nt) * 128 + p.win.q_off;
+                        if (d0 < 127 || (d0 + 127 >= p.win.window && nt * 128 + 127 >= p.win.sinks)) {
+                            const int d_lane = d0 + 64 * h + 2 * q4 - (quad * 32 + (lane >> 2));
+#pragma unroll
+                            for (int g = 0; g < 4; ++g) {
+                                const int key = nt * 128 + quad * 32 + (lane >> 2) + 8 * g;
+                                const uint32_t most = key < p.win.sinks ? 0x7fffffffu : static_cast<uint32_t>(p.win.window - 1);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j)
+#pragma unroll
+                                    for (int e2 = 0; e2 < 2; ++e2) {   // a negative distance is above `most` as well
+                                        const int o = 32 * (g >> 1) + 4 * j + 2 * (g & 1) + e2;
+                                        if (static_cast<uint32_t>(d_lane - 8 * g + 8 * j + e2) > most) pr[o] = 0.f;
+                                    }
+                            }
+                        }
+                    } else if (w != 0xffffu) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
                             if (!((w >> (mbit0 + 4 * h + (j >> 1))) & 1u)) {
@@ -824,6 +892,28 @@ extern "C" int fba_bwd_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv, ui
     return FBA_OK;
 }
 
+// Row statistics, and zeros in the dQ accumulator (null: none is used).
+static int launch_prep(const void* o, const void* dout, const float* lse, float* lse_delta, float* dq_accum, int Sq,
+                       long long n_bhq, float scale, cudaStream_t stream) {
+    const int rows_pad = (Sq + 127) / 128 * 128;
+    const long long total_rows = n_bhq * rows_pad;
+    if (total_rows > 0x7fffff00LL) return set_error(FBA_ERR_TOO_LARGE, "fba_bwd: more than 2^31 query rows");
+    long long blocks = (total_rows + 31) / 32;             // 8 warps x 4 rows per step
+    if (blocks > 148 * 16) blocks = 148 * 16;
+    bwd_prep_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
+        static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(dout), lse,
+        reinterpret_cast<float2*>(lse_delta), static_cast<uint32_t>(Sq), static_cast<uint32_t>(rows_pad),
+        static_cast<uint32_t>(total_rows), scale);
+    const int rc = check_launch("bwd_prep_kernel");
+    if (rc != FBA_OK) return rc;
+    if (dq_accum &&
+        cudaMemsetAsync(dq_accum, 0, static_cast<size_t>(total_rows) * 128 * sizeof(float), stream) != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(FBA_ERR_LAUNCH, "fba_bwd: cudaMemsetAsync failed");
+    }
+    return FBA_OK;
+}
+
 extern "C" int fba_bwd_ex(const void* q, const void* k, const void* v, const void* o, const float* lse,
                           const void* dout, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq,
                           int Skv, const fba_list_t* k2q, const fba_list_t* q2k, float softmax_scale, int dq_mode,
@@ -898,23 +988,8 @@ extern "C" int fba_bwd_split(const void* q, const void* k, const void* v, const 
     if ((rc = make_tmap_bf16(&tm_dv, dv, Skv, n_bhk, 128)) != FBA_OK) return rc;
     if (qmajor && (rc = make_tmap_bf16(&tm_dq, dq, Sq, n_bhq, 128)) != FBA_OK) return rc;
 
-    const int rows_pad = n_mtiles * 128;
-    const long long total_rows = n_bhq * rows_pad;
-    {
-        if (total_rows > 0x7fffff00LL) return set_error(FBA_ERR_TOO_LARGE, "fba_bwd: more than 2^31 query rows");
-        long long blocks = (total_rows + 31) / 32;             // 8 warps x 4 rows per step
-        if (blocks > 148 * 16) blocks = 148 * 16;
-        bwd_prep_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
-            static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(dout), lse,
-            reinterpret_cast<float2*>(lse_delta), static_cast<uint32_t>(Sq), static_cast<uint32_t>(rows_pad),
-            static_cast<uint32_t>(total_rows), softmax_scale);
-        if ((rc = check_launch("bwd_prep_kernel")) != FBA_OK) return rc;
-    }
-    if (!qmajor &&
-        cudaMemsetAsync(dq_accum, 0, static_cast<size_t>(total_rows) * 128 * sizeof(float), stream) != cudaSuccess) {
-        cudaGetLastError();
-        return set_error(FBA_ERR_LAUNCH, "fba_bwd: cudaMemsetAsync failed");
-    }
+    rc = launch_prep(o, dout, lse, lse_delta, qmajor ? nullptr : dq_accum, Sq, n_bhq, softmax_scale, stream);
+    if (rc != FBA_OK) return rc;
     {
         BwdParams p;
         p.list = to_dev(*k2q);
@@ -968,6 +1043,103 @@ extern "C" int fba_bwd_split(const void* q, const void* k, const void* v, const 
         if ((rc = check_launch("bwd_convert_kernel")) != FBA_OK) return rc;
     }
     return FBA_OK;
+}
+
+// Split of the key tiles with sinks under a window: how many CTAs divide one such tile's steps.
+//
+// Every query behind a sink sees it, so its tile has group * ceil(Sq / 128) steps where the others have about
+// group * (window / 128 + 1); unsplit it would be what the whole launch waits for.  A part gets no fewer steps than the
+// other tiles have, nor than half of an SM's share of all steps: shorter ones end no launch sooner.
+static int window_parts(int B, int Hq, int Hkv, int Sq, int Skv, const WindowDev& win) {
+    const int sink_tiles = (win.sinks + 127) / 128, n_ntiles = (Skv + 127) / 128;
+    if (sink_tiles == 0 || win.window >= Skv) return 1;   // no sinks, or a causal mask without a window
+    const long long group = Hq / Hkv, n_bhk = static_cast<long long>(B) * Hkv;
+    const int first = win.q_off < 0 ? -win.q_off / 128 : 0;   // rows ahead of every key see nothing
+    const long long sink_steps = group * ((Sq + 127) / 128 - first);
+    long long tile_steps = group * ((win.window + 254) / 128 + 1);
+    if (tile_steps > sink_steps) tile_steps = sink_steps;
+    const long long all = n_bhk * (sink_tiles * sink_steps + (n_ntiles - sink_tiles) * tile_steps);
+    const long long least = tile_steps > all / (2 * kSms) ? tile_steps : all / (2 * kSms);
+    long long parts = (sink_steps + least - 1) / least;
+    const long long room = 4 * kSms / (n_bhk * sink_tiles);   // at most 592 parts in all: 74 MB of partial sums
+    if (parts > room) parts = room;
+    return parts < 1 ? 1 : static_cast<int>(parts);
+}
+
+extern "C" int fba_window_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks, uint64_t* bytes) {
+    WindowDev win;
+    const int rc = window_args("fba_window_partial_bytes", B, Hq, Hkv, Sq, Skv, window, sinks, 1.f, &win);
+    if (rc != FBA_OK) return rc;
+    if (!bytes) return set_error(FBA_ERR_BAD_ARG, "fba_window_partial_bytes: null pointer argument");
+    const int parts = window_parts(B, Hq, Hkv, Sq, Skv, win);
+    *bytes = parts == 1 ? 0 : static_cast<uint64_t>(B) * Hkv * ((win.sinks + 127) / 128) * parts * 2 * 128 * 128 * sizeof(float);
+    return FBA_OK;
+}
+
+extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                              const void* dout, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq, int Skv,
+                              int window, int sinks, float softmax_scale, float* lse_delta, float* dq_accum,
+                              float* partial, uint64_t partial_bytes, uint32_t* status, void* stream_) {
+    ProfRange range("fba_window_bwd");
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    if (!q || !k || !v || !o || !lse || !dout || !dq || !dk || !dv || !lse_delta || !dq_accum || !status)
+        return set_error(FBA_ERR_BAD_ARG, "fba_window_bwd: null pointer argument");
+    WindowDev win;
+    int rc = window_args("fba_window_bwd", B, Hq, Hkv, Sq, Skv, window, sinks, softmax_scale, &win);
+    if (rc != FBA_OK) return rc;
+    uint64_t need = 0;
+    if ((rc = fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, window, sinks, &need)) != FBA_OK) return rc;
+    if (need != 0 && (!partial || partial_bytes < need || reinterpret_cast<uintptr_t>(partial) % 16 != 0))
+        return set_error(FBA_ERR_BAD_ARG, "fba_window_bwd: partial must be 16-byte aligned, of fba_window_partial_bytes() bytes");
+    const int n_mtiles = (Sq + 127) / 128, n_ntiles = (Skv + 127) / 128, sink_tiles = (win.sinks + 127) / 128;
+    const int parts = need ? window_parts(B, Hq, Hkv, Sq, Skv, win) : 1;
+    const long long n_bhq = static_cast<long long>(B) * Hq, n_bhk = static_cast<long long>(B) * Hkv;
+    const long long sum_blocks = parts > 1 ? 8 * n_bhk * sink_tiles : 0;
+    if (n_bhq + (sum_blocks + n_mtiles - 1) / n_mtiles > 65535)
+        return set_error(FBA_ERR_TOO_LARGE, "fba_window_bwd: B * Hq and the sums of the split tiles exceed 65535 rows of a grid");
+
+    CUtensorMap tm_q, tm_k, tm_v, tm_do, tm_dk, tm_dv;
+    DeviceGuard guard;
+    if ((rc = guard.bind(q)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_q, q, Sq, n_bhq, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_k, k, Skv, n_bhk, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_v, v, Skv, n_bhk, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_do, dout, Sq, n_bhq, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_dk, dk, Skv, n_bhk, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_dv, dv, Skv, n_bhk, 128)) != FBA_OK) return rc;
+    if ((rc = launch_prep(o, dout, lse, lse_delta, dq_accum, Sq, n_bhq, softmax_scale, stream)) != FBA_OK) return rc;
+
+    BwdParams p = {};
+    p.ld = reinterpret_cast<const float2*>(lse_delta);
+    p.dq_accum = dq_accum;
+    p.status = status;
+    p.n_mtiles = n_mtiles;
+    p.Hq = Hq;
+    p.Hkv = Hkv;
+    p.scale = softmax_scale;
+    p.partial = partial;
+    p.n_ntiles = n_ntiles;
+    p.parts = parts;
+    p.n_whole = sink_tiles;
+    p.win = win;
+    p.Sq = Sq;
+    auto kernel = parts > 1 ? fba_bwd_kernel<true, true, true> : fba_bwd_kernel<true, false, true>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBwdSmemBytes)) !=
+        cudaSuccess) {
+        cudaGetLastError();
+        return set_error(FBA_ERR_LAUNCH, "fba_window_bwd: cannot raise the dynamic shared memory limit");
+    }
+    timing_mark(2, true, stream);
+    kernel<<<dim3(n_ntiles + (parts - 1) * sink_tiles, static_cast<unsigned>(n_bhk)), kBwdThreads, kBwdSmemBytes, stream>>>(
+        tm_q, tm_k, tm_v, tm_do, tm_dk, tm_dv, p);
+    rc = check_launch("fba_bwd_kernel");
+    timing_mark(2, false, stream);
+    if (rc != FBA_OK) return rc;
+    PartialSums sums = {partial, static_cast<__nv_bfloat16*>(dv), static_cast<__nv_bfloat16*>(dk), static_cast<int>(n_bhq),
+                        static_cast<int>(sum_blocks), 0, parts, sink_tiles, Skv};
+    dim3 grid(n_mtiles, static_cast<unsigned>(n_bhq + (sum_blocks + n_mtiles - 1) / n_mtiles));
+    bwd_convert_kernel<<<grid, 256, 0, stream>>>(dq_accum, static_cast<__nv_bfloat16*>(dq), Sq, n_mtiles, sums);
+    return check_launch("bwd_convert_kernel");
 }
 
 extern "C" int fba_bwd_scaled(const void* q, const void* k, const void* v, const void* o, const float* lse,

@@ -29,6 +29,15 @@ inline ListDev to_dev(const fba_list_t& l) {
     return ListDev{l.idx, l.cnt, l.msk, l.order, l.stride, l.rows_per_bh, l.bh_stride, l.rows_div, l.sub};
 }
 
+// Sliding window with sinks: the query of row i stands at position i + q_off and sees the keys j <= position of which it
+// is less than `window` away, and of the first `sinks` keys all up to its position.
+struct WindowDev {
+    int q_off, window, sinks;
+};
+// Checks the arguments of the window entry points and fills `win` (fba_api.cu).
+int window_args(const char* who, int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks, float softmax_scale,
+                WindowDev* win);
+
 // Optional timeline probe for tuning (compiled out unless -DFBA_TRACE): CTA (0,0) stores SM clock
 // stamps as 64-bit words after the 8 status words, so the status buffer must then be large.
 #ifdef FBA_TRACE

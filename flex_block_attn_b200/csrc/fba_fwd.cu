@@ -52,7 +52,51 @@ struct FwdParams {
     uint32_t* status;
     int n_mtiles, Sq, Hq, Hkv;
     float scale_log2;      // softmax scale * log2(e)
+    WindowDev win;         // fba_window_fwd alone
 };
+
+// The key tiles of a pair of query tiles under a sliding window, without a list in memory.  Tile t (0: A, 1: B) sees
+// the key tiles [0, s) u [w, e], which differ between A and B by one tile at either end (B's window begins and ends one
+// tile later).  The tiles both see are streamed once for both; what only one sees comes first when each has one such
+// tile ("lead"; both are then at the same step), else last.
+struct WindowWalk {
+    int n[2];           // steps of A and B
+    int common[2];      // steps that come from the arithmetic list below; a single list for both when paired
+    int s[2], w[2];     // the list: 0 .. s - 1, then w, w + 1, ...
+    int alone[2];       // the tile outside the common list (paired)
+    int lead;           // 1: `alone` is step 0, else it is the last step
+    bool paired;
+};
+__device__ __forceinline__ WindowWalk window_walk(const WindowDev& win, int mt0, int Sq) {
+    WindowWalk k;
+    int e[2], s[2], w[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const int first = (mt0 + t) * 128 + win.q_off;                    // position of the tile's first row
+        const int rows = min(128, Sq - (mt0 + t) * 128);
+        const int last = first + rows - 1;
+        e[t] = rows <= 0 || last < 0 ? -1 : last / 128;                   // the last key tile; -1: no key is visible
+        w[t] = max(0, first - win.window + 1) / 128;
+        s[t] = min(w[t], min(e[t] + 1, (win.sinks + 127) / 128));
+        k.n[t] = e[t] < 0 ? 0 : s[t] + e[t] + 1 - w[t];
+        k.common[t] = k.n[t];
+        k.s[t] = s[t];
+        k.w[t] = w[t];
+        k.alone[t] = 0;
+    }
+    k.lead = 0;
+    k.paired = k.n[0] > 0 && k.n[1] > 0 && w[1] - w[0] <= 1 && e[1] - e[0] <= 1;
+    if (k.paired) {
+        const bool a = w[0] < w[1] && w[0] >= s[1], b = e[1] > e[0];      // A's first tile, B's last one
+        k.alone[0] = w[0];
+        k.alone[1] = e[1];
+        k.lead = a && b ? 1 : 0;
+        k.common[0] = k.common[1] = k.n[0] - (a ? 1 : 0);
+        k.s[0] = k.s[1] = s[1];
+        k.w[0] = k.w[1] = w[1];
+    }
+    return k;
+}
 
 // Barrier slots (8 bytes each) inside the barrier block.
 enum FwdBar : uint32_t {
@@ -68,6 +112,9 @@ enum FwdBar : uint32_t {
 static_assert(8 * kBarCount + 16 <= 256, "barrier block overflows its 256-byte slot");
 static_assert(kFwdSmemBytes <= 232448, "exceeds the 227 KiB shared memory of an sm_100 CTA");
 
+// The lowest n bits (n may lie outside 0 .. 32).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
+
 // One piece (8 / kFwdPieces k-steps of 16 keys) of O += P V.
 __device__ __forceinline__ void mma_pv_piece(uint32_t d_tmem, uint32_t p_tmem, uint32_t v_smem, int piece,
                                              bool accumulate) {
@@ -81,6 +128,9 @@ __device__ __forceinline__ void mma_pv_piece(uint32_t d_tmem, uint32_t p_tmem, u
     }
 }
 
+// kWindow: the key tiles follow from a sliding window and sinks (WindowWalk) instead of from lists, and scores outside
+// them are masked key by key.
+template <bool kWindow>
 __global__ void __launch_bounds__(kFwdThreads, 1)
 fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_o,
@@ -100,7 +150,9 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // Work item of this CTA: the blockIdx.x-th entry of the (batch, head)'s longest-first order when
     // one is given (CTAs are dispatched in blockIdx order, so the shortest items of the grid run
     // last and the tail of the launch stays short), else blockIdx.x itself.
-    const int pair = p.list.order
+    // Under a window the later rows have the longer lists.
+    const int pair = kWindow ? static_cast<int>(gridDim.x - 1 - blockIdx.x)
+                     : p.list.order
                          ? p.list.order[static_cast<long long>(p.list.bh_stride ? bh : 0) * gridDim.x + blockIdx.x]
                          : static_cast<int>(blockIdx.x);
     const int hr = p.Hq / p.Hkv;
@@ -109,12 +161,26 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // Per-tile list rows and lengths (identical in every thread).
     const int mt0 = 2 * pair, mt1 = 2 * pair + 1;
     const bool tile1_valid = mt1 < p.n_mtiles;
-    const long long lrow0 = static_cast<long long>(bh) * p.list.bh_stride + mt0 / p.list.rows_div;
-    const long long lrow1 = static_cast<long long>(bh) * p.list.bh_stride + (tile1_valid ? mt1 / p.list.rows_div : 0);
-    const int sub = p.list.sub;
-    const int n0 = warp_uniform(p.list.cnt[lrow0] * sub);
-    const int n1 = warp_uniform(tile1_valid ? p.list.cnt[lrow1] * sub : 0);
-    const bool shared_mode = tile1_valid && lrow0 == lrow1;
+    long long lrow0 = 0, lrow1 = 0;
+    int sub = 1, n0, n1;
+    WindowWalk walk;
+    if constexpr (kWindow) {
+        walk = window_walk(p.win, mt0, p.Sq);
+        n0 = warp_uniform(walk.n[0]);
+        n1 = warp_uniform(walk.n[1]);
+    } else {
+        lrow0 = static_cast<long long>(bh) * p.list.bh_stride + mt0 / p.list.rows_div;
+        lrow1 = static_cast<long long>(bh) * p.list.bh_stride + (tile1_valid ? mt1 / p.list.rows_div : 0);
+        sub = p.list.sub;
+        n0 = warp_uniform(p.list.cnt[lrow0] * sub);
+        n1 = warp_uniform(tile1_valid ? p.list.cnt[lrow1] * sub : 0);
+    }
+    const bool shared_mode = !kWindow && tile1_valid && lrow0 == lrow1;
+    // Whether the two tiles share the K / V tiles of step i (only asked where a tile has that step).
+    auto shared_at = [&](int i) {
+        if constexpr (kWindow) return walk.paired && i >= walk.lead && i < walk.lead + walk.common[0];
+        return shared_mode;
+    };
 
     if (threadIdx.x == 0) {
         *abort_flag = 0;
@@ -149,6 +215,11 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const uint32_t sQ0 = base + kFwdSmemQ, sQ1 = base + kFwdSmemQ + kTileBytes;
     auto ring = [&](int s) { return base + kFwdSmemRing + static_cast<uint32_t>(s) * kTileBytes; };
     auto kv_tile_of = [&](int t, int i) {
+        if constexpr (kWindow) {
+            const int j = i - walk.lead, s = t ? walk.s[1] : walk.s[0], w = t ? walk.w[1] : walk.w[0];
+            if (j < 0 || j >= (t ? walk.common[1] : walk.common[0])) return t ? walk.alone[1] : walk.alone[0];
+            return j < s ? j : w + j - s;
+        }
         const int e = i / sub;
         return p.list.idx[(t ? lrow1 : lrow0) * p.list.stride + e] * sub + (i - e * sub);
     };
@@ -189,13 +260,24 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 };
                 const int ln[2] = {n0, shared_mode ? 0 : n1};
                 const int nmax = ln[0] > ln[1] ? ln[0] : ln[1];
-                for (int t = 0; t < 2; ++t)
-                    if (ln[t] > 0) load(&tm_k, kv_tile_of(t, 0), 100 + t);
-                for (int i = 0; i < nmax && ok; ++i) {
-                    for (int t = 0; t < 2; ++t) {
-                        if (i < ln[t]) {
-                            load(&tm_v, kv_tile_of(t, i), 200 + t);
-                            if (i + 1 < ln[t]) load(&tm_k, kv_tile_of(t, i + 1), 100 + t);
+                if constexpr (kWindow) {   // tile B's load of a step that both share is tile A's
+                    for (int t = 0; t < 2; ++t)
+                        if (ln[t] > 0 && !(t && shared_at(0))) load(&tm_k, kv_tile_of(t, 0), 100 + t);
+                    for (int i = 0; i < nmax && ok; ++i) {
+                        for (int t = 0; t < 2; ++t) {
+                            if (i < ln[t] && !(t && shared_at(i))) load(&tm_v, kv_tile_of(t, i), 200 + t);
+                            if (i + 1 < ln[t] && !(t && shared_at(i + 1))) load(&tm_k, kv_tile_of(t, i + 1), 100 + t);
+                        }
+                    }
+                } else {
+                    for (int t = 0; t < 2; ++t)
+                        if (ln[t] > 0) load(&tm_k, kv_tile_of(t, 0), 100 + t);
+                    for (int i = 0; i < nmax && ok; ++i) {
+                        for (int t = 0; t < 2; ++t) {
+                            if (i < ln[t]) {
+                                load(&tm_v, kv_tile_of(t, i), 200 + t);
+                                if (i + 1 < ln[t]) load(&tm_k, kv_tile_of(t, i + 1), 100 + t);
+                            }
                         }
                     }
                 }
@@ -227,13 +309,14 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                 };
                 // Every ring slot needs two releases per use: one from each tile's issuer when the
                 // tiles share the stream, both from the only consumer otherwise.
-                auto release = [&](int s) {
+                auto release = [&](int s, int i) {
                     umma_commit(bar(kBarRingEmpty + s));
-                    if (!shared_mode) umma_commit(bar(kBarRingEmpty + s));
+                    if (!shared_at(i)) umma_commit(bar(kBarRingEmpty + s));
                 };
                 // Loader order: K(A,0) K(B,0), then per step i: V(A,i) K(A,i+1) V(B,i) K(B,i+1).
-                uint32_t g = (n0 > 0 ? 1u : 0u) + (ln1 > 0 ? 1u : 0u);   // loads before step 0
-                const uint32_t pos_k0 = (t == 1 && !shared_mode) ? (n0 > 0 ? 1u : 0u) : 0u;
+                // Loads before step 0; under a window B's loads leave out the steps that the two share.
+                uint32_t g = (n0 > 0 ? 1u : 0u) + (ln1 > 0 && !(kWindow && shared_at(0)) ? 1u : 0u);
+                const uint32_t pos_k0 = (t == 1 && !shared_at(0)) ? (n0 > 0 ? 1u : 0u) : 0u;
                 if (!mbar_wait_warp(bar(kBarQFull + t), 0, abort_flag)) {
                     report_timeout(p.status, 1, static_cast<uint32_t>(warp), 0, 300 + t);
                     ok = false;
@@ -262,13 +345,22 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     tc_fence_after();
                     mma_tile_kk(tS, sQt, ring(slot_k), false);
                     umma_commit(bar(kBarSFull + t));
-                    release(slot_k);
+                    release(slot_k, 0);
                 }
                 for (int i = 0; i < nt && ok; ++i) {
-                    const uint32_t a_v = (i < n0), a_k = (i + 1 < n0), b_v = (i < ln1), b_k = (i + 1 < ln1);
-                    const bool own_a = t == 0 || shared_mode;
-                    const uint32_t pos_v = own_a ? g : g + a_v + a_k;
-                    const uint32_t pos_k = pos_v + 1;
+                    const uint32_t a_v = (i < n0), a_k = (i + 1 < n0);
+                    uint32_t b_v = (i < ln1), b_k = (i + 1 < ln1), pos_v, pos_k;
+                    if constexpr (kWindow) {
+                        const bool sv = shared_at(i), sk = shared_at(i + 1);
+                        b_v = b_v && !sv;
+                        b_k = b_k && !sk;
+                        pos_v = t == 0 || sv ? g : g + a_v + a_k;
+                        pos_k = t == 0 || sk ? g + a_v : g + a_v + a_k + b_v;
+                    } else {
+                        const bool own_a = t == 0 || shared_mode;
+                        pos_v = own_a ? g : g + a_v + a_k;
+                        pos_k = pos_v + 1;
+                    }
                     g += a_v + a_k + b_v + b_k;
                     const bool more = i + 1 < nt;
                     const int slot_v = wait_full(pos_v, 330 + t);
@@ -283,7 +375,7 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                 tc_fence_after();
                                 mma_tile_kk(tS, sQt, ring(slot_k), false);
                                 umma_commit(bar(kBarSFull + t));
-                                release(slot_k);
+                                release(slot_k, i + 1);
                             }
                             if (i < 64) FBA_TRACE_REC(p.status, 1024 + i * 8 + t * 4 + 1);
                         }
@@ -298,7 +390,7 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                     }
                     if (!ok) break;
                     umma_commit(bar(kBarPvDone + t));
-                    release(slot_v);
+                    release(slot_v, i);
                     if (i < 64) FBA_TRACE_REC(p.status, 1024 + i * 8 + t * 4 + 2);
                 }
             }
@@ -344,7 +436,21 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
             mbar_arrive(bar(kBarSLoaded + t));
             if (tracer && i < 64) FBA_TRACE_REC(p.status, i * 8 + t * 4 + 1);
 
-            if (p.list.msk != nullptr) {
+            if constexpr (kWindow) {
+                // Keys of this tile that the row sees: [lo, hi] and those below `sk`.
+                const int kb = kv_tile_of(t, i) * 128;
+                const int hi = mt * 128 + row + p.win.q_off - kb;
+                const int lo = hi - p.win.window + 1, sk = p.win.sinks - kb;
+                if (__any_sync(0xffffffffu, hi < 127 || (lo > 0 && sk < lo))) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {   // as a bit per key, 32 keys at a time
+                        const uint32_t keep = bits_below(hi + 1 - 32 * q) & (~bits_below(lo - 32 * q) | bits_below(sk - 32 * q));
+#pragma unroll
+                        for (int j = 0; j < 32; ++j)
+                            if (!((keep >> j) & 1u)) u[32 * q + j] = 0xff800000u;
+                    }
+                }
+            } else if (p.list.msk != nullptr) {
                 const uint32_t w = p.list.msk[lrow * p.list.stride + i / sub];
                 if (w != 0xffffu) {
                     const bool keep0 = (w >> g) & 1u, keep1 = (w >> (8 + g)) & 1u;
@@ -504,6 +610,48 @@ static int check_list(const fba_list_t* l, const char* who) {
     return FBA_OK;
 }
 
+// Launches the kernel over lists (q2k) or under a window (win); the arguments have been checked.
+static int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv, int Sq,
+                      int Skv, const fba_list_t* q2k, const WindowDev* win, float softmax_scale, uint32_t* status,
+                      cudaStream_t stream) {
+    int rc;
+    const int n_mtiles = (Sq + 127) / 128;
+    DeviceGuard guard;
+    if ((rc = guard.bind(q)) != FBA_OK) return rc;
+
+    CUtensorMap tm_q, tm_k, tm_v, tm_o;
+    if ((rc = make_tmap_bf16(&tm_q, q, Sq, static_cast<long long>(B) * Hq, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_k, k, Skv, static_cast<long long>(B) * Hkv, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_v, v, Skv, static_cast<long long>(B) * Hkv, 128)) != FBA_OK) return rc;
+    if ((rc = make_tmap_bf16(&tm_o, o, Sq, static_cast<long long>(B) * Hq, 128)) != FBA_OK) return rc;
+
+    auto kernel = win ? fba_fwd_kernel<true> : fba_fwd_kernel<false>;
+    {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             static_cast<int>(kFwdSmemBytes));
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return set_error(FBA_ERR_LAUNCH, "fba_fwd: cannot raise the dynamic shared memory limit");
+        }
+    }
+    FwdParams p;
+    p.list = win ? ListDev{} : to_dev(*q2k);
+    p.win = win ? *win : WindowDev{};
+    p.lse = lse;
+    p.status = status;
+    p.n_mtiles = n_mtiles;
+    p.Sq = Sq;
+    p.Hq = Hq;
+    p.Hkv = Hkv;
+    p.scale_log2 = softmax_scale * kLog2e;
+    dim3 grid((n_mtiles + 1) / 2, B * Hq);
+    timing_mark(1, true, stream);
+    kernel<<<grid, kFwdThreads, kFwdSmemBytes, stream>>>(tm_q, tm_k, tm_v, tm_o, p);
+    rc = check_launch("fba_fwd_kernel");
+    timing_mark(1, false, stream);
+    return rc;
+}
+
 static int fwd_impl(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq,
                     int Hkv, int Sq, int Skv, const fba_list_t* q2k, float softmax_scale, uint32_t* status,
                     void* stream_) {
@@ -532,38 +680,19 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
                          "fba_fwd: ceil(Skv/128) must be a multiple of q2k->sub and ceil(Sq/128) of q2k->rows_div");
     if (static_cast<long long>(B) * Hq > 65535)
         return set_error(FBA_ERR_TOO_LARGE, "fba_fwd: B * Hq exceeds 65535");
-    DeviceGuard guard;
-    if ((rc = guard.bind(q)) != FBA_OK) return rc;
+    return launch_fwd(q, k, v, o, lse, B, Hq, Hkv, Sq, Skv, q2k, nullptr, softmax_scale, status, stream);
+}
 
-    CUtensorMap tm_q, tm_k, tm_v, tm_o;
-    if ((rc = make_tmap_bf16(&tm_q, q, Sq, static_cast<long long>(B) * Hq, 128)) != FBA_OK) return rc;
-    if ((rc = make_tmap_bf16(&tm_k, k, Skv, static_cast<long long>(B) * Hkv, 128)) != FBA_OK) return rc;
-    if ((rc = make_tmap_bf16(&tm_v, v, Skv, static_cast<long long>(B) * Hkv, 128)) != FBA_OK) return rc;
-    if ((rc = make_tmap_bf16(&tm_o, o, Sq, static_cast<long long>(B) * Hq, 128)) != FBA_OK) return rc;
-
-    {
-        cudaError_t e = cudaFuncSetAttribute(fba_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(kFwdSmemBytes));
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return set_error(FBA_ERR_LAUNCH, "fba_fwd: cannot raise the dynamic shared memory limit");
-        }
-    }
-    FwdParams p;
-    p.list = to_dev(*q2k);
-    p.lse = lse;
-    p.status = status;
-    p.n_mtiles = n_mtiles;
-    p.Sq = Sq;
-    p.Hq = Hq;
-    p.Hkv = Hkv;
-    p.scale_log2 = softmax_scale * kLog2e;
-    dim3 grid((n_mtiles + 1) / 2, B * Hq);
-    timing_mark(1, true, stream);
-    fba_fwd_kernel<<<grid, kFwdThreads, kFwdSmemBytes, stream>>>(tm_q, tm_k, tm_v, tm_o, p);
-    rc = check_launch("fba_fwd_kernel");
-    timing_mark(1, false, stream);
-    return rc;
+extern "C" int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv,
+                              int Sq, int Skv, int window, int sinks, float softmax_scale, uint32_t* status,
+                              void* stream) {
+    ProfRange range("fba_window_fwd");
+    if (!q || !k || !v || !o || !status) return set_error(FBA_ERR_BAD_ARG, "fba_window_fwd: null pointer argument");
+    WindowDev win;
+    int rc = window_args("fba_window_fwd", B, Hq, Hkv, Sq, Skv, window, sinks, softmax_scale, &win);
+    if (rc != FBA_OK) return rc;
+    return launch_fwd(q, k, v, o, lse, B, Hq, Hkv, Sq, Skv, nullptr, &win, softmax_scale, status,
+                      static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int fba_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq,

@@ -46,13 +46,15 @@ class _StatusMonitor:
         self.pending = False
 
     def after_call(self) -> None:
+        if torch.cuda.is_current_stream_capturing():   # a replay writes the words; check_status() or a later call sees them
+            return
         self.host.copy_(self.buf, non_blocking=True)
         self.event.record(torch.cuda.current_stream(self.device))
         self.pending = True
 
     def poll(self) -> None:
         """Raise if a mirror copy that has already completed shows a timed-out wait."""
-        if self.pending and self.event.query():
+        if self.pending and not torch.cuda.is_current_stream_capturing() and self.event.query():
             self.pending = False
             if int(self.host[0]) != 0:
                 self.raise_from(self.host.tolist())
@@ -73,6 +75,8 @@ def _monitor(device: torch.device) -> _StatusMonitor:
     key = device.index if device.index is not None else torch.cuda.current_device()
     mon = _monitors.get(key)
     if mon is None:
+        if torch.cuda.is_current_stream_capturing():   # the words must not live in a graph's memory
+            raise RuntimeError("flex_block_attn_b200: make one call on this device before a stream capture")
         mon = _StatusMonitor(torch.device("cuda", key))
         _monitors[key] = mon
     return mon

@@ -290,6 +290,29 @@ int fba_bwd_split(const void* q, const void* k, const void* v, const void* o, co
                   uint32_t* status, void* stream);
 
 /*
+ * Causal attention under a sliding window with sinks (no counterpart in the reference).  The query of row i stands at
+ * position i + Skv - Sq (the last query and the last key are the same token's); it sees key j when
+ *     j <= position  and  (position - j < window  or  j < sinks).
+ * window = 0 means no limit (a causal mask; sinks then change nothing).  A row that sees no key (Sq > Skv: the first
+ * Sq - Skv rows) has a zero output row, lse = -inf and zero gradients.  Layouts and types are fba_fwd's, lengths from 1 to
+ * 2^29 rows; lse may be NULL in the forward.  No list is built: the kernels derive their tiles from the arguments, and read
+ * only tiles that hold visible pairs.  K and V must be finite: a NaN or infinity in a value row may also reach rows of
+ * the same 128-row tiles that do not see it (0 * inf in the product).
+ *
+ * Backward: scratch buffers as fba_bwd's (fba_bwd_scratch_bytes), and `partial`, 16-byte aligned, of
+ * fba_window_partial_bytes() bytes, at most 74 MB (0: NULL is accepted) for the fp32 dK / dV of the key tiles with sinks,
+ * which every query sees and whose steps are therefore divided over several CTAs.  dK and dV are reproducible bit by bit;
+ * dQ is summed in scheduling order, like fba_bwd's.
+ */
+int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv, int Sq,
+                   int Skv, int window, int sinks, float softmax_scale, uint32_t* status, void* stream);
+int fba_window_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks, uint64_t* bytes);
+int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
+                   void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks,
+                   float softmax_scale, float* lse_delta, float* dq_accum, float* partial, uint64_t partial_bytes,
+                   uint32_t* status, void* stream);
+
+/*
  * The reference extension's own call shape (reference attn.cpp:12-21 and
  * flex_block_attn_h100.cu:810-818, 1009-1021): q, k, v (+ o, lse, dO), the two block sizes, the bool
  * block mask(s) and use_small_block_mode in; o, lse / dq, dk, dv out.  Where the reference allocates
