@@ -18,6 +18,12 @@ from .interface import (  # noqa: F401
     ssta_lists,
     sta_lists,
 )
+from .paged import (  # noqa: F401
+    PagedKVCache,
+    append_kv,
+    new_paged_cache,
+    paged_decode_attn,
+)
 from .window import (  # noqa: F401
     SlidingWindowAttnFunc,
     backward_with_window,
@@ -42,6 +48,10 @@ __all__ = [
     "Fp8KVCache",
     "quantize_kv",
     "flex_block_attn_fp8kv",
+    "PagedKVCache",
+    "new_paged_cache",
+    "append_kv",
+    "paged_decode_attn",
     "sliding_window_attn_func",
     "SlidingWindowAttnFunc",
     "forward_with_window",

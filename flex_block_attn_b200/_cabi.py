@@ -14,6 +14,7 @@ from pathlib import Path
 _LIB = None
 FBA_ERR_TIMEOUT = -4
 FBA_ERR_TOO_LARGE = -5
+FBA_ERR_BAD_CACHE = -6
 LIB_PATH = Path(__file__).resolve().parent / "libfba_b200.so"
 
 EXPORTED_SYMBOLS = (
@@ -45,6 +46,9 @@ EXPORTED_SYMBOLS = (
     "fba_bwd_partial_bytes",
     "fba_bwd_split",
     "fba_set_bwd_kernel",
+    "fba_paged_append",
+    "fba_paged_decode_workspace_bytes",
+    "fba_paged_decode",
     "fba_window_fwd",
     "fba_window_partial_bytes",
     "fba_window_bwd",
@@ -77,6 +81,13 @@ class FbaList(ctypes.Structure):
     def __init__(self, idx=None, cnt=None, msk=None, stride=0, rows_per_bh=0, bh_stride=0, rows_div=1, sub=1,
                  order=None):
         super().__init__(idx, cnt, msk, stride, rows_per_bh, bh_stride, rows_div, sub, order)
+
+
+class FbaPaged(ctypes.Structure):
+    """Mirror of ``fba_paged_t``."""
+
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "weight", "position", "table")] + [
+        (n, ctypes.c_int32) for n in ("n_pages", "Hkv", "page_size", "max_pages", "e4m3")]
 
 
 def lib() -> ctypes.CDLL:
@@ -154,6 +165,14 @@ def lib() -> ctypes.CDLL:
                                                         vp, vp, vp, ctypes.c_uint64, vp, vp]
     L.fba_set_bwd_kernel.restype = i32
     L.fba_set_bwd_kernel.argtypes = [i32]
+    paged, strides = ctypes.POINTER(FbaPaged), ctypes.POINTER(ctypes.c_int64)
+    L.fba_paged_append.restype = i32
+    L.fba_paged_append.argtypes = [paged, vp, vp, strides, strides, i32, i32] + [vp] * 6
+    L.fba_paged_decode_workspace_bytes.restype = i32
+    L.fba_paged_decode_workspace_bytes.argtypes = [i32] * 6 + [ctypes.POINTER(ctypes.c_uint64)]
+    L.fba_paged_decode.restype = i32
+    L.fba_paged_decode.argtypes = [paged, vp, strides, vp, vp, i32, i32, vp, i32, i32, ctypes.c_float, i32, vp,
+                                   ctypes.c_uint64, vp, vp]
     L.fba_window_fwd.restype = i32
     L.fba_window_fwd.argtypes = [vp] * 5 + [i32] * 7 + [ctypes.c_float, vp, vp]
     L.fba_window_partial_bytes.restype = i32

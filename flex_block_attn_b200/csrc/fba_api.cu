@@ -205,6 +205,12 @@ extern "C" int fba_check_status(uint32_t* status, void* stream_) {
     if (w[StatusWords::kFlag] == 0) return FBA_OK;
     cudaMemsetAsync(status, 0, sizeof(w), stream);
     char buf[256];
+    if (w[StatusWords::kFlag] != 1) {   // PagedReport, fba_paged.cuh
+        snprintf(buf, sizeof(buf), "a paged cache was given %s %d for sequence %u; its rows were left out",
+                 w[StatusWords::kFlag] == 2 ? "the page number" : "the length", static_cast<int>(w[StatusWords::kTag]),
+                 w[StatusWords::kBx]);
+        return set_error(FBA_ERR_BAD_CACHE, buf);
+    }
     snprintf(buf, sizeof(buf),
              "a device-side wait timed out (kernel=%u role=%u block=(%u,%u) iter=%u tag=%u); the outputs of that "
              "call are undefined",

@@ -1,0 +1,832 @@
+// Paged key / value cache: the writer of new tokens and the attention of one new token per sequence.
+#include <math.h>
+#include <stdio.h>
+
+#include "fba_paged.cuh"
+
+namespace fba {
+
+// ------------------------------------------------------------------------------------------ writer
+struct AppendParams {
+    const __nv_bfloat16 *k, *v;
+    long long ks[3], vs[3];   // strides of batch, head and token, in elements
+    const int32_t *seq_lens, *new_lens, *positions;
+    int32_t* out_lens;
+    uint32_t* status;
+    int T;
+};
+
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// A half-warp per (token, kv head): 16 lanes x 16 bytes are one row of K, then the row of V.  Nothing is computed that
+// could hold the memory back: bound by the rows read and written.
+template <bool kE4m3>
+__global__ void __launch_bounds__(256) paged_append_kernel(const PagedDev c, const AppendParams p) {
+    const int b = blockIdx.y;
+    const int lane = threadIdx.x & 31, l16 = lane & 15;
+    const int start = paged_length(c, p.seq_lens, b, p.status);
+    const int room = c.max_pages * c.page_size - start;
+    int n = p.new_lens ? p.new_lens[b] : p.T;
+    if (n < 0 || n > p.T || n > room) {
+        if (threadIdx.x == 0 && blockIdx.x == 0) report_paged(p.status, kBadLength, b, n);
+        n = max(0, min(min(n, p.T), room));
+    }
+    if (p.out_lens && blockIdx.x == 0 && threadIdx.x == 0) p.out_lens[b] = start + n;
+    const int pos0 = p.positions ? p.positions[b] : start;
+    const int rows = n * c.Hkv;   // host-checked: T * Hkv < 2^31
+    for (int r = (blockIdx.x * 256 + threadIdx.x) >> 4; r < rows; r += gridDim.x * 16) {
+        const int t = r / c.Hkv, h = r - t * c.Hkv;
+        const long long dst = paged_row(c, b, h, start + t, p.status);
+        if (dst < 0) continue;
+        const uint4 kv[2] = {
+            reinterpret_cast<const uint4*>(p.k + b * p.ks[0] + h * p.ks[1] + t * p.ks[2])[l16],
+            reinterpret_cast<const uint4*>(p.v + b * p.vs[0] + h * p.vs[1] + t * p.vs[2])[l16]};
+        if (!kE4m3) {
+            reinterpret_cast<uint4*>(c.k)[dst * 16 + l16] = kv[0];
+            reinterpret_cast<uint4*>(c.v)[dst * 16 + l16] = kv[1];
+        } else {
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const __nv_bfloat162* x2 = reinterpret_cast<const __nv_bfloat162*>(&kv[z]);
+                float2 x[4];
+                float m = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[j] = __bfloat1622float2(x2[j]);
+                    m = max_nan(m, max_nan(fabsf(x[j].x), fabsf(x[j].y)));
+                }
+                const uint32_t half = 0xffffu << (lane & 16);   // both half-warps need not be in the loop
+#pragma unroll
+                for (int s = 8; s > 0; s >>= 1) m = max_nan(m, __shfl_xor_sync(half, m, s));
+                // The floor keeps 1 / scale finite; a row with a NaN or an infinity gets a NaN.
+                float scale = m > 0.f ? fmaxf(m * (1.f / 448.f), 1.17549435e-38f) : 1.f;
+                if (!(m < INFINITY)) scale = NAN;
+                const float inv = 1.f / scale;
+                const uint2 w = make_uint2(pack_e4m3x4(x[0].x * inv, x[0].y * inv, x[1].x * inv, x[1].y * inv),
+                                           pack_e4m3x4(x[2].x * inv, x[2].y * inv, x[3].x * inv, x[3].y * inv));
+                reinterpret_cast<uint2*>(z ? c.v : c.k)[dst * 16 + l16] = w;
+                if (l16 == 0) (z ? c.v_scale : c.k_scale)[dst] = scale;
+            }
+        }
+        if (c.weight && l16 == 0) {
+            c.weight[dst] = 0.f;
+            c.position[dst] = pos0 + t;
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------ decode
+//
+// The rows of a (sequence, kv head) are taken 16 at a time ("tiles", which never straddle a page).  All tiles of all
+// sequences form one list, which is cut into equal pieces, one per CTA; a CTA's piece may cover parts of several rows
+// ("row": sequence, kv head, group of at most 8 * NT of its query heads), and a row may be cut over several CTAs, whose
+// partial results (running maximum, sum, unnormalised output) a second kernel joins.
+//
+// In a CTA the four warps take the tiles in turn, each with a ring of its own in shared memory that cp.async fills several
+// tiles ahead, across the seams between rows; rows that the query does not see are filled with zeros instead of being
+// read.  With so few queries the time goes into reading K and V (per tile 8 KB in bf16, for 2 x 16 x 128 x 8
+// multiply-adds per 8 query heads), so the products run on the warp-level tensor instructions, keys as the 16 rows of
+// a tile and query heads as its 8 columns:
+//     S^T[16 keys x 8 heads] = K q^T,   O^T[128 x 8 heads] += V^T P^T,
+// with K and V^T through ldmatrix from a swizzled ring and P^T turned in registers (movmatrix).  The running maximum is
+// raised, and O^T rescaled, only when a score exceeds it by 2^8.  P is rounded to bf16 for its product like the prompt
+// kernels' P; sums and statistics are fp32.
+// e4m3: bytes become bf16 exactly (shifts and a multiplication by 2^120); a row's K scale multiplies its scores, its V
+// scale its probabilities.
+constexpr int kDecThreads = 128;
+constexpr int kTileKeys = 16;
+constexpr int kDecMinTiles = 16;      // tiles a CTA gets at least: 256 keys, four tiles a warp
+constexpr int kOStride = 132;         // floats between the heads of the exchange buffer (bank offset 4 a head)
+
+template <bool kE4m3>
+struct DecShape {
+    static constexpr int kRow = kE4m3 ? 128 : 256;                                     // bytes
+    static constexpr int kStage = 2 * kTileKeys * kRow + (kE4m3 ? 2 * kTileKeys * 4 : 0);   // K, V, scales
+    static constexpr int kStages = kE4m3 ? 5 : 3;
+    static constexpr int kRing = 4 * kStages * kStage;
+    static constexpr int kSmem = kRing + 4 * 8 * kOStride * 4 + 4 * 8 * 2 * 4 + 4 * 8 * 4;
+};
+static_assert(2 * (DecShape<false>::kSmem + 1024) <= 233472 && 2 * (DecShape<true>::kSmem + 1024) <= 233472,
+              "two CTAs of the decode kernel must fit into an SM's shared memory");
+
+struct DecodeParams {
+    const __nv_bfloat16* q;
+    long long qs[2];
+    __nv_bfloat16* o;
+    float* lse;
+    const int32_t* seq_lens;
+    uint32_t* status;
+    float* part_o;       // [slot][8 NT][128]
+    float* part_ml;      // [slot][8 NT][2]
+    float* scores;       // accumulate: [B, Hq, score_stride] in units of log2, else null
+    int score_stride;
+    int B, Hq, group, q_tiles;      // query heads a kv head; groups of 8 NT of them
+    int window, sinks;              // window 0: none
+    int n_ctas;                     // 0: one CTA per row, nothing to join
+    float scale_log2;
+};
+
+// A sequence's tiles: the first `sink_tiles`, then those from `first` on; nt in all.
+struct SeqTiles {
+    int n, sink_tiles, first, nt, lo;   // slots j < n with j < sinks or j >= lo are visible
+};
+__device__ __forceinline__ SeqTiles seq_tiles(int n, int window, int sinks) {
+    SeqTiles s;
+    s.n = n;
+    s.lo = window > 0 && window < n ? n - window : 0;
+    s.first = s.lo / kTileKeys;
+    s.sink_tiles = min(s.first, (sinks + kTileKeys - 1) / kTileKeys);
+    s.nt = s.sink_tiles + (n + kTileKeys - 1) / kTileKeys - s.first;
+    return s;
+}
+
+// Sum over the sequences of their tiles, and where tile `at` of the list [sequence][head row][tile] falls.  Every lane of
+// the warp takes part and gets the answers.
+struct ListPlace {
+    int b, before;   // the sequence, and how many tiles a head row of the sequences ahead of it has in all
+};
+__device__ __forceinline__ int list_total(const PagedDev& c, const DecodeParams& p) {
+    const int lane = threadIdx.x & 31;
+    int sum = 0;
+    for (int b = lane; b < p.B; b += 32) sum += seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks).nt;
+    return __reduce_add_sync(0xffffffffu, sum);
+}
+// The last sequence whose tiles begin at or before `at` (a place in one head row's concatenation, scaled by `rows`).
+__device__ __forceinline__ ListPlace list_find(const PagedDev& c, const DecodeParams& p, long long at, int rows) {
+    const int lane = threadIdx.x & 31;
+    ListPlace r = {0, 0};
+    int before = 0;
+    for (int base = 0; base < p.B; base += 32) {
+        const int b = base + lane;
+        const int nt = b < p.B ? seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks).nt : 0;
+        int upto = nt;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, s);
+            if (lane >= s) upto += x;
+        }
+        // sequences with tiles whose end lies behind `at`: the first of them is the place
+        const uint32_t hit = __ballot_sync(0xffffffffu, nt > 0 && static_cast<long long>(before + upto) * rows > at);
+        if (hit) {
+            const int first = __ffs(hit) - 1;
+            r.b = base + first;
+            r.before = before + __shfl_sync(0xffffffffu, upto - nt, first);
+            return r;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    r.b = p.B;
+    r.before = before;
+    return r;
+}
+// Tiles a CTA takes.
+__device__ __forceinline__ long long list_piece(long long total, int n_ctas) {
+    const long long per = (total + n_ctas - 1) / n_ctas;
+    return per < kDecMinTiles ? kDecMinTiles : per;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 8 x 8 matrix of 16-bit elements, turned.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+// D[16 x 8] += A[16 x 16] B[16 x 8], bf16.
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four e4m3 bytes -> two bf16 pairs, exactly: (bytes 0, 2) and (bytes 1, 3).  Sign and the seven other bits moved to
+// their places in bf16 read as the value times 2^-120 (exponent bias 127 instead of 7), subnormals included.  The one
+// pattern that this does not cover is NaN (0x7f, 0xff), which reads as 480.
+__device__ __forceinline__ void e4m3_to_bf16(uint32_t r, uint32_t& even, uint32_t& odd) {
+    const uint32_t e = ((r << 8) & 0x80008000u) | ((r << 4) & 0x07f007f0u);
+    const uint32_t o = (r & 0x80008000u) | ((r >> 4) & 0x07f007f0u);
+    constexpr uint32_t k2p120 = 0x7b807b80u;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(even) : "r"(e), "r"(k2p120));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(odd) : "r"(o), "r"(k2p120));
+}
+
+template <bool kE4m3, int NT>
+__global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const PagedDev c, const DecodeParams p) {
+    using Sh = DecShape<kE4m3>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t4 = lane & 3;
+    const uint32_t ring = smem_u32(smem) + warp * Sh::kStages * Sh::kStage;
+    float* ex_o = reinterpret_cast<float*>(smem + Sh::kRing);            // [warp][8][kOStride]
+    float* ex_ml = ex_o + 4 * 8 * kOStride;                              // [warp][8][2]
+    uint32_t* ring_vis = reinterpret_cast<uint32_t*>(ex_ml + 4 * 8 * 2) + warp * 8;   // [stage]: visible rows
+    const int rows_per_seq = c.Hkv * p.q_tiles;
+
+    // This CTA's piece: `left` tiles from tile `at` of row (b, hr) on.
+    struct Cursor {
+        int b, hr;           // sequence, head row (kv head * q_tiles + group)
+        int i, end;          // next tile of this warp in the row, and where the CTA's part of the row ends
+        long long left;      // tiles of the piece behind this row's part
+        SeqTiles s;
+    };
+    Cursor first;
+    if (p.n_ctas == 0) {
+        first.b = blockIdx.x / rows_per_seq;
+        first.hr = blockIdx.x - first.b * rows_per_seq;
+        first.s = seq_tiles(paged_length(c, p.seq_lens, first.b, p.status), p.window, p.sinks);
+        first.i = 0;
+        first.end = first.s.nt;
+        first.left = 0;
+    } else {
+        const long long total = static_cast<long long>(list_total(c, p)) * rows_per_seq;
+        const long long per = list_piece(total, p.n_ctas);
+        const long long at = per * blockIdx.x;
+        if (at >= total) return;
+        const ListPlace place = list_find(c, p, at, rows_per_seq);
+        first.b = place.b;
+        first.s = seq_tiles(paged_length(c, p.seq_lens, place.b, p.status), p.window, p.sinks);
+        const long long in = at - static_cast<long long>(place.before) * rows_per_seq;   // within the sequence
+        first.hr = static_cast<int>(in / first.s.nt);
+        first.i = static_cast<int>(in - static_cast<long long>(first.hr) * first.s.nt);
+        const long long mine = min(per, total - at);
+        first.end = static_cast<int>(min(static_cast<long long>(first.s.nt), first.i + mine));
+        first.left = mine - (first.end - first.i);
+    }
+    // The next row's part of the piece; the caller has checked that tiles are left.
+    auto next_row = [&](Cursor& r) {
+        if (++r.hr == rows_per_seq) {
+            r.hr = 0;
+            do {   // sequences without a tile have no part in the list; one with tiles follows, as tiles are left
+                ++r.b;
+                r.s = seq_tiles(paged_length(c, p.seq_lens, r.b, p.status), p.window, p.sinks);
+            } while (r.s.nt == 0);
+        }
+        r.i = 0;
+        r.end = static_cast<int>(min(static_cast<long long>(r.s.nt), r.left));
+        r.left -= r.end;
+    };
+    auto tile_slot = [&](const SeqTiles& s, int i) { return (i < s.sink_tiles ? i : s.first + i - s.sink_tiles) * kTileKeys; };
+    // Which of the 16 slots from j0 on are visible.
+    auto visible = [&](const SeqTiles& s, int j0) {
+        uint32_t m = j0 + 16 <= s.n ? 0xffffu : (1u << (s.n - j0)) - 1u;
+        if (j0 < s.lo) {
+            const int sk = p.sinks - j0, lo = s.lo - j0;
+            m &= (sk <= 0 ? 0u : sk >= 16 ? 0xffffu : (1u << sk) - 1u) | (lo >= 16 ? 0u : ~((1u << lo) - 1u));
+        }
+        return m;
+    };
+
+    // ---- loader: this warp's tiles, Sh::kStages - 1 ahead of the products
+    Cursor ld = first;
+    ld.i += warp;
+    int ld_pages = 0, ld_k = 32;       // page numbers of this warp's next tiles of the row, one per lane
+    bool ld_done = false;
+    auto load_next = [&](int stage) {
+        while (!ld_done && ld.i >= ld.end) {
+            if (ld.left == 0) {
+                ld_done = true;
+                break;
+            }
+            next_row(ld);
+            ld.i += warp;
+            ld_k = 32;
+        }
+        if (!ld_done) {
+            if (ld_k == 32) {   // the page numbers of the warp's next 32 tiles, a lane each
+                const int i = ld.i + 4 * lane;
+                ld_pages = i < ld.end ? c.table[static_cast<long long>(ld.b) * c.max_pages + (tile_slot(ld.s, i) >> c.page_shift)] : 0;
+                if (static_cast<uint32_t>(ld_pages) >= static_cast<uint32_t>(c.n_pages)) {
+                    report_paged(p.status, kBadPage, ld.b, ld_pages);
+                    ld_pages = -1;
+                }
+                ld_k = 0;
+            }
+            const int page = __shfl_sync(0xffffffffu, ld_pages, ld_k);
+            ++ld_k;
+            const int j0 = tile_slot(ld.s, ld.i);
+            const uint32_t vis = page < 0 ? 0u : visible(ld.s, j0);
+            if (lane == 0) ring_vis[stage] = vis;   // read behind the barrier that follows the stage's wait
+            const int h = ld.hr / p.q_tiles;
+            const long long row = (static_cast<long long>(max(page, 0)) * c.Hkv + h) * c.page_size + (j0 & (c.page_size - 1));
+            const uint32_t dst = ring + stage * Sh::kStage;
+            constexpr int kLanes = Sh::kRow / 16;                     // lanes a row
+            const int r0 = lane / kLanes, ch = lane % kLanes;
+#pragma unroll
+            for (int z = 0; z < 2; ++z) {
+                const uint8_t* src = (z ? c.v : c.k) + row * Sh::kRow + r0 * Sh::kRow + ch * 16;
+#pragma unroll
+                for (int it = 0; it < kTileKeys * kLanes / 32; ++it) {
+                    const int r = r0 + it * (32 / kLanes);
+                    cp_async16(dst + z * kTileKeys * Sh::kRow + r * Sh::kRow + ((ch ^ (r & 7)) << 4),
+                               src + it * (32 / kLanes) * Sh::kRow, (vis >> r) & 1u);
+                }
+            }
+            if (kE4m3 && lane < 8) {
+                const float* src = (lane < 4 ? c.k_scale : c.v_scale) + row + (lane & 3) * 4;
+                cp_async16(dst + 2 * kTileKeys * Sh::kRow + lane * 16, src, page >= 0);
+            }
+            ld.i += 4;
+        }
+        cp_async_commit();   // an empty group where nothing is left, so that the count of groups stays the stages'
+    };
+#pragma unroll
+    for (int s = 0; s < Sh::kStages - 1; ++s) load_next(s);
+
+    // ---- products
+    Cursor cur = first;
+    int stage = 0;
+    while (true) {
+        const int h = cur.hr / p.q_tiles, q0 = h * p.group + (cur.hr - h * p.q_tiles) * 8 * NT;   // first query head
+        const int heads = min(8 * NT, (h + 1) * p.group - q0);
+        // q as the right operand: of k-step ks thread (g, t4) holds head g, two dims and two more 8 further on; with
+        // e4m3 the dims follow the byte order of e4m3_to_bf16.
+        uint32_t qf[NT][16];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const bool real = 8 * nt + g < heads;
+            const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + cur.b * p.qs[0] + (q0 + (real ? 8 * nt + g : 0)) * p.qs[1]);
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {
+                if (kE4m3) {
+                    const uint32_t x = real ? src[ks * 8 + 2 * t4] : 0u, y = real ? src[ks * 8 + 2 * t4 + 1] : 0u;
+                    qf[nt][2 * ks] = __byte_perm(x, y, 0x5410);
+                    qf[nt][2 * ks + 1] = __byte_perm(x, y, 0x7632);
+                } else {
+                    qf[nt][2 * ks] = real ? src[ks * 8 + t4] : 0u;
+                    qf[nt][2 * ks + 1] = real ? src[ks * 8 + 4 + t4] : 0u;
+                }
+            }
+        }
+        float acc[NT][8][4];
+        float m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[nt][j][e] = 0.f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.f;
+        }
+        const int row_from = cur.i;
+        const bool whole = row_from == 0 && cur.end == cur.s.nt;   // nothing of the row is elsewhere
+        for (int i = row_from + warp; i < cur.end; i += 4) {
+            load_next(stage == 0 ? Sh::kStages - 1 : stage - 1);
+            cp_async_wait<Sh::kStages - 1>();
+            __syncwarp();
+            const uint32_t sk = ring + stage * Sh::kStage, sv = sk + kTileKeys * Sh::kRow;
+            const int j0 = tile_slot(cur.s, i);
+            float s[NT][4];
+            {
+                float s2[NT][2][4];   // two chains
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s2[nt][0][e] = s2[nt][1][e] = 0.f;
+                const uint32_t row = sk + (lane & 15) * Sh::kRow;
+                const uint32_t hi = lane >> 4, sw = lane & 7;
+                if (kE4m3) {
+#pragma unroll
+                    for (int ci = 0; ci < 4; ++ci) {
+                        uint32_t r[4], a[2][4];
+                        ldmatrix_x4(r, row + (((2 * ci + hi) ^ sw) << 4));
+                        e4m3_to_bf16(r[0], a[0][0], a[0][2]);
+                        e4m3_to_bf16(r[1], a[0][1], a[0][3]);
+                        e4m3_to_bf16(r[2], a[1][0], a[1][2]);
+                        e4m3_to_bf16(r[3], a[1][1], a[1][3]);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma_16816(s2[nt][0], a[0], qf[nt][4 * ci], qf[nt][4 * ci + 1]);
+                            mma_16816(s2[nt][1], a[1], qf[nt][4 * ci + 2], qf[nt][4 * ci + 3]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        uint32_t a[4];
+                        ldmatrix_x4(a, row + (((2 * ks + hi) ^ sw) << 4));
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) mma_16816(s2[nt][ks & 1], a, qf[nt][2 * ks], qf[nt][2 * ks + 1]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][0][e] + s2[nt][1][e];
+            }
+            // Elements: (key g, head 2 t4), (g, + 1), (key g + 8, 2 t4), (g + 8, + 1).
+            const uint32_t vis = ring_vis[stage];
+            float mul[2] = {p.scale_log2, p.scale_log2};
+            float vs[2] = {1.f, 1.f};
+            if (kE4m3) {
+                const float* sc = reinterpret_cast<const float*>(smem + (sk - smem_u32(smem)) + 2 * kTileKeys * Sh::kRow);
+                mul[0] *= sc[g];
+                mul[1] *= sc[g + 8];
+                vs[0] = (vis >> g) & 1u ? sc[16 + g] : 0.f;   // the scales are loaded for all rows, whatever they hold
+                vs[1] = (vis >> (g + 8)) & 1u ? sc[24 + g] : 0.f;
+            }
+            bool over = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    s[nt][e] = (vis >> (g + 8 * (e >> 1))) & 1u ? s[nt][e] * mul[e >> 1] : -INFINITY;
+                    over = over || s[nt][e] > m[nt][e & 1] + 8.f;
+                }
+            }
+            if (p.scores) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int hq = 8 * nt + 2 * t4 + (e & 1);
+                        if (hq < heads)
+                            p.scores[(static_cast<long long>(cur.b) * p.Hq + q0 + hq) * p.score_stride + j0 + g + 8 * (e >> 1)] = s[nt][e];
+                    }
+            }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        float mx = fmaxf(m[nt][x], fmaxf(s[nt][x], s[nt][x + 2]));
+#pragma unroll
+                        for (int sh = 4; sh < 32; sh <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, sh));
+                        const float alpha = mx == -INFINITY ? 1.f : ex2_approx(m[nt][x] - mx);
+                        m[nt][x] = mx;
+                        l[nt][x] *= alpha;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            acc[nt][j][x] *= alpha;
+                            acc[nt][j][x + 2] *= alpha;
+                        }
+                    }
+            }
+            uint32_t pb[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float e4[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float mm = m[nt][e & 1];
+                    e4[e] = ex2_approx(s[nt][e] - (mm == -INFINITY ? 0.f : mm));
+                    l[nt][e & 1] += e4[e];
+                    if (kE4m3) e4[e] *= vs[e >> 1];
+                }
+                pb[nt][0] = movmatrix(pack_bf16x2(e4[0], e4[1]));
+                pb[nt][1] = movmatrix(pack_bf16x2(e4[2], e4[3]));
+            }
+            if (kE4m3) {
+                const uint32_t row = sv + (lane & 15) * Sh::kRow;
+                const uint32_t hi = lane >> 4, sw = lane & 7;
+#pragma unroll
+                for (int ci = 0; ci < 4; ++ci) {
+                    uint32_t r[4], a[2][4];
+                    ldmatrix_x4_trans(r, row + (((2 * ci + hi) ^ sw) << 4));
+                    e4m3_to_bf16(r[0], a[0][0], a[0][1]);
+                    e4m3_to_bf16(r[1], a[0][2], a[0][3]);
+                    e4m3_to_bf16(r[2], a[1][0], a[1][1]);
+                    e4m3_to_bf16(r[3], a[1][2], a[1][3]);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma_16816(acc[nt][2 * ci], a[0], pb[nt][0], pb[nt][1]);
+                        mma_16816(acc[nt][2 * ci + 1], a[1], pb[nt][0], pb[nt][1]);
+                    }
+                }
+            } else {
+                const uint32_t row = sv + ((lane & 7) + ((lane >> 4) << 3)) * Sh::kRow;
+                const uint32_t hi = (lane >> 3) & 1, sw = lane & 7;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    uint32_t a[4];
+                    ldmatrix_x4_trans(a, row + (((2 * j + hi) ^ sw) << 4));
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_16816(acc[nt][j], a, pb[nt][0], pb[nt][1]);
+                }
+            }
+            __syncwarp();   // the stage may be filled again
+            stage = stage + 1 == Sh::kStages ? 0 : stage + 1;
+        }
+
+        // The four warps' parts of the row, eight heads at a time; thread = dim.
+        const int row_id = cur.b * rows_per_seq + cur.hr;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            if (8 * nt >= heads) break;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                float sum = l[nt][x];
+#pragma unroll
+                for (int sh = 4; sh < 32; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
+                if (g == 0) {
+                    ex_ml[(warp * 8 + 2 * t4 + x) * 2] = m[nt][x];
+                    ex_ml[(warp * 8 + 2 * t4 + x) * 2 + 1] = sum;
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    float* dst = ex_o + (warp * 8 + 2 * t4 + x) * kOStride + 16 * j;
+                    dst[kE4m3 ? 2 * g : g] = acc[nt][j][x];
+                    dst[kE4m3 ? 2 * g + 1 : g + 8] = acc[nt][j][x + 2];
+                }
+            }
+            __syncthreads();
+            const int d = threadIdx.x;
+            for (int hq = 0; hq < min(8, heads - 8 * nt); ++hq) {
+                float mw[4], top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) top = fmaxf(top, mw[w] = ex_ml[(w * 8 + hq) * 2]);
+                float sum = 0.f, o = 0.f;
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float a = top == -INFINITY ? 0.f : ex2_approx(mw[w] - top);
+                    sum = fmaf(a, ex_ml[(w * 8 + hq) * 2 + 1], sum);
+                    o = fmaf(a, ex_o[(w * 8 + hq) * kOStride + d], o);
+                }
+                if (whole) {
+                    const long long out = static_cast<long long>(cur.b) * p.Hq + q0 + 8 * nt + hq;
+                    p.o[out * 128 + d] = __float2bfloat16(sum > 0.f || isnan(sum) ? o / sum : 0.f);
+                    if (p.lse && d == 0) p.lse[out] = sum > 0.f || isnan(sum) ? (top + log2f(sum)) * kLn2 : -INFINITY;
+                } else {
+                    const long long slot = (static_cast<long long>(blockIdx.x) + row_id) * (8 * NT) + 8 * nt + hq;
+                    p.part_o[slot * 128 + d] = o;
+                    if (d == 0) {
+                        p.part_ml[slot * 2] = top;
+                        p.part_ml[slot * 2 + 1] = sum;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (cur.left == 0) break;
+        next_row(cur);
+    }
+    cp_async_wait<0>();
+}
+
+// Joins the parts of the rows that several CTAs share, gives the rows without a tile their zeros, and adds the
+// probabilities to the weights.  blockIdx.x = row, blockIdx.y = a stretch of its slots; thread = dim, then slot.
+template <int NT>
+__global__ void __launch_bounds__(128) paged_join_kernel(const PagedDev c, const DecodeParams p) {
+    __shared__ float s_lse[8 * NT];
+    const int rows_per_seq = c.Hkv * p.q_tiles;
+    const int b = blockIdx.x / rows_per_seq, hr = blockIdx.x - b * rows_per_seq;
+    const int h = hr / p.q_tiles, q0 = h * p.group + (hr - h * p.q_tiles) * 8 * NT;
+    const int heads = min(8 * NT, (h + 1) * p.group - q0);
+    const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
+    const int lane = threadIdx.x & 31;
+    int c0 = 0, c1 = -1;
+    bool whole = p.n_ctas == 0;
+    if (!whole && s.nt > 0) {
+        int ahead = 0, all = 0;   // tiles of the sequences before b, and of all
+        for (int x = lane; x < p.B; x += 32) {
+            const int nt = seq_tiles(paged_length(c, p.seq_lens, x, p.status), p.window, p.sinks).nt;
+            all += nt;
+            if (x < b) ahead += nt;
+        }
+        ahead = __reduce_add_sync(0xffffffffu, ahead);
+        all = __reduce_add_sync(0xffffffffu, all);
+        const long long per = list_piece(static_cast<long long>(all) * rows_per_seq, p.n_ctas);
+        const long long at = static_cast<long long>(ahead) * rows_per_seq + static_cast<long long>(hr) * s.nt;
+        c0 = static_cast<int>(at / per);
+        c1 = static_cast<int>((at + s.nt - 1) / per);
+        whole = c0 == c1;
+    }
+    const int d = threadIdx.x;
+    for (int hq = 0; hq < heads; ++hq) {
+        const long long out = static_cast<long long>(b) * p.Hq + q0 + hq;
+        if (whole && s.nt > 0) {
+            if (d == 0 && p.scores) s_lse[hq] = p.lse[out] * kLog2e;
+            continue;
+        }
+        float top = -INFINITY, sum = 0.f, o = 0.f;
+        for (int x = c0; x <= c1; ++x) {
+            const long long slot = (static_cast<long long>(x) + blockIdx.x) * (8 * NT) + hq;
+            const float m = p.part_ml[slot * 2], l = p.part_ml[slot * 2 + 1], v = p.part_o[slot * 128 + d];
+            const float now = fmaxf(top, m);
+            if (now == -INFINITY && !isnan(l)) continue;
+            const float keep = ex2_approx(top - now), take = ex2_approx(m - now);
+            sum = sum * keep + l * take;
+            o = o * keep + v * take;
+            top = now;
+        }
+        const bool some = sum > 0.f || isnan(sum);
+        if (blockIdx.y == 0) {
+            p.o[out * 128 + d] = __float2bfloat16(some ? o / sum : 0.f);
+            if (p.lse && d == 0) p.lse[out] = some ? (top + log2f(sum)) * kLn2 : -INFINITY;
+        }
+        if (d == 0) s_lse[hq] = top + log2f(sum);
+    }
+    if (p.scores == nullptr) return;
+    __syncthreads();
+    for (int j = blockIdx.y * 128 + threadIdx.x; j < s.n; j += gridDim.y * 128) {
+        const long long row = paged_row(c, b, h, j, p.status);
+        if (row < 0) continue;
+        float w = 0.f;
+        for (int hq = 0; hq < heads; ++hq)
+            w += ex2_approx(p.scores[(static_cast<long long>(b) * p.Hq + q0 + hq) * p.score_stride + j] - s_lse[hq]);
+        c.weight[row] += w;
+    }
+}
+
+int paged_args(const char* who, const fba_paged_t* cache, int B, PagedDev* dev) {
+    const char* why = nullptr;
+    int code = FBA_ERR_BAD_ARG;
+    const auto misaligned = [](const void* x) { return reinterpret_cast<uintptr_t>(x) % 16 != 0; };
+    if (!cache || !cache->k || !cache->v || !cache->table) why = "null pointer in the cache";
+    else if (B <= 0 || cache->n_pages <= 0 || cache->Hkv <= 0 || cache->max_pages <= 0) why = "non-positive size";
+    else if (cache->page_size < 16 || cache->page_size > 256 || (cache->page_size & (cache->page_size - 1)))
+        why = "page_size must be 16, 32, 64, 128 or 256";
+    else if (cache->e4m3 && (!cache->k_scale || !cache->v_scale)) why = "an e4m3 cache needs k_scale and v_scale";
+    else if (!cache->weight != !cache->position) why = "weight and position come together";
+    else if (misaligned(cache->k) || misaligned(cache->v) || misaligned(cache->k_scale) || misaligned(cache->v_scale))
+        why = "the pools must be 16-byte aligned";
+    else if (static_cast<long long>(cache->max_pages) * cache->page_size >= 1 << 30)
+        code = FBA_ERR_TOO_LARGE, why = "max_pages * page_size reaches 2^30";
+    else if (B > 65535) code = FBA_ERR_TOO_LARGE, why = "more than 65535 sequences";
+    if (why) {
+        char buf[160];
+        snprintf(buf, sizeof(buf), "%s: %s", who, why);
+        return set_error(code, buf);
+    }
+    int shift = 4;
+    while ((1 << shift) < cache->page_size) ++shift;
+    *dev = PagedDev{static_cast<uint8_t*>(cache->k), static_cast<uint8_t*>(cache->v), cache->e4m3 ? cache->k_scale : nullptr,
+                    cache->e4m3 ? cache->v_scale : nullptr, cache->weight, cache->position, cache->table, cache->n_pages,
+                    cache->Hkv, cache->page_size, shift, cache->max_pages};
+    return FBA_OK;
+}
+
+}  // namespace fba
+
+using namespace fba;
+
+extern "C" int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, const int64_t* k_strides,
+                                const int64_t* v_strides, int B, int T, const int32_t* seq_lens, const int32_t* new_lens,
+                                const int32_t* positions, int32_t* out_lens, uint32_t* status, void* stream) {
+    ProfRange range("fba_paged_append");
+    PagedDev c;
+    int rc = paged_args("fba_paged_append", cache, B, &c);
+    if (rc != FBA_OK) return rc;
+    if (!k || !v || !k_strides || !v_strides || !seq_lens || !status)
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: null pointer argument");
+    if (out_lens && out_lens == seq_lens)
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: out_lens must not be seq_lens");
+    if (T <= 0) return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: non-positive size");
+    if (static_cast<long long>(T) * c.Hkv > 0x7fffff00LL)
+        return set_error(FBA_ERR_TOO_LARGE, "fba_paged_append: more than 2^31 rows of a sequence");
+    if (reinterpret_cast<uintptr_t>(k) % 16 != 0 || reinterpret_cast<uintptr_t>(v) % 16 != 0)
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: k and v must be 16-byte aligned");
+    AppendParams p = {static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), {}, {}, seq_lens, new_lens,
+                      positions, out_lens, status, T};
+    for (int i = 0; i < 3; ++i) {
+        if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0)
+            return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: strides must be multiples of 8 elements");
+        p.ks[i] = k_strides[i];
+        p.vs[i] = v_strides[i];
+    }
+    DeviceGuard guard;
+    if ((rc = guard.bind(cache->k)) != FBA_OK) return rc;
+    const long long blocks = (static_cast<long long>(T) * c.Hkv + 15) / 16;   // 16 rows a block and step
+    const long long most = (148 * 16 + B - 1) / B;
+    dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most), B);
+    auto kernel = cache->e4m3 ? paged_append_kernel<true> : paged_append_kernel<false>;
+    kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(c, p);
+    return check_launch("paged_append_kernel");
+}
+
+namespace {
+// How a decode call is cut up.
+struct DecodePlan {
+    int nt, q_tiles, n_ctas, score_stride;
+    long long rows;
+    uint64_t part_o, part_ml, scores;   // bytes of the workspace, each rounded up to 256
+};
+DecodePlan decode_plan(int B, int Hq, int Hkv, int page_size, int max_pages, bool accumulate) {
+    DecodePlan d;
+    const int group = Hq / Hkv;
+    d.nt = group > 8 ? 2 : 1;
+    d.q_tiles = (group + 8 * d.nt - 1) / (8 * d.nt);
+    d.rows = static_cast<long long>(B) * Hkv * d.q_tiles;
+    const long long tiles = static_cast<long long>(max_pages) * page_size / kTileKeys;   // a row has at most
+    // One CTA per row where a row is short: nothing is joined then.  Otherwise as many as are resident.
+    const long long pieces = (d.rows * tiles + kDecMinTiles - 1) / kDecMinTiles;
+    d.n_ctas = tiles <= 2 * kDecMinTiles ? 0 : static_cast<int>(pieces < 2 * 148 ? pieces : 2 * 148);
+    auto up = [](uint64_t n) { return (n + 255) / 256 * 256; };
+    const uint64_t slots = d.n_ctas ? (d.n_ctas + d.rows) * 8 * d.nt : 0;
+    d.part_o = up(slots * 128 * sizeof(float));
+    d.part_ml = up(slots * 2 * sizeof(float));
+    d.score_stride = static_cast<int>(tiles * kTileKeys);
+    d.scores = accumulate ? up(static_cast<uint64_t>(B) * Hq * d.score_stride * sizeof(float)) : 0;
+    return d;
+}
+template <bool kE4m3, int NT>
+int launch_decode(const PagedDev& c, const DecodeParams& p, const DecodePlan& d, bool join, cudaStream_t stream) {
+    constexpr int smem = DecShape<kE4m3>::kSmem;
+    if (cudaFuncSetAttribute(paged_decode_kernel<kE4m3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
+        cudaGetLastError();
+        return set_error(FBA_ERR_LAUNCH, "fba_paged_decode: cannot raise the dynamic shared memory limit");
+    }
+    paged_decode_kernel<kE4m3, NT><<<d.n_ctas ? d.n_ctas : static_cast<unsigned>(d.rows), kDecThreads, smem, stream>>>(c, p);
+    int rc = check_launch("paged_decode_kernel");
+    if (rc != FBA_OK || !join) return rc;
+    int stretches = 1;
+    if (p.scores) stretches = static_cast<int>(min(64ll, (d.score_stride + 511ll) / 512));
+    paged_join_kernel<NT><<<dim3(static_cast<unsigned>(d.rows), stretches), 128, 0, stream>>>(c, p);
+    return check_launch("paged_join_kernel");
+}
+}  // namespace
+
+static int decode_args(const char* who, int B, int Hq, int Hkv, int page_size, int max_pages) {
+    if (B <= 0 || Hq <= 0 || Hkv <= 0 || page_size <= 0 || max_pages <= 0 || Hq % Hkv != 0)
+        return set_error(FBA_ERR_BAD_ARG, who);
+    if (static_cast<long long>(B) * Hq > 1 << 24) return set_error(FBA_ERR_TOO_LARGE, who);
+    if (static_cast<long long>(max_pages) * page_size >= 1 << 30 ||   // tiles of all sequences are counted in 31 bits
+        static_cast<long long>(B) * max_pages * page_size / kTileKeys >= 1ll << 31)
+        return set_error(FBA_ERR_TOO_LARGE, who);
+    return FBA_OK;
+}
+
+extern "C" int fba_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages, int accumulate,
+                                                uint64_t* bytes) {
+    const int rc = decode_args("fba_paged_decode_workspace_bytes: bad size", B, Hq, Hkv, page_size, max_pages);
+    if (rc != FBA_OK) return rc;
+    if (!bytes) return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode_workspace_bytes: null pointer argument");
+    const DecodePlan d = decode_plan(B, Hq, Hkv, page_size, max_pages, accumulate != 0);
+    *bytes = d.part_o + d.part_ml + d.scores;
+    return FBA_OK;
+}
+
+extern "C" int fba_paged_decode(const fba_paged_t* cache, const void* q, const int64_t* q_strides, void* o, float* lse, int B,
+                                int Hq, const int32_t* seq_lens, int window, int sinks, float softmax_scale, int accumulate,
+                                void* workspace, uint64_t workspace_bytes, uint32_t* status, void* stream_) {
+    ProfRange range("fba_paged_decode");
+    cudaStream_t stream = static_cast<cudaStream_t>(stream_);
+    PagedDev c;
+    int rc = paged_args("fba_paged_decode", cache, B, &c);
+    if (rc != FBA_OK) return rc;
+    if (!q || !q_strides || !o || !seq_lens || !status)
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: null pointer argument");
+    rc = decode_args("fba_paged_decode: bad size, or Hq not a multiple of Hkv", B, Hq, c.Hkv, c.page_size, c.max_pages);
+    if (rc != FBA_OK) return rc;
+    if (window < 0 || sinks < 0) return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: window and sinks must not be negative");
+    if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY))
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: softmax_scale must be positive and finite");
+    if (accumulate && (!c.weight || window != 0 || !lse))
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: accumulation needs a cache with weights, lse, and no window");
+    if (accumulate && Hq / c.Hkv > 16)
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: accumulation takes at most 16 query heads a kv head");
+    if (reinterpret_cast<uintptr_t>(q) % 4 != 0 || q_strides[0] % 2 != 0 || q_strides[1] % 2 != 0)
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: q must be 4-byte aligned, its strides multiples of 2");
+    const DecodePlan d = decode_plan(B, Hq, c.Hkv, c.page_size, c.max_pages, accumulate != 0);
+    const uint64_t need = d.part_o + d.part_ml + d.scores;
+    if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
+        return set_error(FBA_ERR_BAD_ARG,
+                         "fba_paged_decode: workspace must be 256-byte aligned, of fba_paged_decode_workspace_bytes() bytes");
+    if (d.rows > 0x7fffffffLL) return set_error(FBA_ERR_TOO_LARGE, "fba_paged_decode: more than 2^31 rows");
+    DeviceGuard guard;
+    if ((rc = guard.bind(cache->k)) != FBA_OK) return rc;
+
+    DecodeParams p = {};
+    p.q = static_cast<const __nv_bfloat16*>(q);
+    p.qs[0] = q_strides[0];
+    p.qs[1] = q_strides[1];
+    p.o = static_cast<__nv_bfloat16*>(o);
+    p.lse = lse;
+    p.seq_lens = seq_lens;
+    p.status = status;
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    p.part_o = reinterpret_cast<float*>(ws);
+    p.part_ml = reinterpret_cast<float*>(ws + d.part_o);
+    p.scores = accumulate ? reinterpret_cast<float*>(ws + d.part_o + d.part_ml) : nullptr;
+    p.score_stride = d.score_stride;
+    p.B = B;
+    p.Hq = Hq;
+    p.group = Hq / c.Hkv;
+    p.q_tiles = d.q_tiles;
+    p.window = window;
+    p.sinks = sinks;
+    p.n_ctas = d.n_ctas;
+    p.scale_log2 = softmax_scale * kLog2e;
+    const bool join = d.n_ctas != 0 || accumulate;
+    if (cache->e4m3) return d.nt == 1 ? launch_decode<true, 1>(c, p, d, join, stream) : launch_decode<true, 2>(c, p, d, join, stream);
+    return d.nt == 1 ? launch_decode<false, 1>(c, p, d, join, stream) : launch_decode<false, 2>(c, p, d, join, stream);
+}

@@ -1,0 +1,47 @@
+// What the kernels of the paged key / value cache share.
+#pragma once
+#include "fba_common.cuh"
+
+namespace fba {
+
+// Device view of fba_paged_t.
+struct PagedDev {
+    uint8_t *k, *v;              // [n_pages, Hkv, page_size, 128] bf16 or e4m3
+    float *k_scale, *v_scale;    // [n_pages, Hkv, page_size]; null unless e4m3
+    float* weight;               // likewise, or null
+    int32_t* position;           // likewise, or null
+    const int32_t* table;        // [B, max_pages]
+    int n_pages, Hkv, page_size, page_shift, max_pages;
+};
+
+// First of the status words: what is reported there.
+enum PagedReport : uint32_t { kBadPage = 2, kBadLength = 3 };
+__device__ __forceinline__ void report_paged(uint32_t* status, uint32_t what, int b, int value) {
+    if (atomicCAS(status + StatusWords::kFlag, 0u, what) == 0u) {
+        status[StatusWords::kBx] = static_cast<uint32_t>(b);
+        status[StatusWords::kTag] = static_cast<uint32_t>(value);
+    }
+}
+
+// Length of sequence b, held to what its row of the table can address.
+__device__ __forceinline__ int paged_length(const PagedDev& c, const int32_t* seq_lens, int b, uint32_t* status) {
+    const int n = seq_lens[b], most = c.max_pages * c.page_size;   // host-checked to stay below 2^31
+    if (n >= 0 && n <= most) return n;
+    report_paged(status, kBadLength, b, n);
+    return n < 0 ? 0 : most;
+}
+
+// Row of the pools that slot `slot` of sequence b and kv head h lives in, or -1 when the table names no page there.
+__device__ __forceinline__ long long paged_row(const PagedDev& c, int b, int h, int slot, uint32_t* status) {
+    const int page = c.table[static_cast<long long>(b) * c.max_pages + (slot >> c.page_shift)];
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.n_pages)) {
+        report_paged(status, kBadPage, b, page);
+        return -1;
+    }
+    return (static_cast<long long>(page) * c.Hkv + h) * c.page_size + (slot & (c.page_size - 1));
+}
+
+// Checks a cache and fills its device view (fba_paged.cu).
+int paged_args(const char* who, const fba_paged_t* cache, int B, PagedDev* dev);
+
+}  // namespace fba

@@ -62,6 +62,10 @@ class _StatusMonitor:
     def raise_from(self, words) -> None:
         self.buf.zero_()
         self.host.zero_()
+        if words[0] != 1:
+            raise RuntimeError(
+                "flex_block_attn_b200: a paged cache was given the "
+                f"{'page number' if words[0] == 2 else 'length'} {words[6]} for sequence {words[3]}; its rows were left out")
         raise RuntimeError(
             "flex_block_attn_b200: a device-side wait timed out; the outputs of that call are undefined "
             f"(kernel={words[1]} role={words[2]} block=({words[3]},{words[4]}) iter={words[5]} tag={words[6]})"
@@ -97,7 +101,7 @@ def check_status(device: Optional[torch.device] = None) -> None:
     mon = _monitor(device)
     rc = _cabi.lib().fba_check_status(mon.buf.data_ptr(), _stream_ptr(device))
     mon.pending = False
-    if rc == _cabi.FBA_ERR_TIMEOUT:
+    if rc in (_cabi.FBA_ERR_TIMEOUT, _cabi.FBA_ERR_BAD_CACHE):
         mon.host.zero_()
         raise RuntimeError("flex_block_attn_b200: " + _cabi.lib().fba_last_error().decode("utf-8", "replace"))
     _cabi.check(rc, "fba_check_status")

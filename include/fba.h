@@ -61,6 +61,7 @@ extern "C" {
 #define FBA_ERR_DRIVER (-3)         /* could not resolve / run cuTensorMapEncodeTiled */
 #define FBA_ERR_TIMEOUT (-4)        /* a bounded device-side wait gave up (see status words) */
 #define FBA_ERR_TOO_LARGE (-5)      /* problem exceeds a documented fixed limit */
+#define FBA_ERR_BAD_CACHE (-6)      /* a kernel met a page number or a length that the paged cache does not have */
 
 typedef struct fba_list {
     const int32_t* idx;   /* [rows_total, stride] */
@@ -311,6 +312,64 @@ int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, c
                    void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks,
                    float softmax_scale, float* lse_delta, float* dq_accum, float* partial, uint64_t partial_bytes,
                    uint32_t* status, void* stream);
+
+/*
+ * Paged key / value cache (no counterpart in the reference): a pool of pages of `page_size` rows per kv head that
+ * sequences of any length take theirs from.  Slot s of sequence b is row s % page_size of page
+ * table[b * max_pages + s / page_size].  The entry points below take it as this struct:
+ *   k, v         [n_pages, Hkv, page_size, 128] bf16, or e4m3 when `e4m3` is not 0; 16-byte aligned
+ *   k_scale, v_scale   fp32 [n_pages, Hkv, page_size], one scale per row (e4m3 only, else NULL); 16-byte aligned
+ *   weight       fp32 [n_pages, Hkv, page_size]: attention weight that the token in a slot has received, or NULL
+ *   position     int32, likewise: the token's place in its sequence, or NULL (both or neither)
+ *   table        int32 [B, max_pages], page numbers; entries behind a sequence's last page are not read
+ *   page_size    16, 32, 64, 128 or 256; max_pages * page_size < 2^30
+ * Lengths (`seq_lens`, int32 [B]) are read on the device.  A page number outside 0 .. n_pages - 1, or a length outside
+ * 0 .. max_pages * page_size, is never followed: the kernel leaves out the rows concerned (holds the length to the limit)
+ * and reports it in the status words; fba_check_status() then returns FBA_ERR_BAD_CACHE.  Pages that a call writes must
+ * belong to one sequence only; pages that are read may be shared.
+ */
+typedef struct fba_paged {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    float* weight;
+    int32_t* position;
+    const int32_t* table;
+    int32_t n_pages, Hkv, page_size, max_pages;
+    int32_t e4m3;
+} fba_paged_t;
+
+/*
+ * Write new tokens behind the sequences' ends: token t < new_lens[b] (NULL: T) of sequence b goes to slot
+ * seq_lens[b] + t.  k, v: bf16, element (b, h, t, d) at b * stride[0] + h * stride[1] + t * stride[2] + d, strides in
+ * elements and multiples of 8, bases 16-byte aligned.  e4m3: per row scale = max(max|x| * fp32(1/448), 2^-126) (1 for an
+ * all-zero row, NaN for a row with a NaN or an infinity), byte = e4m3(x * (1 / scale)), round to nearest even.  With weight / position: 0 and positions[b] + t
+ * (NULL: the slot).  out_lens (NULL, or int32 [B], not seq_lens itself) receives seq_lens[b] + new_lens[b].  Tokens that do not fit
+ * into the table's row are left out, with the report above, and not counted.
+ */
+int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, const int64_t* k_strides,
+                     const int64_t* v_strides, int B, int T, const int32_t* seq_lens, const int32_t* new_lens,
+                     const int32_t* positions, int32_t* out_lens, uint32_t* status, void* stream);
+
+/*
+ * Attention of one new token per sequence over its cached rows, the token's own (the last) among them:
+ *   o[b, h] = softmax(softmax_scale * q[b, h] . K) V over the slots j < n = seq_lens[b] with n - 1 - j < window or
+ *   j < sinks (window 0: all).  q, o: bf16 [B, Hq, 128], q element (b, h, d) at b * q_strides[0] + h * q_strides[1] + d
+ *   (multiples of 2), o contiguous; lse fp32 [B, Hq] or NULL.  n = 0: zeros, lse = -inf.
+ * Rows outside what a query sees are not read: whatever they hold, NaN included, does not matter.
+ * e4m3: a row stands for byte values times its scale; the NaN bytes 0x7f and 0xff read as 480 and -480 (a row that is not
+ * finite is marked by its scale).
+ * accumulate != 0 (window 0, lse not NULL, at most 16 query heads a kv head): weight[slot] += the sum of the slot's
+ * probabilities over the query heads of its kv head, in a fixed order.
+ * The tiles of all sequences are divided evenly over the SMs; parts of one sequence are joined by a second kernel
+ * through `workspace` (256-byte aligned, fba_paged_decode_workspace_bytes()).  Results do not depend on the order in which
+ * CTAs run.  They may differ in the last bit with the other sequences' lengths, which move the seams.
+ */
+int fba_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages, int accumulate, uint64_t* bytes);
+int fba_paged_decode(const fba_paged_t* cache, const void* q, const int64_t* q_strides, void* o, float* lse, int B, int Hq,
+                     const int32_t* seq_lens, int window, int sinks, float softmax_scale, int accumulate, void* workspace,
+                     uint64_t workspace_bytes, uint32_t* status, void* stream);
 
 /*
  * The reference extension's own call shape (reference attn.cpp:12-21 and

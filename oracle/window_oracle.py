@@ -38,3 +38,48 @@ def masked_attention(q, k, v, mask, dout=None, softmax_scale: Optional[float] = 
     dq = ds @ k[:, :, None]
     dk = (ds.transpose(-1, -2) @ qg).sum(2)
     return o.reshape(q.shape), lse.reshape(B, Hq, Sq), dq.reshape(q.shape), dk, dv
+
+
+# ------------------------------------------------------------------------------------------------------- paged cache
+def quantize_rows(x: torch.Tensor):
+    """(e4m3 bytes, fp32 scales) of bf16 rows, as the cache writer defines them."""
+    x = x.float()
+    most = x.abs().amax(-1)
+    scale = torch.where(most > 0, (most * torch.tensor(1 / 448, dtype=torch.float32)).clamp_min(2.0**-126), torch.ones(()))
+    bad = ~torch.isfinite(x).all(-1)
+    scale = torch.where(bad, torch.full((), math.nan), scale)
+    return (x * (1.0 / scale)[..., None]).to(torch.float8_e4m3fn).view(torch.uint8), scale
+
+
+def rows_of(pool: torch.Tensor, table_row, n: int, h: int) -> torch.Tensor:
+    """The first n rows of a sequence for kv head h, in slot order: plain loop over its pages."""
+    size = pool.shape[2]
+    pages = [int(p) for p in table_row[: -(-n // size)]]
+    got = [pool[p, h] for p in pages]
+    return torch.cat(got)[:n] if got else pool[0, 0][:0]
+
+
+def decode(q, pools, table, lens, window: Optional[int] = None, sinks: int = 0, softmax_scale: Optional[float] = None):
+    """(o, lse, weight per sequence: list of [Hkv, n]) in 64 bits; ``pools``: dict of CPU tensors, k, v and scales."""
+    B, Hq, D = q.shape
+    Hkv = pools["k"].shape[1]
+    G = Hq // Hkv
+    scale = 1 / math.sqrt(D) if softmax_scale is None else softmax_scale
+    o, lse, weight = torch.zeros((B, Hq, D), dtype=torch.float64), torch.full((B, Hq), -math.inf, dtype=torch.float64), []
+    for b, n in enumerate(int(x) for x in lens):
+        w = torch.zeros((Hkv, n), dtype=torch.float64)
+        j = torch.arange(n)
+        vis = torch.ones(n, dtype=torch.bool) if window is None else (n - 1 - j < window) | (j < sinks)
+        for h in range(Hkv if n else 0):
+            k, v = (rows_of(pools[x], table[b], n, h) for x in "kv")
+            if k.dtype == torch.uint8:
+                k, v = (x.view(torch.float8_e4m3fn).double() * rows_of(pools[s], table[b], n, h).double()[:, None]
+                        for x, s in ((k, "k_scale"), (v, "v_scale")))
+            k, v = k.double()[vis], v.double()[vis]
+            s = q[b, h * G:(h + 1) * G].double() @ k.T * scale
+            lse[b, h * G:(h + 1) * G] = torch.logsumexp(s, -1)
+            p = s.softmax(-1)
+            o[b, h * G:(h + 1) * G] = p @ v
+            w[h, vis] = p.sum(0)
+        weight.append(w)
+    return o, lse, weight
