@@ -49,6 +49,8 @@ EXPORTED_SYMBOLS = (
     "fba_paged_append",
     "fba_paged_decode_workspace_bytes",
     "fba_paged_decode",
+    "fba_paged_evict_workspace_bytes",
+    "fba_paged_evict",
     "fba_window_fwd",
     "fba_window_partial_bytes",
     "fba_window_bwd",
@@ -173,6 +175,10 @@ def lib() -> ctypes.CDLL:
     L.fba_paged_decode.restype = i32
     L.fba_paged_decode.argtypes = [paged, vp, strides, vp, vp, i32, i32, vp, i32, i32, ctypes.c_float, i32, vp,
                                    ctypes.c_uint64, vp, vp]
+    L.fba_paged_evict_workspace_bytes.restype = i32
+    L.fba_paged_evict_workspace_bytes.argtypes = [i32] * 5 + [ctypes.POINTER(ctypes.c_uint64)]
+    L.fba_paged_evict.restype = i32
+    L.fba_paged_evict.argtypes = [paged, i32, vp, i32, i32, i32, vp, vp, i32, vp, vp, ctypes.c_uint64, vp, vp]
     L.fba_window_fwd.restype = i32
     L.fba_window_fwd.argtypes = [vp] * 5 + [i32] * 7 + [ctypes.c_float, vp, vp]
     L.fba_window_partial_bytes.restype = i32

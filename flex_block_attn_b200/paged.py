@@ -1,4 +1,4 @@
-"""Paged key / value cache: the writer of new tokens and the attention of one new token per sequence.
+"""Paged key / value cache: the writer of new tokens, the attention of one new token per sequence, and eviction.
 
 No counterpart in the reference.  A pool of pages holds the keys and values of all sequences; slot s of sequence b is row
 ``s % page_size`` of page ``block_table[b, s // page_size]``.  Page tables and lengths are read on the device, so the calls
@@ -190,3 +190,42 @@ def paged_decode_attn(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
                               _status(dev).data_ptr(), _stream_ptr(dev))
     _check(rc, "fba_paged_decode", dev)
     return (o, lse) if need_lse else o
+
+
+def evict_kv(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Tensor, budget: int, sinks: int = 0,
+             recent: int = 0, next_positions: Optional[torch.Tensor] = None,
+             out_table: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Cut sequences to at most ``budget`` tokens by the attention weight they have received; returns the new lengths.
+
+    Every kv head drops, of its n tokens, the n - budget with the least ``cache.weight`` (of equal ones the lowest slots)
+    that are not protected: the first ``sinks`` positions and the last ``recent`` ones stay (sinks + recent <= budget).
+    ``next_positions``: int32 [B], how many tokens the sequences have seen; None = seq_lens (never cut before).
+
+    In place, the staying tokens behind the budget move to the slots that came free before it: the slots are then in no
+    order of positions (``cache.position`` keeps them), the pages from ``ceil(budget / page_size)`` on are free, and
+    ``paged_decode_attn`` goes on without a window.  With ``out_table`` (int32 [B, pages], pages that ``block_table`` does not
+    name) the staying tokens are copied there in slot order instead, and the source, which others may share, is left.
+    """
+    arg, B = _cache_arg(cache, block_table)
+    dev = cache.k.device
+    if cache.weight is None:
+        raise ValueError("evict_kv needs a cache with weights (new_paged_cache(..., track=True))")
+    for name, x, least in (("budget", budget, 1), ("sinks", sinks, 0), ("recent", recent, 0)):
+        if isinstance(x, bool) or not isinstance(x, int) or not least <= x < 2**31:
+            raise ValueError(f"{name} must be an integer from {least} on")
+    if sinks + recent > budget:
+        raise ValueError("sinks + recent must not exceed budget")
+    lens = _i32("seq_lens", seq_lens, (B,), dev)
+    nxt = None if next_positions is None else _i32("next_positions", next_positions, (B,), dev)
+    to = None if out_table is None else _i32("out_table", out_table, (B, None), dev)
+    lib = _cabi.lib()
+    n = ctypes.c_uint64(0)
+    _cabi.check(lib.fba_paged_evict_workspace_bytes(B, arg.Hkv, arg.page_size, arg.max_pages, budget, ctypes.byref(n)),
+                "fba_paged_evict_workspace_bytes")
+    ws = torch.empty((n.value,), dtype=torch.uint8, device=dev)
+    out = torch.empty_like(seq_lens)
+    rc = lib.fba_paged_evict(ctypes.byref(arg), B, lens, budget, sinks, recent, nxt, to,
+                             0 if out_table is None else out_table.shape[1], out.data_ptr(), ws.data_ptr(), n.value,
+                             _status(dev).data_ptr(), _stream_ptr(dev))
+    _check(rc, "fba_paged_evict", dev)
+    return out

@@ -372,6 +372,25 @@ int fba_paged_decode(const fba_paged_t* cache, const void* q, const int64_t* q_s
                      uint64_t workspace_bytes, uint32_t* status, void* stream);
 
 /*
+ * Cut sequences to at most `budget` (> 0) slots, for every kv head by itself: of the n = seq_lens[b] tokens the n - budget leave
+ * that come first by (weight, slot), among those that are not protected.  Protected are tokens with position < sinks and
+ * those with position >= next_positions[b] - recent (NULL: n - recent); sinks + recent <= budget.  A NaN weight counts as
+ * the largest.  (Should more than `budget` positions be protected all the same, the lowest slots of them leave.)
+ * out_lens[b] (not seq_lens itself) = min(n, budget).
+ *   out_table NULL: in place.  A token that stays keeps its slot if that is below the budget; the others that stay go, in
+ *     slot order, to the slots below the budget that came free, in slot order.  Slots from the budget on keep what they
+ *     hold.  The slots are in no order of positions afterwards; attention does not depend on it.
+ *   out_table int32 [B, out_pages]: the tokens that stay are copied in slot order to slots 0, 1, ... of that table (all n
+ *     where n <= budget), whose pages must not be among those that `table` names; the source is left as it is.
+ * K, V, scales, weights and positions move together.  workspace: 4-byte aligned, fba_paged_evict_workspace_bytes() bytes.
+ * The result does not depend on timing.
+ */
+int fba_paged_evict_workspace_bytes(int B, int Hkv, int page_size, int max_pages, int budget, uint64_t* bytes);
+int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* seq_lens, int budget, int sinks, int recent,
+                    const int32_t* next_positions, const int32_t* out_table, int out_pages, int32_t* out_lens,
+                    void* workspace, uint64_t workspace_bytes, uint32_t* status, void* stream);
+
+/*
  * The reference extension's own call shape (reference attn.cpp:12-21 and
  * flex_block_attn_h100.cu:810-818, 1009-1021): q, k, v (+ o, lse, dO), the two block sizes, the bool
  * block mask(s) and use_small_block_mode in; o, lse / dq, dk, dv out.  Where the reference allocates

@@ -83,3 +83,32 @@ def decode(q, pools, table, lens, window: Optional[int] = None, sinks: int = 0, 
             w[h, vis] = p.sum(0)
         weight.append(w)
     return o, lse, weight
+
+
+def evict(pools, table, lens, budget: int, sinks: int = 0, recent: int = 0, next_positions=None, out_table=None):
+    """New lengths; ``pools`` (CPU tensors) are changed.  Plain loops over sequences, heads and tokens."""
+    size = pools["k"].shape[2]
+    fresh = {n: x.clone() for n, x in pools.items()}
+    for b, n in enumerate(int(x) for x in lens):
+        left = min(n, budget)
+        start = (n if next_positions is None else int(next_positions[b])) - recent
+        for h in range(pools["k"].shape[1]):
+            at = [(int(table[b, j // size]), h, j % size) for j in range(n)]
+
+            def order(j):
+                pos, w = int(pools["position"][at[j]]), float(pools["weight"][at[j]])
+                return (2 if pos < sinks or pos >= start else 1 if math.isnan(w) else 0, 0.0 if math.isnan(w) else w, j)
+
+            # a protected token's weight does not matter, nor a NaN's sign
+            gone = set(sorted(range(n), key=lambda j: order(j) if order(j)[0] == 0 else (order(j)[0], 0.0, j))[: n - left])
+            kept = [j for j in range(n) if j not in gone]
+            if out_table is not None:
+                moves = [(j, (int(out_table[b, i // size]), h, i % size)) for i, j in enumerate(kept)]
+            else:
+                moves = list(zip((j for j in kept if j >= left), (at[j] for j in range(left) if j in gone)))
+            for j, to in moves:
+                for name, x in fresh.items():
+                    x[to] = pools[name][at[j]]
+    for name, x in fresh.items():
+        pools[name].copy_(x)
+    return [min(int(n), budget) for n in lens]

@@ -137,3 +137,47 @@ def test_workspace_holds_a_slot_for_every_seam(lib, B, Hq, Hkv, page, mp):
     tiles = mp * page // 16
     ctas = min(296, -(-rows * tiles // 16))
     assert n.value >= (ctas + rows) * 8 * nt * (128 + 2) * 4
+
+
+def test_oracle_evict_by_hand():
+    pools, table = make([6], 1, 16, track=True, seed=0, spare=2)
+    p = int(table[0, 0])
+    pools["weight"][p, 0, :6] = torch.tensor([5.0, 1.0, 3.0, 1.0, math.nan, 0.0])
+    old = pools["k"].clone()
+    assert orc.evict(pools, table, [6], 4, sinks=1, recent=1) == [4]   # 1 and 3 leave (0.0 is the last token's)
+    assert torch.equal(pools["k"][p, 0, :4], old[p, 0, [0, 4, 2, 5]])
+    assert pools["position"][p, 0, :4].tolist() == [0, 4, 2, 5]
+    assert torch.equal(pools["k"][p, 0, 4:6], old[p, 0, 4:6])
+    pools, table = make([6], 1, 16, track=True, seed=0, spare=2)
+    pools["weight"][p, 0, :6] = torch.tensor([5.0, 1.0, 3.0, 1.0, math.nan, 0.0])
+    free = next(x for x in range(3) if x != p)
+    assert orc.evict(pools, table, [6], 3, out_table=torch.tensor([[free]])) == [3]
+    assert torch.equal(pools["k"][free, 0, :3], old[p, 0, [0, 2, 4]])
+    assert torch.equal(pools["k"][p, 0, :6], old[p, 0, :6])
+
+
+def test_evict_refuses_bad_arguments(lib):
+    some = ctypes.c_void_p(256)
+    track = {"weight": 256, "position": 256}
+    n = ctypes.c_uint64()
+    assert lib.fba_paged_evict_workspace_bytes(2, 3, 16, 10, 100, ctypes.byref(n)) == 0 and n.value == 2 * 3 * 100 * 8
+    assert lib.fba_paged_evict_workspace_bytes(2, 3, 16, 10, 1000, ctypes.byref(n)) == 0 and n.value == 2 * 3 * 160 * 8
+    for bad in ((0, 3, 16, 10, 100), (2, 0, 16, 10, 100), (2, 3, 16, 10, 0)):
+        assert lib.fba_paged_evict_workspace_bytes(*bad, ctypes.byref(n)) == -1
+    assert lib.fba_paged_evict_workspace_bytes(2, 3, 256, 2**22, 100, ctypes.byref(n)) == -5
+
+    def call(c=None, B=1, lens=some, budget=20, sinks=0, recent=0, out=None, out_pages=0, out_lens=ctypes.c_void_p(512), ws=some,
+             size=2**30):
+        return lib.fba_paged_evict(c or struct(**track), B, lens, budget, sinks, recent, None, out, out_pages, out_lens, ws,
+                                   size, some, None)
+
+    assert call(struct()) == -1 and b"no weights" in lib.fba_last_error()
+    assert call(lens=None) == -1 and call(out_lens=None) == -1 and call(out_lens=some) == -1
+    assert call(budget=0) == -1 and call(sinks=-1) == -1 and call(recent=-1) == -1 and call(sinks=15, recent=6) == -1
+    assert call(out=some, out_pages=1) == -1 and call(out=some, out_pages=0) == -1
+    assert call(ws=None) == -1 and call(ws=ctypes.c_void_p(258)) == -1 and call(size=2 * 20 * 8 - 1) == -1
+    for bad in BAD_CACHES:
+        assert call(struct(**(track | bad | ({"weight": None} if "position" in bad else {})
+                              | ({"position": None} if "weight" in bad else {})))) == -1
+    with pytest.raises(RuntimeError, match="no CPU path"):
+        fba.evict_kv(cache(), torch.zeros((1, 4), dtype=torch.int32), torch.ones(1, dtype=torch.int32), 4)
