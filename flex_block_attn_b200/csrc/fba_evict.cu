@@ -1,17 +1,17 @@
 // Eviction from a paged cache by accumulated attention weight.
 //
 // Per (sequence, kv head) of n slots the n - budget tokens that come first in the order (protected, weight, slot) leave.
-// One cluster of CTAs per (sequence, kv head), each CTA with a contiguous stretch of the slots:
-//   1. weights become 32-bit keys in their order (in shared memory where they fit), protected tokens the largest key;
+// One CTA per (sequence, kv head), or a cluster where the keys of its slots do not fit into one CTA's shared memory:
+//   1. weights become 32-bit keys in their order, protected tokens the largest key;
 //   2. the key T of the last token that leaves is found from its digits, 11 + 11 + 10 bits from the top: a histogram of a
 //      digit per CTA, all of them added up by every CTA through distributed shared memory;
 //   3. counts per warp (tokens with the key T; slots that come free; tokens to be moved), exchanged the same way, give
 //      every warp the place of its entries in the lists of slots to move from and to, which are in slot order
 //      therefore, whatever the timing;
-//   4. all CTAs of the cluster divide the list and copy the rows.
+//   4. the rows on the lists are copied, by a second kernel where there can be many.
 // In place, the i-th staying token behind slot `budget` goes to the i-th slot that came free before it: only as many rows move as
 // tokens leave from there, and no row is both read and written.
-// What bounds it: the rows copied (and, with few rows, the latency of the steps before).
+// What bounds it: the rows copied, and with few rows the latency of the steps before.
 #include <math.h>
 #include <stdio.h>
 
@@ -23,7 +23,7 @@ namespace fba {
 
 namespace cg = cooperative_groups;
 
-constexpr int kEvThreads = 512;
+constexpr int kEvThreads = 1024;
 constexpr int kEvWarps = kEvThreads / 32;
 constexpr int kEvBins = 2048;
 
@@ -32,6 +32,7 @@ struct EvictParams {
     int32_t* out_lens;
     int32_t *from, *to;      // [B * Hkv, list]: slots; `to` is not used with an out_table
     uint32_t* status;
+    int32_t* moves;          // [B * Hkv]: entries of the lists, for the second kernel; null: the first one copies
     int budget, sinks, recent, out_pages, list;
     int key_room;            // keys a CTA holds in shared memory; 0: read again on every use
 };
@@ -44,20 +45,74 @@ struct EvictShared {
     uint32_t digit, below;         // of the bin that holds the wanted rank: its number, and how many keys lie before it
 };
 
-__device__ __forceinline__ uint32_t evict_key(const PagedDev& c, const EvictParams& p, int b, int h, int slot, long long recent_from) {
-    const long long row = paged_row(c, b, h, slot, p.status);
-    if (row < 0) return 0u;   // a page that is not there: the first to leave
-    const int pos = c.position[row];
+__device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int pos, float weight, long long recent_from) {
     if (pos < p.sinks || pos >= recent_from) return 0xffffffffu;
-    const float w = c.weight[row] + 0.f;   // -0 counts as 0
+    const float w = weight + 0.f;          // -0 counts as 0
     if (isnan(w)) return 0xfffffffeu;      // above infinity
     const uint32_t u = __float_as_uint(w);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// Copies the entries i0, i0 + 1, ... < total of a head's lists, 32 at a time: a lane looks up one entry's rows, then the
+// warp copies them one after the other, half a warp each for K and V in bf16 (16 bytes a lane), a quarter each in e4m3,
+// then two tokens at a time.  `stride`: from one batch of the warp to its next.
+__device__ __forceinline__ void copy_rows(const PagedDev& c, const EvictParams& p, int b, int h, const int32_t* from,
+                                          const int32_t* to, int i0, int total, int stride) {
+    const int lane = threadIdx.x & 31;
+    const bool e4m3 = c.k_scale != nullptr;
+    const int lanes = e4m3 ? 8 : 16;
+    const int sub = lane / (2 * lanes), kv = lane / lanes & 1, l = lane % lanes;
+    PagedDev dst_c = c;
+    if (p.out_table) {
+        dst_c.table = p.out_table;
+        dst_c.max_pages = p.out_pages;
+    }
+    uint4* pool = reinterpret_cast<uint4*>(kv ? c.v : c.k);
+    for (int base = i0; base < total; base += stride) {
+        long long src = -1, dst = -1;
+        if (base + lane < total) {
+            src = paged_row(c, b, h, from[base + lane], p.status);
+            dst = paged_row(dst_c, b, h, p.out_table ? base + lane : to[base + lane], p.status);
+            if (src < 0 || dst < 0) {
+                dst = -1;   // a page that is not there
+            } else {   // what there is one of per row
+                if (e4m3) {
+                    const float ks = c.k_scale[src], vs = c.v_scale[src];
+                    c.k_scale[dst] = ks;
+                    c.v_scale[dst] = vs;
+                }
+                const float w = c.weight[src];
+                const int pos = c.position[src];
+                c.weight[dst] = w;
+                c.position[dst] = pos;
+            }
+        }
+        const int n = min(32, total - base);
+        constexpr int kFlight = 8;   // rows a lane has under way
+        const int tokens = e4m3 ? 2 : 1;
+        for (int j0 = 0; j0 < n; j0 += kFlight * tokens) {
+            uint4 x[kFlight];
+            long long d[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) {
+                const int j = j0 + u * tokens + sub;   // below 32 + 16; lanes repeat modulo 32
+                const long long s = __shfl_sync(0xffffffffu, src, j & 31);
+                d[u] = __shfl_sync(0xffffffffu, dst, j & 31);
+                if (j >= n) d[u] = -1;
+                if (d[u] >= 0) x[u] = pool[s * lanes + l];
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u)
+                if (d[u] >= 0) pool[d[u] * lanes + l] = x[u];
+        }
+    }
+}
+
 __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev c, const EvictParams p) {
     extern __shared__ uint32_t keys[];
     __shared__ EvictShared sh;
+    pdl_launch_dependents();
+    pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
     const int head = blockIdx.x / ctas, b = head / c.Hkv, h = head - b * c.Hkv;
@@ -65,7 +120,10 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     const int n = paged_length(c, p.seq_lens, b, p.status);
     const int left = min(n, p.budget), leave = n - left;
     if (h == 0 && rank == 0 && tid == 0) p.out_lens[b] = left;
-    if (leave == 0 && !p.out_table) return;   // the whole cluster, nothing to do
+    if (leave == 0 && !p.out_table) {   // the whole cluster, nothing to do
+        if (p.moves && rank == 0 && tid == 0) p.moves[head] = 0;
+        return;
+    }
     const long long recent_from = static_cast<long long>(p.next_positions ? p.next_positions[b] : n) - p.recent;
 
     // This CTA's slots, and of them this warp's; both multiples of 32 long.
@@ -74,10 +132,35 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     const int per_warp = ((end - begin + kEvWarps - 1) / kEvWarps + 31) / 32 * 32;
     const int w_begin = min(end, begin + warp * per_warp), w_end = min(end, w_begin + per_warp);
     const bool cached = per_cta <= p.key_room;
-    if (cached)
-        for (int i = begin + tid; i < end; i += kEvThreads) keys[i - begin] = evict_key(c, p, b, h, i, recent_from);
+    if (cached) {
+        constexpr int kFlight = 4;
+        for (int i0 = begin + tid; i0 < end; i0 += kFlight * kEvThreads) {
+            long long row[kFlight];
+            float w[kFlight];
+            int pos[kFlight];
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) {
+                const int i = i0 + u * kEvThreads;
+                row[u] = i < end ? paged_row(c, b, h, i, p.status) : -1;
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) {
+                w[u] = row[u] >= 0 ? c.weight[row[u]] : 0.f;
+                pos[u] = row[u] >= 0 ? c.position[row[u]] : 0;
+            }
+#pragma unroll
+            for (int u = 0; u < kFlight; ++u) {
+                const int i = i0 + u * kEvThreads;   // a page that is not there: the first to leave
+                if (i < end) keys[i - begin] = row[u] >= 0 ? evict_key(p, pos[u], w[u], recent_from) : 0u;
+            }
+        }
+    }
     __syncthreads();
-    auto key_of = [&](int i) { return cached ? keys[i - begin] : evict_key(c, p, b, h, i, recent_from); };
+    auto key_of = [&](int i) {
+        if (cached) return keys[i - begin];
+        const long long row = paged_row(c, b, h, i, p.status);
+        return row >= 0 ? evict_key(p, c.position[row], c.weight[row], recent_from) : 0u;
+    };
 
     // T, and how many tokens with a smaller key there are.
     uint32_t prefix = 0, below = 0;
@@ -94,17 +177,18 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
                 if (pass == 0 || (k >> kShift[pass ? pass - 1 : 0]) == prefix) atomicAdd(&sh.hist[(k >> shift) & (bins - 1)], 1u);
             }
             cluster.sync();
-            // Thread t: bins 4 t .. 4 t + 3 (2 t and 2 t + 1 in the last pass) of all CTAs.
-            uint32_t mine[4] = {0, 0, 0, 0}, sum = 0;
+            // Thread t: bins 2 t and 2 t + 1 (t alone in the last pass) of all CTAs.
+            constexpr int kPer = kEvBins / kEvThreads;
+            uint32_t mine[kPer] = {}, sum = 0;
             const int per = bins / kEvThreads;
             for (int r = 0; r < ctas; ++r) {
                 const uint32_t* other = cluster.map_shared_rank(sh.hist, r);
 #pragma unroll
-                for (int x = 0; x < 4; ++x)
+                for (int x = 0; x < kPer; ++x)
                     if (x < per) mine[x] += other[tid * per + x];
             }
 #pragma unroll
-            for (int x = 0; x < 4; ++x) sum += mine[x];
+            for (int x = 0; x < kPer; ++x) sum += mine[x];
             uint32_t upto = sum;
 #pragma unroll
             for (int s = 1; s < 32; s <<= 1) {
@@ -117,7 +201,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
             for (int w = 0; w < warp; ++w) before += sh.scan[w];
             if (rank_left >= before && rank_left < before + sum) {
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
+                for (int x = 0; x < kPer; ++x) {
                     if (rank_left >= before && rank_left < before + mine[x]) {
                         sh.digit = tid * per + x;
                         sh.below = before;
@@ -191,48 +275,23 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     });
     cluster.sync();   // the lists are written, and no CTA's shared memory is read any more
 
-    // Rows: half a warp each for K and V in bf16 (16 bytes a lane), a quarter each in e4m3, then two tokens at a time.
-    const bool e4m3 = c.k_scale != nullptr;
-    const int lanes = e4m3 ? 8 : 16, tokens = 16 / lanes;     // a warp's tokens at a time
-    const int sub = lane / (2 * lanes), kv = lane / lanes & 1, l = lane % lanes;
-    PagedDev dst_c = c;
-    if (out) {
-        dst_c.table = p.out_table;
-        dst_c.max_pages = p.out_pages;
-    }
-    uint8_t* pool = kv ? c.v : c.k;
     const int total = static_cast<int>(all_moves);
-    const int step = ctas * kEvWarps * tokens;
-    constexpr int kFlight = 4;   // rows a lane has under way
-    for (int i0 = (rank * kEvWarps + warp) * tokens + sub; i0 < total; i0 += step * kFlight) {
-        long long dst[kFlight];
-        uint4 x[kFlight];
-        float f[kFlight];
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u) {
-            const int i = i0 + u * step;
-            dst[u] = -1;
-            if (i >= total) continue;
-            const long long src = paged_row(c, b, h, from[i], p.status);
-            dst[u] = paged_row(dst_c, b, h, out ? i : to[i], p.status);
-            if (src < 0) dst[u] = -1;
-            if (dst[u] < 0) continue;
-            x[u] = reinterpret_cast<const uint4*>(pool)[src * lanes + l];
-            // lane 0: the row's scale, lane 1: weight (by K's lanes) or position (by V's)
-            if (l == 0 && e4m3) f[u] = (kv ? c.v_scale : c.k_scale)[src];
-            if (l == 1) f[u] = kv ? __int_as_float(c.position[src]) : c.weight[src];
-        }
-#pragma unroll
-        for (int u = 0; u < kFlight; ++u) {
-            if (dst[u] < 0) continue;
-            reinterpret_cast<uint4*>(pool)[dst[u] * lanes + l] = x[u];
-            if (l == 0 && e4m3) (kv ? c.v_scale : c.k_scale)[dst[u]] = f[u];
-            if (l == 1) {
-                if (kv) c.position[dst[u]] = __float_as_int(f[u]);
-                else c.weight[dst[u]] = f[u];
-            }
-        }
+    if (p.moves) {
+        if (rank == 0 && tid == 0) p.moves[head] = total;
+        return;
     }
+    copy_rows(c, p, b, h, from, to, (rank * kEvWarps + warp) * 32, total, ctas * kEvWarps * 32);
+}
+
+// The copies, a warp per 32 entries of a head's lists.
+constexpr int kMoveWarps = 4;
+__global__ void __launch_bounds__(kMoveWarps * 32) paged_move_kernel(const PagedDev c, const EvictParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int head = blockIdx.y, b = head / c.Hkv, h = head - b * c.Hkv;
+    const int total = p.moves[head];
+    copy_rows(c, p, b, h, p.from + static_cast<long long>(head) * p.list, p.to + static_cast<long long>(head) * p.list,
+              (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * 32, total, gridDim.x * kMoveWarps * 32);
 }
 
 }  // namespace fba
@@ -240,6 +299,9 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
 using namespace fba;
 
 namespace {
+// Up to so many rows a head are copied by the CTA that chose them; more by a kernel of their own, whose launch costs
+// less than leaving most SMs idle.
+constexpr int kMoveHere = 256;
 int evict_list(int page_size, int max_pages, int budget) {
     const long long cap = static_cast<long long>(max_pages) * page_size;
     return static_cast<int>(cap < budget ? cap : budget);
@@ -251,7 +313,7 @@ extern "C" int fba_paged_evict_workspace_bytes(int B, int Hkv, int page_size, in
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict_workspace_bytes: bad argument");
     if (static_cast<long long>(max_pages) * page_size >= 1 << 30)
         return set_error(FBA_ERR_TOO_LARGE, "fba_paged_evict_workspace_bytes: max_pages * page_size reaches 2^30");
-    *bytes = static_cast<uint64_t>(B) * Hkv * evict_list(page_size, max_pages, budget) * 2 * sizeof(int32_t);
+    *bytes = static_cast<uint64_t>(B) * Hkv * (evict_list(page_size, max_pages, budget) * 2ull + 1) * sizeof(int32_t);
     return FBA_OK;
 }
 
@@ -277,7 +339,7 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
         return set_error(FBA_ERR_BAD_ARG,
                          "fba_paged_evict: workspace must be 4-byte aligned, of fba_paged_evict_workspace_bytes() bytes");
     const long long heads = static_cast<long long>(B) * c.Hkv;
-    if (heads > 1 << 24) return set_error(FBA_ERR_TOO_LARGE, "fba_paged_evict: more than 2^24 heads of sequences");
+    if (heads > 65535) return set_error(FBA_ERR_TOO_LARGE, "fba_paged_evict: B * Hkv exceeds 65535");
     EvictParams p = {};
     p.seq_lens = seq_lens;
     p.next_positions = next_positions;
@@ -291,13 +353,16 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     p.recent = recent;
     p.out_pages = out_pages;
     p.list = list;
-    // A cluster grows while there are idle SMs and a CTA would have more than 2048 slots.
+    // The keys of a CTA's slots stay in shared memory beside the histogram, with a cluster of up to 8 CTAs if need be.
+    constexpr long long kMostKeys = 200 * 1024 / 4;
     const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
     int ctas = 1;
-    while (ctas < 8 && heads * ctas < 148 && cap / ctas > 2048) ctas *= 2;
-    // The keys of a CTA's slots in shared memory where they fit beside the histogram.
+    while (ctas < 8 && cap > kMostKeys * ctas) ctas *= 2;
     const long long room = ((cap + ctas - 1) / ctas + 31) / 32 * 32;
-    p.key_room = room * 4 <= 200 * 1024 ? static_cast<int>(room) : 0;
+    p.key_room = room <= kMostKeys ? static_cast<int>(room) : 0;
+    // The most rows that a head can have to copy.
+    const long long most = out_table ? list : (cap - budget < list ? cap - budget : list);
+    if (most > kMoveHere) p.moves = p.to + heads * list;
 
     DeviceGuard guard;
     if ((rc = guard.bind(cache->k)) != FBA_OK) return rc;
@@ -310,12 +375,19 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     config.blockDim = dim3(kEvThreads);
     config.dynamicSmemBytes = static_cast<size_t>(p.key_room) * 4;
     config.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = ctas;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attr;
-    config.numAttrs = 1;
-    if (cudaLaunchKernelEx(&config, paged_evict_kernel, c, p) != cudaSuccess) return check_launch("paged_evict_kernel");
-    return check_launch("paged_evict_kernel");
+    config.numAttrs = 2;
+    cudaLaunchKernelEx(&config, paged_evict_kernel, c, p);
+    if ((rc = check_launch("paged_evict_kernel")) != FBA_OK || !p.moves) return rc;
+    // Blocks for all of a head's entries while the grid stays within a few waves; a warp takes further batches beyond.
+    long long blocks = (most + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
+    const long long enough = (148 * 16 + heads - 1) / heads;
+    return launch_chained(paged_move_kernel, dim3(static_cast<unsigned>(blocks < enough ? blocks : enough), static_cast<unsigned>(heads)),
+                          kMoveWarps * 32, 0, static_cast<cudaStream_t>(stream), c, p);
 }

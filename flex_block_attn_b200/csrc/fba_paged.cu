@@ -26,6 +26,8 @@ __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either 
 // could hold the memory back: bound by the rows read and written.
 template <bool kE4m3>
 __global__ void __launch_bounds__(256) paged_append_kernel(const PagedDev c, const AppendParams p) {
+    pdl_launch_dependents();
+    pdl_wait();
     const int b = blockIdx.y;
     const int lane = threadIdx.x & 31, l16 = lane & 15;
     const int start = paged_length(c, p.seq_lens, b, p.status);
@@ -233,6 +235,8 @@ template <bool kE4m3, int NT>
 __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const PagedDev c, const DecodeParams p) {
     using Sh = DecShape<kE4m3>;
     extern __shared__ __align__(128) uint8_t smem[];
+    pdl_launch_dependents();
+    pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * Sh::kStages * Sh::kStage;
@@ -582,67 +586,127 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
     cp_async_wait<0>();
 }
 
-// Joins the parts of the rows that several CTAs share, gives the rows without a tile their zeros, and adds the
-// probabilities to the weights.  blockIdx.x = row, blockIdx.y = a stretch of its slots; thread = dim, then slot.
+// A row's tiles are in the pieces of CTAs first .. last; `whole`: of one, which wrote the result itself.  No tile: none.
+struct RowParts {
+    int first, last;
+    bool whole;
+};
+__device__ __forceinline__ RowParts row_parts(const PagedDev& c, const DecodeParams& p, int b, int hr, int nt) {
+    if (p.n_ctas == 0) return {0, 0, true};
+    if (nt == 0) return {0, -1, false};
+    const int rows_per_seq = c.Hkv * p.q_tiles;
+    int ahead = 0, all = 0;   // tiles of the sequences before b, and of all
+    for (int x = threadIdx.x & 31; x < p.B; x += 32) {
+        const int n = seq_tiles(paged_length(c, p.seq_lens, x, p.status), p.window, p.sinks).nt;
+        all += n;
+        if (x < b) ahead += n;
+    }
+    ahead = __reduce_add_sync(0xffffffffu, ahead);
+    all = __reduce_add_sync(0xffffffffu, all);
+    const long long per = list_piece(static_cast<long long>(all) * rows_per_seq, p.n_ctas);
+    const long long at = static_cast<long long>(ahead) * rows_per_seq + static_cast<long long>(hr) * nt;
+    const int first = static_cast<int>(at / per), last = static_cast<int>((at + nt - 1) / per);
+    return {first, last, first == last};
+}
+// Largest maximum of the parts of a query head; every lane of the warp takes part.
+__device__ __forceinline__ float parts_max(const DecodeParams& p, const RowParts& r, long long slot0, int step) {
+    float top = -INFINITY;
+    for (int x = r.first + (threadIdx.x & 31); x <= r.last; x += 32) top = fmaxf(top, p.part_ml[(slot0 + static_cast<long long>(x) * step) * 2]);
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
+    return top;
+}
+// Weight of a part with maximum m; where no part has a finite score, the sums (0, or NaN) stand as they are.
+__device__ __forceinline__ float part_scale(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
+
+// Joins the parts of the rows that several CTAs share, and gives the rows without a tile their zeros.  One block per row
+// and query head; the four warps take the parts in turn, a lane four dims.  Latency-bound: a few KB per block, so the
+// loads of a warp's parts are independent of one another.  (One block per row with its heads in turn and the sums carried
+// from part to part took 11 us for 64 sequences, 24 us for 16 of 8 heads a kv head, 36 us for two long ones.)
 template <int NT>
 __global__ void __launch_bounds__(128) paged_join_kernel(const PagedDev c, const DecodeParams p) {
-    __shared__ float s_lse[8 * NT];
+    __shared__ float4 s_o[4][32];
+    __shared__ float s_l[4];
     const int rows_per_seq = c.Hkv * p.q_tiles;
     const int b = blockIdx.x / rows_per_seq, hr = blockIdx.x - b * rows_per_seq;
     const int h = hr / p.q_tiles, q0 = h * p.group + (hr - h * p.q_tiles) * 8 * NT;
-    const int heads = min(8 * NT, (h + 1) * p.group - q0);
+    const int hq = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    if (hq >= min(8 * NT, (h + 1) * p.group - q0)) return;
     const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
-    const int lane = threadIdx.x & 31;
-    int c0 = 0, c1 = -1;
-    bool whole = p.n_ctas == 0;
-    if (!whole && s.nt > 0) {
-        int ahead = 0, all = 0;   // tiles of the sequences before b, and of all
-        for (int x = lane; x < p.B; x += 32) {
-            const int nt = seq_tiles(paged_length(c, p.seq_lens, x, p.status), p.window, p.sinks).nt;
-            all += nt;
-            if (x < b) ahead += nt;
-        }
-        ahead = __reduce_add_sync(0xffffffffu, ahead);
-        all = __reduce_add_sync(0xffffffffu, all);
-        const long long per = list_piece(static_cast<long long>(all) * rows_per_seq, p.n_ctas);
-        const long long at = static_cast<long long>(ahead) * rows_per_seq + static_cast<long long>(hr) * s.nt;
-        c0 = static_cast<int>(at / per);
-        c1 = static_cast<int>((at + s.nt - 1) / per);
-        whole = c0 == c1;
+    const RowParts r = row_parts(c, p, b, hr, s.nt);
+    if (r.whole) return;
+    const long long slot0 = static_cast<long long>(blockIdx.x) * (8 * NT) + hq;   // a part x CTAs on is x * 8 NT slots on
+    const float top = parts_max(p, r, slot0, 8 * NT);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float l = 0.f;
+#pragma unroll 8
+    for (int x = r.first + warp; x <= r.last; x += 4) {
+        const long long slot = slot0 + static_cast<long long>(x) * (8 * NT);
+        const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[slot];
+        const float4 v = reinterpret_cast<const float4*>(p.part_o)[slot * 32 + lane];
+        const float a = part_scale(ml.x, top);
+        l = fmaf(a, ml.y, l);
+        o.x = fmaf(a, v.x, o.x);
+        o.y = fmaf(a, v.y, o.y);
+        o.z = fmaf(a, v.z, o.z);
+        o.w = fmaf(a, v.w, o.w);
     }
-    const int d = threadIdx.x;
-    for (int hq = 0; hq < heads; ++hq) {
-        const long long out = static_cast<long long>(b) * p.Hq + q0 + hq;
-        if (whole && s.nt > 0) {
-            if (d == 0 && p.scores) s_lse[hq] = p.lse[out] * kLog2e;
-            continue;
-        }
-        float top = -INFINITY, sum = 0.f, o = 0.f;
-        for (int x = c0; x <= c1; ++x) {
-            const long long slot = (static_cast<long long>(x) + blockIdx.x) * (8 * NT) + hq;
-            const float m = p.part_ml[slot * 2], l = p.part_ml[slot * 2 + 1], v = p.part_o[slot * 128 + d];
-            const float now = fmaxf(top, m);
-            if (now == -INFINITY && !isnan(l)) continue;
-            const float keep = ex2_approx(top - now), take = ex2_approx(m - now);
-            sum = sum * keep + l * take;
-            o = o * keep + v * take;
-            top = now;
-        }
-        const bool some = sum > 0.f || isnan(sum);
-        if (blockIdx.y == 0) {
-            p.o[out * 128 + d] = __float2bfloat16(some ? o / sum : 0.f);
-            if (p.lse && d == 0) p.lse[out] = some ? (top + log2f(sum)) * kLn2 : -INFINITY;
-        }
-        if (d == 0) s_lse[hq] = top + log2f(sum);
-    }
-    if (p.scores == nullptr) return;
+    s_o[warp][lane] = o;
+    if (lane == 0) s_l[warp] = l;
     __syncthreads();
-    for (int j = blockIdx.y * 128 + threadIdx.x; j < s.n; j += gridDim.y * 128) {
+    const int d = threadIdx.x;
+    const float* so = reinterpret_cast<const float*>(s_o);
+    const float sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    const float x = (so[d] + so[128 + d]) + (so[256 + d] + so[384 + d]);
+    const bool some = sum > 0.f || isnan(sum);
+    const long long out = static_cast<long long>(b) * p.Hq + q0 + hq;
+    p.o[out * 128 + d] = __float2bfloat16(some ? x / sum : 0.f);
+    if (p.lse && d == 0) p.lse[out] = some ? (top + log2f(sum)) * kLn2 : -INFINITY;
+}
+
+// Adds the probabilities to the weights, from the scores and the parts' sums.  blockIdx.x = row, blockIdx.y = a stretch of
+// kWeighSlots slots.
+constexpr int kWeighSlots = 1024;
+template <int NT>
+__global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDev c, const DecodeParams p) {
+    __shared__ float s_lse[8 * NT];   // in units of log2
+    const int rows_per_seq = c.Hkv;   // host-checked: q_tiles is 1
+    const int b = blockIdx.x / rows_per_seq, h = blockIdx.x - b * rows_per_seq;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
+    if (static_cast<int>(blockIdx.y) * kWeighSlots >= s.n) return;
+    const RowParts r = row_parts(c, p, b, h, s.nt);
+    const long long q0 = static_cast<long long>(b) * p.Hq + h * p.group;
+    for (int hq = warp; hq < p.group; hq += 8) {
+        float lse;
+        if (r.whole) {
+            lse = p.lse[q0 + hq] * kLog2e;
+        } else {
+            const long long slot0 = static_cast<long long>(blockIdx.x) * (8 * NT) + hq;
+            const float top = parts_max(p, r, slot0, 8 * NT);
+            float l = 0.f;
+            for (int x = r.first + lane; x <= r.last; x += 32) {
+                const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[slot0 + static_cast<long long>(x) * (8 * NT)];
+                l = fmaf(part_scale(ml.x, top), ml.y, l);
+            }
+#pragma unroll
+            for (int sh = 16; sh > 0; sh >>= 1) l += __shfl_xor_sync(0xffffffffu, l, sh);
+            lse = top + log2f(l);
+        }
+        if (lane == 0) s_lse[hq] = lse;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kWeighSlots / 256; ++u) {
+        const int j = blockIdx.y * kWeighSlots + u * 256 + threadIdx.x;
+        if (j >= s.n) continue;
         const long long row = paged_row(c, b, h, j, p.status);
         if (row < 0) continue;
         float w = 0.f;
-        for (int hq = 0; hq < heads; ++hq)
-            w += ex2_approx(p.scores[(static_cast<long long>(b) * p.Hq + q0 + hq) * p.score_stride + j] - s_lse[hq]);
+#pragma unroll 8
+        for (int hq = 0; hq < p.group; ++hq) w += ex2_approx(p.scores[(q0 + hq) * p.score_stride + j] - s_lse[hq]);
         c.weight[row] += w;
     }
 }
@@ -709,8 +773,7 @@ extern "C" int fba_paged_append(const fba_paged_t* cache, const void* k, const v
     const long long most = (148 * 16 + B - 1) / B;
     dim3 grid(static_cast<unsigned>(blocks < most ? blocks : most), B);
     auto kernel = cache->e4m3 ? paged_append_kernel<true> : paged_append_kernel<false>;
-    kernel<<<grid, 256, 0, static_cast<cudaStream_t>(stream)>>>(c, p);
-    return check_launch("paged_append_kernel");
+    return launch_chained(kernel, grid, 256, 0, static_cast<cudaStream_t>(stream), c, p);
 }
 
 namespace {
@@ -739,19 +802,19 @@ DecodePlan decode_plan(int B, int Hq, int Hkv, int page_size, int max_pages, boo
     return d;
 }
 template <bool kE4m3, int NT>
-int launch_decode(const PagedDev& c, const DecodeParams& p, const DecodePlan& d, bool join, cudaStream_t stream) {
+int launch_decode(const PagedDev& c, const DecodeParams& p, const DecodePlan& d, cudaStream_t stream) {
     constexpr int smem = DecShape<kE4m3>::kSmem;
     if (cudaFuncSetAttribute(paged_decode_kernel<kE4m3, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) {
         cudaGetLastError();
         return set_error(FBA_ERR_LAUNCH, "fba_paged_decode: cannot raise the dynamic shared memory limit");
     }
-    paged_decode_kernel<kE4m3, NT><<<d.n_ctas ? d.n_ctas : static_cast<unsigned>(d.rows), kDecThreads, smem, stream>>>(c, p);
-    int rc = check_launch("paged_decode_kernel");
-    if (rc != FBA_OK || !join) return rc;
-    int stretches = 1;
-    if (p.scores) stretches = static_cast<int>(min(64ll, (d.score_stride + 511ll) / 512));
-    paged_join_kernel<NT><<<dim3(static_cast<unsigned>(d.rows), stretches), 128, 0, stream>>>(c, p);
-    return check_launch("paged_join_kernel");
+    const unsigned rows = static_cast<unsigned>(d.rows);
+    int rc = launch_chained(paged_decode_kernel<kE4m3, NT>, dim3(d.n_ctas ? d.n_ctas : rows), kDecThreads, smem, stream, c, p);
+    if (rc == FBA_OK && d.n_ctas)
+        rc = launch_chained(paged_join_kernel<NT>, dim3(rows, p.group < 8 * NT ? p.group : 8 * NT), 128, 0, stream, c, p);
+    if (rc == FBA_OK && p.scores)
+        rc = launch_chained(paged_weigh_kernel<NT>, dim3(rows, (d.score_stride + kWeighSlots - 1) / kWeighSlots), 256, 0, stream, c, p);
+    return rc;
 }
 }  // namespace
 
@@ -826,7 +889,6 @@ extern "C" int fba_paged_decode(const fba_paged_t* cache, const void* q, const i
     p.sinks = sinks;
     p.n_ctas = d.n_ctas;
     p.scale_log2 = softmax_scale * kLog2e;
-    const bool join = d.n_ctas != 0 || accumulate;
-    if (cache->e4m3) return d.nt == 1 ? launch_decode<true, 1>(c, p, d, join, stream) : launch_decode<true, 2>(c, p, d, join, stream);
-    return d.nt == 1 ? launch_decode<false, 1>(c, p, d, join, stream) : launch_decode<false, 2>(c, p, d, join, stream);
+    if (cache->e4m3) return d.nt == 1 ? launch_decode<true, 1>(c, p, d, stream) : launch_decode<true, 2>(c, p, d, stream);
+    return d.nt == 1 ? launch_decode<false, 1>(c, p, d, stream) : launch_decode<false, 2>(c, p, d, stream);
 }

@@ -41,6 +41,27 @@ __device__ __forceinline__ long long paged_row(const PagedDev& c, int b, int h, 
     return (static_cast<long long>(page) * c.Hkv + h) * c.page_size + (slot & (c.page_size - 1));
 }
 
+// Programmatic dependent launch: a kernel of this family may be set up while the one before it in the stream still runs.  Each
+// waits for its predecessor's end (and with it, as the predecessor did the same, for all before) ahead of its first
+// access to memory, in every thread.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <class... Params, class... Args>
+int launch_chained(void (*kernel)(Params...), dim3 grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
+    cudaLaunchConfig_t config = {};
+    config.gridDim = grid;
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attr;
+    config.numAttrs = 1;
+    cudaLaunchKernelEx(&config, kernel, args...);
+    return check_launch("launch of a paged-cache kernel");
+}
+
 // Checks a cache and fills its device view (fba_paged.cu).
 int paged_args(const char* who, const fba_paged_t* cache, int B, PagedDev* dev);
 

@@ -160,8 +160,8 @@ def test_evict_refuses_bad_arguments(lib):
     some = ctypes.c_void_p(256)
     track = {"weight": 256, "position": 256}
     n = ctypes.c_uint64()
-    assert lib.fba_paged_evict_workspace_bytes(2, 3, 16, 10, 100, ctypes.byref(n)) == 0 and n.value == 2 * 3 * 100 * 8
-    assert lib.fba_paged_evict_workspace_bytes(2, 3, 16, 10, 1000, ctypes.byref(n)) == 0 and n.value == 2 * 3 * 160 * 8
+    assert lib.fba_paged_evict_workspace_bytes(2, 3, 16, 10, 100, ctypes.byref(n)) == 0 and n.value == 2 * 3 * (100 * 8 + 4)
+    assert lib.fba_paged_evict_workspace_bytes(2, 3, 16, 10, 1000, ctypes.byref(n)) == 0 and n.value == 2 * 3 * (160 * 8 + 4)
     for bad in ((0, 3, 16, 10, 100), (2, 0, 16, 10, 100), (2, 3, 16, 10, 0)):
         assert lib.fba_paged_evict_workspace_bytes(*bad, ctypes.byref(n)) == -1
     assert lib.fba_paged_evict_workspace_bytes(2, 3, 256, 2**22, 100, ctypes.byref(n)) == -5
@@ -175,7 +175,7 @@ def test_evict_refuses_bad_arguments(lib):
     assert call(lens=None) == -1 and call(out_lens=None) == -1 and call(out_lens=some) == -1
     assert call(budget=0) == -1 and call(sinks=-1) == -1 and call(recent=-1) == -1 and call(sinks=15, recent=6) == -1
     assert call(out=some, out_pages=1) == -1 and call(out=some, out_pages=0) == -1
-    assert call(ws=None) == -1 and call(ws=ctypes.c_void_p(258)) == -1 and call(size=2 * 20 * 8 - 1) == -1
+    assert call(ws=None) == -1 and call(ws=ctypes.c_void_p(258)) == -1 and call(size=2 * (20 * 8 + 4) - 1) == -1
     for bad in BAD_CACHES:
         assert call(struct(**(track | bad | ({"weight": None} if "position" in bad else {})
                               | ({"position": None} if "weight" in bad else {})))) == -1
