@@ -40,8 +40,8 @@ struct EvictParams {
 struct EvictShared {
     uint32_t hist[kEvBins];
     uint32_t scan[kEvWarps];
-    uint32_t count[3][kEvWarps];   // per warp: ties, holes, movers
-    uint32_t total[3];             // of the CTA
+    uint2 count[2][kEvWarps];      // per warp: ties, then holes and moves
+    uint2 total[2];                // of the CTA
     uint32_t digit, below;         // of the bin that holds the wanted rank: its number, and how many keys lie before it
 };
 
@@ -56,11 +56,11 @@ __device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int pos, flo
 // Copies the entries i0, i0 + 1, ... < total of a head's lists, 32 at a time: a lane looks up one entry's rows, then the
 // warp copies them one after the other, half a warp each for K and V in bf16 (16 bytes a lane), a quarter each in e4m3,
 // then two tokens at a time.  `stride`: from one batch of the warp to its next.
+template <bool e4m3>
 __device__ __forceinline__ void copy_rows(const PagedDev& c, const EvictParams& p, int b, int h, const int32_t* from,
                                           const int32_t* to, int i0, int total, int stride) {
     const int lane = threadIdx.x & 31;
-    const bool e4m3 = c.k_scale != nullptr;
-    const int lanes = e4m3 ? 8 : 16;
+    constexpr int lanes = e4m3 ? 8 : 16, tokens = e4m3 ? 2 : 1;
     const int sub = lane / (2 * lanes), kv = lane / lanes & 1, l = lane % lanes;
     PagedDev dst_c = c;
     if (p.out_table) {
@@ -89,7 +89,6 @@ __device__ __forceinline__ void copy_rows(const PagedDev& c, const EvictParams& 
         }
         const int n = min(32, total - base);
         constexpr int kFlight = 8;   // rows a lane has under way
-        const int tokens = e4m3 ? 2 : 1;
         for (int j0 = 0; j0 < n; j0 += kFlight * tokens) {
             uint4 x[kFlight];
             long long d[kFlight];
@@ -115,6 +114,10 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    auto sync_all = [&]() {
+        if (ctas > 1) cluster.sync();
+        else __syncthreads();
+    };
     const int head = blockIdx.x / ctas, b = head / c.Hkv, h = head - b * c.Hkv;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int n = paged_length(c, p.seq_lens, b, p.status);
@@ -133,7 +136,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     const int w_begin = min(end, begin + warp * per_warp), w_end = min(end, w_begin + per_warp);
     const bool cached = per_cta <= p.key_room;
     if (cached) {
-        constexpr int kFlight = 4;
+        constexpr int kFlight = 8;
         for (int i0 = begin + tid; i0 < end; i0 += kFlight * kEvThreads) {
             long long row[kFlight];
             float w[kFlight];
@@ -176,7 +179,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
                 const uint32_t k = key_of(i);
                 if (pass == 0 || (k >> kShift[pass ? pass - 1 : 0]) == prefix) atomicAdd(&sh.hist[(k >> shift) & (bins - 1)], 1u);
             }
-            cluster.sync();
+            sync_all();
             // Thread t: bins 2 t and 2 t + 1 (t alone in the last pass) of all CTAs.
             constexpr int kPer = kEvBins / kEvThreads;
             uint32_t mine[kPer] = {}, sum = 0;
@@ -209,7 +212,7 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
                     before += mine[x];
                 }
             }
-            cluster.sync();   // all have read the histograms, and `digit` is there
+            sync_all();   // all have read the histograms, and `digit` is there
             prefix = (prefix << kBits[pass]) | sh.digit;
             below += sh.below;
             rank_left -= sh.below;
@@ -217,30 +220,36 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     }
     const uint32_t T = prefix, ties_leave = leave - below;   // of the tokens with key T the first so many leave
 
-    // Sums over the warps ahead of this one, in this CTA and in those before it, and over the cluster.
-    auto place = [&](int what, uint32_t count, uint32_t& all) {
+    // Sums of a pair of counts over the warps ahead of this one, in this CTA and in those before it, and over the cluster.
+    static_assert(kEvWarps == 32, "a lane reads a warp's counts");
+    auto place = [&](int what, uint2 count, uint2& all) {
         if (lane == 0) sh.count[what][warp] = count;
         __syncthreads();
-        if (tid == 0) {
-            uint32_t t = 0;
-            for (int w = 0; w < kEvWarps; ++w) t += sh.count[what][w];
-            sh.total[what] = t;
+        const uint2 x = sh.count[what][lane];
+        uint2 before = make_uint2(__reduce_add_sync(0xffffffffu, lane < warp ? x.x : 0u),
+                                  __reduce_add_sync(0xffffffffu, lane < warp ? x.y : 0u));
+        all = make_uint2(__reduce_add_sync(0xffffffffu, x.x), __reduce_add_sync(0xffffffffu, x.y));
+        if (ctas > 1) {
+            if (tid == 0) sh.total[what] = all;
+            cluster.sync();
+            all = make_uint2(0, 0);
+            for (int r = 0; r < ctas; ++r) {
+                const uint2 y = *cluster.map_shared_rank(&sh.total[what], r);
+                all.x += y.x;
+                all.y += y.y;
+                if (r < rank) {
+                    before.x += y.x;
+                    before.y += y.y;
+                }
+            }
         }
-        cluster.sync();
-        uint32_t before = 0;
-        all = 0;
-        for (int r = 0; r < ctas; ++r) {
-            const uint32_t t = *cluster.map_shared_rank(&sh.total[what], r);
-            all += t;
-            if (r < rank) before += t;
-        }
-        for (int w = 0; w < warp; ++w) before += sh.count[what][w];
         return before;
     };
-    uint32_t ties = 0, unused;
+    uint32_t ties = 0;
     for (int i = w_begin + lane; i < w_end; i += 32) ties += key_of(i) == T;
     ties = __reduce_add_sync(0xffffffffu, ties);
-    const uint32_t ties_before = place(0, ties, unused);
+    uint2 unused;
+    const uint32_t ties_before = place(0, make_uint2(ties, 0), unused).x;
     // Calls f(slot, stays) for the warp's slots, a full warp at a time.
     auto for_slots = [&](auto f) {
         uint32_t tie = ties_before;
@@ -260,8 +269,9 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
         n_moves += __popc(__ballot_sync(0xffffffffu, stays && (out || i >= left)));
         n_holes += __popc(__ballot_sync(0xffffffffu, goes && i < left));
     });
-    uint32_t all_moves, all_holes;
-    uint32_t move = place(2, n_moves, all_moves), hole = place(1, n_holes, all_holes);
+    uint2 all;
+    const uint2 at = place(1, make_uint2(n_holes, n_moves), all);
+    uint32_t hole = at.x, move = at.y;
     int32_t* from = p.from + static_cast<long long>(head) * p.list;
     int32_t* to = p.to + static_cast<long long>(head) * p.list;
     for_slots([&](int i, bool stays, bool goes) {
@@ -273,24 +283,26 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
         move += __popc(mv);
         hole += __popc(hl);
     });
-    cluster.sync();   // the lists are written, and no CTA's shared memory is read any more
+    sync_all();   // the lists are written, and no CTA's shared memory is read any more
 
-    const int total = static_cast<int>(all_moves);
+    const int total = static_cast<int>(all.y);
     if (p.moves) {
         if (rank == 0 && tid == 0) p.moves[head] = total;
         return;
     }
-    copy_rows(c, p, b, h, from, to, (rank * kEvWarps + warp) * 32, total, ctas * kEvWarps * 32);
+    if (c.k_scale) copy_rows<true>(c, p, b, h, from, to, (rank * kEvWarps + warp) * 32, total, ctas * kEvWarps * 32);
+    else copy_rows<false>(c, p, b, h, from, to, (rank * kEvWarps + warp) * 32, total, ctas * kEvWarps * 32);
 }
 
 // The copies, a warp per 32 entries of a head's lists.
 constexpr int kMoveWarps = 4;
-__global__ void __launch_bounds__(kMoveWarps * 32) paged_move_kernel(const PagedDev c, const EvictParams p) {
+template <bool e4m3>
+__global__ void __launch_bounds__(kMoveWarps * 32, 8) paged_move_kernel(const PagedDev c, const EvictParams p) {
     pdl_launch_dependents();
     pdl_wait();
     const int head = blockIdx.y, b = head / c.Hkv, h = head - b * c.Hkv;
     const int total = p.moves[head];
-    copy_rows(c, p, b, h, p.from + static_cast<long long>(head) * p.list, p.to + static_cast<long long>(head) * p.list,
+    copy_rows<e4m3>(c, p, b, h, p.from + static_cast<long long>(head) * p.list, p.to + static_cast<long long>(head) * p.list,
               (blockIdx.x * kMoveWarps + (threadIdx.x >> 5)) * 32, total, gridDim.x * kMoveWarps * 32);
 }
 
@@ -388,6 +400,6 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     // Blocks for all of a head's entries while the grid stays within a few waves; a warp takes further batches beyond.
     long long blocks = (most + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
     const long long enough = (148 * 16 + heads - 1) / heads;
-    return launch_chained(paged_move_kernel, dim3(static_cast<unsigned>(blocks < enough ? blocks : enough), static_cast<unsigned>(heads)),
+    return launch_chained(cache->e4m3 ? paged_move_kernel<true> : paged_move_kernel<false>, dim3(static_cast<unsigned>(blocks < enough ? blocks : enough), static_cast<unsigned>(heads)),
                           kMoveWarps * 32, 0, static_cast<cudaStream_t>(stream), c, p);
 }

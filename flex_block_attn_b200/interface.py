@@ -44,6 +44,18 @@ class _StatusMonitor:
         self.host = torch.zeros(8, dtype=torch.int32).pin_memory()
         self.event = torch.cuda.Event()
         self.pending = False
+        # Words in host memory that the kernels reach as they are (the window and paged-cache entry points): nothing is
+        # copied after a call, and looking at them costs nothing.
+        self.mapped = torch.zeros(8, dtype=torch.int32).pin_memory()
+        self.mapped_ptr = self.mapped.data_ptr()
+        self._mapped_np = self.mapped.numpy()
+
+    def poll_mapped(self) -> None:
+        """Raise if a kernel has reported into the words in host memory."""
+        if self._mapped_np[0]:
+            if not torch.cuda.is_current_stream_capturing():
+                torch.cuda.synchronize(self.device)   # all of the words are there
+            self.raise_from(self.mapped.tolist())
 
     def after_call(self) -> None:
         if torch.cuda.is_current_stream_capturing():   # a replay writes the words; check_status() or a later call sees them
@@ -62,6 +74,7 @@ class _StatusMonitor:
     def raise_from(self, words) -> None:
         self.buf.zero_()
         self.host.zero_()
+        self.mapped.zero_()
         if words[0] != 1:
             raise RuntimeError(
                 "flex_block_attn_b200: a paged cache was given the "
@@ -105,6 +118,7 @@ def check_status(device: Optional[torch.device] = None) -> None:
         mon.host.zero_()
         raise RuntimeError("flex_block_attn_b200: " + _cabi.lib().fba_last_error().decode("utf-8", "replace"))
     _cabi.check(rc, "fba_check_status")
+    mon.poll_mapped()   # the stream is idle: whatever its kernels had to report is there
 
 
 def _maybe_check(device: torch.device) -> None:
@@ -128,6 +142,31 @@ def _new(shape_or_like, dtype=None, device=None) -> torch.Tensor:
 
 def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def _debug_flags() -> tuple[bool, bool]:
+    """(FBA_POISON_OUTPUTS, FBA_CHECK_STATUS), read once per call."""
+    env = os.environ
+    return env.get("FBA_POISON_OUTPUTS", "0") == "1", env.get("FBA_CHECK_STATUS", "0") == "1"
+
+
+def _poisoned(poison: bool, *tensors: torch.Tensor) -> None:
+    if poison:
+        for t in tensors:
+            t.fill_(float("nan"))
+
+
+# The current stream of a device by its index, without building a Stream object (2 us of a call's 15).
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    lambda index: torch.cuda.current_stream(index).cuda_stream
+
+
+def _checked(rc: int, what: str, check: bool, device: torch.device) -> None:
+    """Behind a call that reports into the mapped words: raise its error, and check the status if asked to."""
+    if rc != 0:
+        _cabi.check(rc, what)
+    if check and not torch.cuda.is_current_stream_capturing():
+        check_status(device)
 
 
 def _ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -10,7 +10,6 @@ sequence only, pages that are read may be shared.
 from __future__ import annotations
 
 import ctypes
-import os
 from dataclasses import dataclass
 from typing import Optional
 
@@ -18,7 +17,7 @@ import torch
 
 from . import _cabi
 from ._cabi import FbaPaged
-from .interface import HEAD_DIM, _new, _ptr, _scale_of, _status, _stream_ptr, check_status
+from .interface import HEAD_DIM, _checked, _debug_flags, _monitor, _poisoned, _ptr, _raw_stream, _scale_of
 from .window import _window_of
 
 _Strides3, _Strides2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
@@ -63,56 +62,63 @@ def new_paged_cache(n_pages: int, kv_heads: int, page_size: int, e4m3: bool = Fa
     return cache
 
 
-def _i32(name: str, x: torch.Tensor, shape: tuple, dev: torch.device) -> int:
-    if x.dtype != torch.int32 or x.dim() != len(shape) or not x.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous torch.int32 tensor of {len(shape)} dimension(s)")
-    if any(want is not None and want != got for want, got in zip(shape, x.shape)):
+def _i32(name: str, x: torch.Tensor, B: Optional[int], dev: torch.device) -> int:
+    """Pointer of a checked int32 [B]."""
+    if x.dtype != torch.int32 or x.dim() != 1 or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous torch.int32 tensor of 1 dimension")
+    if x.shape[0] != B:
         raise ValueError(f"{name} has the shape {tuple(x.shape)}, which does not fit")
     if x.device != dev:
         raise RuntimeError(f"{name} must be on the device of the cache")
     return x.data_ptr()
 
 
-def _cache_arg(cache: PagedKVCache, block_table: torch.Tensor, name: str = "block_table") -> tuple[FbaPaged, int]:
-    """The checked cache with its table as the C entry points take it, and the number of sequences."""
+def _table(name: str, x: torch.Tensor, dev: torch.device) -> tuple[int, int, int]:
+    """(pointer, sequences, pages per sequence) of a checked int32 [B, pages]."""
+    if x.dtype != torch.int32 or x.dim() != 2 or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous torch.int32 tensor of 2 dimensions")
+    if x.device != dev:
+        raise RuntimeError(f"{name} must be on the device of the cache")
+    return x.data_ptr(), *x.shape
+
+
+def _cache_arg(cache: PagedKVCache, block_table: torch.Tensor) -> tuple[FbaPaged, int, torch.device]:
+    """The checked cache with its table as the C entry points take it, the number of sequences, and the device."""
     k, v = cache.k, cache.v
     if not k.is_cuda:
         raise RuntimeError("the cache must be on a CUDA device (there is no CPU path)")
-    if k.dtype not in (torch.bfloat16, torch.uint8) or v.dtype != k.dtype:
+    e4m3 = k.dtype == torch.uint8
+    if not e4m3 and k.dtype != torch.bfloat16 or v.dtype != k.dtype:
         raise TypeError("cache.k and cache.v must be torch.bfloat16, or torch.uint8 holding e4m3")
-    if k.dim() != 4 or k.shape[3] != HEAD_DIM or v.shape != k.shape or not k.is_contiguous() or not v.is_contiguous():
+    shape = k.shape
+    if len(shape) != 4 or shape[3] != HEAD_DIM or v.shape != shape or not k.is_contiguous() or not v.is_contiguous():
         raise ValueError("cache.k and cache.v must be contiguous, [pages, kv heads, page size, 128]")
-    dev, e4m3 = k.device, k.dtype == torch.uint8
-    for what, x, dtype, needed in (("k_scale", cache.k_scale, torch.float32, e4m3), ("v_scale", cache.v_scale, torch.float32, e4m3),
-                                   ("weight", cache.weight, torch.float32, False), ("position", cache.position, torch.int32, False)):
-        if x is None:
-            if needed:
-                raise ValueError(f"an e4m3 cache needs {what}")
-        elif x.dtype != dtype or x.shape != k.shape[:3] or not x.is_contiguous():
-            raise ValueError(f"cache.{what} must be a contiguous {dtype} tensor, [pages, kv heads, page size]")
-        elif x.device != dev:
-            raise RuntimeError("the cache's tensors must be on one device")
+    dev = k.device
     if v.device != dev:
         raise RuntimeError("the cache's tensors must be on one device")
+    if e4m3 and (cache.k_scale is None or cache.v_scale is None):
+        raise ValueError("an e4m3 cache needs k_scale and v_scale")
     if (cache.weight is None) != (cache.position is None):
         raise ValueError("cache.weight and cache.position come together")
-    table = _i32(name, block_table, (None, None), dev)
+    for what in ("k_scale", "v_scale", "weight", "position"):
+        x = getattr(cache, what)
+        if x is not None:
+            dtype = torch.int32 if what == "position" else torch.float32
+            if x.dtype != dtype or x.shape != shape[:3] or not x.is_contiguous():
+                raise ValueError(f"cache.{what} must be a contiguous {dtype} tensor, [pages, kv heads, page size]")
+            if x.device != dev:
+                raise RuntimeError("the cache's tensors must be on one device")
+    table, B, pages = _table("block_table", block_table, dev)
     return FbaPaged(k.data_ptr(), v.data_ptr(), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(cache.weight),
-                    _ptr(cache.position), table, k.shape[0], k.shape[1], k.shape[2], block_table.shape[1],
-                    int(e4m3)), block_table.shape[0]
+                    _ptr(cache.position), table, shape[0], shape[1], shape[2], pages, e4m3), B, dev
 
 
-def _strides(name: str, x: torch.Tensor, n: int):
+def _strides(name: str, x: torch.Tensor, n: int) -> list[int]:
     """The strides of the first ``n`` dimensions; one that is never taken counts as 0."""
-    if x.stride(-1) != 1:
+    st = x.stride()
+    if st[n] != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return [x.stride(i) if x.shape[i] > 1 else 0 for i in range(n)]
-
-
-def _check(rc: int, what: str, dev: torch.device) -> None:
-    _cabi.check(rc, what)
-    if os.environ.get("FBA_CHECK_STATUS", "0") == "1" and not torch.cuda.is_current_stream_capturing():
-        check_status(dev)
+    return [s if d > 1 else 0 for s, d in zip(st[:n], x.shape)]
 
 
 def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -128,23 +134,24 @@ def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table
 
     In an e4m3 cache a row gets the scale max|x| / 448 (NaN if it is not finite) and the bytes of x / scale.
     """
-    arg, B = _cache_arg(cache, block_table)
-    dev = cache.k.device
-    for name, x in (("k", k), ("v", v)):
-        if x.dtype != torch.bfloat16 or x.dim() != 4 or x.shape[:2] != (B, arg.Hkv) or x.shape[3] != HEAD_DIM:
-            raise ValueError(f"{name} must be torch.bfloat16, [batch, kv heads, tokens, 128]")
-        if x.device != dev:
-            raise RuntimeError(f"{name} must be on the device of the cache")
-    if k.shape != v.shape:
+    arg, B, dev = _cache_arg(cache, block_table)
+    shape = k.shape
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or len(shape) != 4 or shape[:2] != (B, arg.Hkv) or shape[3] != HEAD_DIM:
+        raise ValueError("k and v must be torch.bfloat16, [batch, kv heads, tokens, 128]")
+    if v.shape != shape:
         raise ValueError("k and v must have the same shape")
-    lens = _i32("seq_lens", seq_lens, (B,), dev)
-    new = None if new_lens is None else _i32("new_lens", new_lens, (B,), dev)
-    pos = None if positions is None else _i32("positions", positions, (B,), dev)
+    if not k.device == v.device == dev:
+        raise RuntimeError("k and v must be on the device of the cache")
+    lens = _i32("seq_lens", seq_lens, B, dev)
+    new = None if new_lens is None else _i32("new_lens", new_lens, B, dev)
+    pos = None if positions is None else _i32("positions", positions, B, dev)
     out = torch.empty_like(seq_lens)
+    mon = _monitor(dev)
+    mon.poll_mapped()
     rc = _cabi.lib().fba_paged_append(ctypes.byref(arg), k.data_ptr(), v.data_ptr(), _Strides3(*_strides("k", k, 3)),
-                                      _Strides3(*_strides("v", v, 3)), B, k.shape[2], lens, new, pos, out.data_ptr(),
-                                      _status(dev).data_ptr(), _stream_ptr(dev))
-    _check(rc, "fba_paged_append", dev)
+                                      _Strides3(*_strides("v", v, 3)), B, shape[2], lens, new, pos, out.data_ptr(),
+                                      mon.mapped_ptr, _raw_stream(dev.index))
+    _checked(rc, "fba_paged_append", _debug_flags()[1], dev)
     return out
 
 
@@ -164,31 +171,35 @@ def paged_decode_attn(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
     gives zeros and -inf.  Not differentiable.
     """
     w, s = _window_of(window, sinks)
-    arg, B = _cache_arg(cache, block_table)
-    dev = cache.k.device
-    if q.dtype != torch.bfloat16 or q.dim() != 3 or q.shape[0] != B or q.shape[2] != HEAD_DIM:
+    arg, B, dev = _cache_arg(cache, block_table)
+    shape = q.shape
+    if q.dtype != torch.bfloat16 or len(shape) != 3 or shape[0] != B or shape[2] != HEAD_DIM:
         raise ValueError("q must be torch.bfloat16, [batch, heads, 128]")
     if q.device != dev:
         raise RuntimeError("q must be on the device of the cache")
-    Hq = q.shape[1]
+    Hq = shape[1]
     if Hq % arg.Hkv != 0 or Hq == 0:
         raise ValueError("the number of query heads must be a multiple of the number of kv heads")
     if accumulate and cache.weight is None:
         raise ValueError("accumulate needs a cache with weights (new_paged_cache(..., track=True))")
     if w and cache.weight is not None:
         raise ValueError("a window goes by slots, which a cache that evict_kv cuts does not keep in order")
-    lens = _i32("seq_lens", seq_lens, (B,), dev)
+    lens = _i32("seq_lens", seq_lens, B, dev)
     lib = _cabi.lib()
     n = ctypes.c_uint64(0)
-    _cabi.check(lib.fba_paged_decode_workspace_bytes(B, Hq, arg.Hkv, arg.page_size, arg.max_pages, int(accumulate),
-                                                     ctypes.byref(n)), "fba_paged_decode_workspace_bytes")
-    ws = torch.empty((n.value,), dtype=torch.uint8, device=dev) if n.value else None
-    o = _new((B, Hq, HEAD_DIM), torch.bfloat16, dev)
-    lse = _new((B, Hq), torch.float32, dev) if need_lse or accumulate else None
+    rc = lib.fba_paged_decode_workspace_bytes(B, Hq, arg.Hkv, arg.page_size, arg.max_pages, accumulate, ctypes.byref(n))
+    _cabi.check(rc, "fba_paged_decode_workspace_bytes")
+    poison, check = _debug_flags()
+    ws = q.new_empty((n.value // 4,), dtype=torch.float32) if n.value else None
+    o = q.new_empty(shape)
+    lse = q.new_empty((B, Hq), dtype=torch.float32) if need_lse or accumulate else None
+    _poisoned(poison, *(x for x in (ws, o, lse) if x is not None))
+    mon = _monitor(dev)
+    mon.poll_mapped()
     rc = lib.fba_paged_decode(ctypes.byref(arg), q.data_ptr(), _Strides2(*_strides("q", q, 2)), o.data_ptr(), _ptr(lse), B, Hq,
-                              lens, w, s, _scale_of(softmax_scale), int(accumulate), _ptr(ws), n.value,
-                              _status(dev).data_ptr(), _stream_ptr(dev))
-    _check(rc, "fba_paged_decode", dev)
+                              lens, w, s, _scale_of(softmax_scale), accumulate, _ptr(ws), n.value, mon.mapped_ptr,
+                              _raw_stream(dev.index))
+    _checked(rc, "fba_paged_decode", check, dev)
     return (o, lse) if need_lse else o
 
 
@@ -206,26 +217,30 @@ def evict_kv(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Ten
     ``paged_decode_attn`` goes on without a window.  With ``out_table`` (int32 [B, pages], pages that ``block_table`` does not
     name) the staying tokens are copied there in slot order instead, and the source, which others may share, is left.
     """
-    arg, B = _cache_arg(cache, block_table)
-    dev = cache.k.device
+    arg, B, dev = _cache_arg(cache, block_table)
     if cache.weight is None:
         raise ValueError("evict_kv needs a cache with weights (new_paged_cache(..., track=True))")
     for name, x, least in (("budget", budget, 1), ("sinks", sinks, 0), ("recent", recent, 0)):
-        if isinstance(x, bool) or not isinstance(x, int) or not least <= x < 2**31:
+        if type(x) is not int or not least <= x < 2**31:
             raise ValueError(f"{name} must be an integer from {least} on")
     if sinks + recent > budget:
         raise ValueError("sinks + recent must not exceed budget")
-    lens = _i32("seq_lens", seq_lens, (B,), dev)
-    nxt = None if next_positions is None else _i32("next_positions", next_positions, (B,), dev)
-    to = None if out_table is None else _i32("out_table", out_table, (B, None), dev)
+    lens = _i32("seq_lens", seq_lens, B, dev)
+    nxt = None if next_positions is None else _i32("next_positions", next_positions, B, dev)
+    to, to_pages = None, 0
+    if out_table is not None:
+        to, to_rows, to_pages = _table("out_table", out_table, dev)
+        if to_rows != B:
+            raise ValueError("out_table must have a row for every sequence")
     lib = _cabi.lib()
     n = ctypes.c_uint64(0)
-    _cabi.check(lib.fba_paged_evict_workspace_bytes(B, arg.Hkv, arg.page_size, arg.max_pages, budget, ctypes.byref(n)),
-                "fba_paged_evict_workspace_bytes")
-    ws = torch.empty((n.value,), dtype=torch.uint8, device=dev)
+    rc = lib.fba_paged_evict_workspace_bytes(B, arg.Hkv, arg.page_size, arg.max_pages, budget, ctypes.byref(n))
+    _cabi.check(rc, "fba_paged_evict_workspace_bytes")
+    ws = seq_lens.new_empty((n.value // 4,))
     out = torch.empty_like(seq_lens)
-    rc = lib.fba_paged_evict(ctypes.byref(arg), B, lens, budget, sinks, recent, nxt, to,
-                             0 if out_table is None else out_table.shape[1], out.data_ptr(), ws.data_ptr(), n.value,
-                             _status(dev).data_ptr(), _stream_ptr(dev))
-    _check(rc, "fba_paged_evict", dev)
+    mon = _monitor(dev)
+    mon.poll_mapped()
+    rc = lib.fba_paged_evict(ctypes.byref(arg), B, lens, budget, sinks, recent, nxt, to, to_pages, out.data_ptr(),
+                             ws.data_ptr(), n.value, mon.mapped_ptr, _raw_stream(dev.index))
+    _checked(rc, "fba_paged_evict", _debug_flags()[1], dev)
     return out

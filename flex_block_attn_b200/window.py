@@ -13,41 +13,43 @@ from typing import Optional
 import torch
 
 from . import _cabi
-from .interface import _check_qkv, _maybe_check, _monitor, _new, _ptr, _scale_of, _status, _stream_ptr
+from .interface import _check_qkv, _checked, _debug_flags, _monitor, _poisoned, _ptr, _raw_stream, _scale_of
 
 
 def _window_of(window: Optional[int], sinks: int) -> tuple[int, int]:
     """(window, sinks) as the C entry points take them: 0 for no limit."""
-    if window is not None and (isinstance(window, bool) or not isinstance(window, int) or window < 1):
+    if window is not None and (type(window) is not int or window < 1):
         raise ValueError("window must be a positive integer, or None for no limit")
-    if isinstance(sinks, bool) or not isinstance(sinks, int) or sinks < 0:
+    if type(sinks) is not int or sinks < 0:
         raise ValueError("sinks must be a non-negative integer")
     most = 2**31 - 1
     return (0 if window is None else min(window, most)), min(sinks, most)
 
 
-def _check_window_qkv(q, k, v) -> None:
+def _sizes(q, k, v) -> tuple[int, int, int, int, int]:
+    """(B, Hq, Hkv, Sq, Skv) of checked inputs."""
     _check_qkv(q, k, v)
-    if min(q.shape[:3]) < 1 or min(k.shape[1:3]) < 1:
+    (B, Hq, Sq, _), (_, Hkv, Skv, _) = q.shape, k.shape
+    if not (B and Hq and Sq and Hkv and Skv):
         raise ValueError("q, k and v must not be empty")
+    return B, Hq, Hkv, Sq, Skv
 
 
 def forward_with_window(q, k, v, window: Optional[int], sinks: int = 0, softmax_scale=None, need_lse: bool = True):
     """Forward kernel alone; returns (o bf16 [B, Hq, Sq, 128], lse fp32 [B, Hq, Sq] or None).  A row that sees no key
     (possible when Sq > Skv) is zero, its lse -inf."""
     w, s = _window_of(window, sinks)
-    _check_window_qkv(q, k, v)
-    B, Hq, Sq, _ = q.shape
-    Hkv, Skv = k.shape[1], k.shape[2]
+    B, Hq, Hkv, Sq, Skv = _sizes(q, k, v)
     dev = q.device
-    o = _new(q)
-    lse = _new((B, Hq, Sq), torch.float32, dev) if need_lse else None
-    _monitor(dev).poll()
-    with torch.cuda.device(dev):
-        rc = _cabi.lib().fba_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), B, Hq, Hkv, Sq,
-                                        Skv, w, s, _scale_of(softmax_scale), _status(dev).data_ptr(), _stream_ptr(dev))
-    _cabi.check(rc, "fba_window_fwd")
-    _maybe_check(dev)
+    poison, check = _debug_flags()
+    o = torch.empty_like(q)
+    lse = q.new_empty((B, Hq, Sq), dtype=torch.float32) if need_lse else None
+    _poisoned(poison, o, *(() if lse is None else (lse,)))
+    mon = _monitor(dev)
+    mon.poll_mapped()
+    rc = _cabi.lib().fba_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), B, Hq, Hkv, Sq, Skv, w,
+                                    s, _scale_of(softmax_scale), mon.mapped_ptr, _raw_stream(dev.index))
+    _checked(rc, "fba_window_fwd", check, dev)
     return o, lse
 
 
@@ -55,35 +57,35 @@ def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: in
     """Backward kernels; ``o`` and ``lse`` are the forward's.  Returns (dq, dk, dv) in bf16.  dK and dV are reproducible
     bit by bit; dQ is summed in fp32 in scheduling order."""
     w, s = _window_of(window, sinks)
-    _check_window_qkv(q, k, v)
-    B, Hq, Sq, _ = q.shape
-    Hkv, Skv = k.shape[1], k.shape[2]
+    B, Hq, Hkv, Sq, Skv = _sizes(q, k, v)
     dev = q.device
-    dout = dout.to(torch.bfloat16).contiguous()
-    o = o.contiguous()
-    lse = lse.reshape(B, Hq, Sq).contiguous()
+    if dout.dtype != torch.bfloat16:
+        dout = dout.to(torch.bfloat16)
+    dout, o, lse = dout.contiguous(), o.contiguous(), lse.reshape(B, Hq, Sq).contiguous()
     if lse.dtype != torch.float32:
         raise TypeError("lse must be torch.float32")
     if dout.shape != q.shape or o.shape != q.shape or o.dtype != torch.bfloat16:
         raise ValueError("o and dout must have the shape of q, and o its type")
-    if any(t.device != dev for t in (o, lse, dout)):
+    if not dout.device == o.device == lse.device == dev:
         raise RuntimeError("o, lse and dout must be on the device of q")
     lib = _cabi.lib()
-    dq, dk, dv = _new(q), _new(k), _new(v)
-    n1, n2, n3 = ctypes.c_uint64(0), ctypes.c_uint64(0), ctypes.c_uint64(0)
-    _cabi.check(lib.fba_bwd_scratch_bytes(B, Hq, Sq, ctypes.byref(n1), ctypes.byref(n2)), "fba_bwd_scratch_bytes")
-    _cabi.check(lib.fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, w, s, ctypes.byref(n3)), "fba_window_partial_bytes")
-    lse_delta = _new((n1.value // 4,), torch.float32, dev)
-    dq_accum = _new((n2.value // 4,), torch.float32, dev)
-    partial = _new((n3.value // 4,), torch.float32, dev) if n3.value else None
-    _monitor(dev).poll()
-    with torch.cuda.device(dev):
-        rc = lib.fba_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Hq, Hkv, Sq, Skv, w, s,
-                                _scale_of(softmax_scale), lse_delta.data_ptr(), dq_accum.data_ptr(), _ptr(partial),
-                                n3.value, _status(dev).data_ptr(), _stream_ptr(dev))
-    _cabi.check(rc, "fba_window_bwd")
-    _maybe_check(dev)
+    poison, check = _debug_flags()
+    n = ctypes.c_uint64(0)
+    _cabi.check(lib.fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, w, s, ctypes.byref(n)), "fba_window_partial_bytes")
+    # One buffer: row statistics, 2 floats a padded row; the dQ accumulator, 128; the partial sums.  All parts start at
+    # multiples of 1 KiB.
+    rows = B * Hq * -(-Sq // 128) * 128
+    scratch = q.new_empty((rows * 130 + n.value // 4,), dtype=torch.float32)
+    dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
+    _poisoned(poison, scratch, dq, dk, dv)
+    at = scratch.data_ptr()
+    mon = _monitor(dev)
+    mon.poll_mapped()
+    rc = lib.fba_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+                            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Hq, Hkv, Sq, Skv, w, s, _scale_of(softmax_scale),
+                            at, at + rows * 8, at + rows * 520 if n.value else None, n.value, mon.mapped_ptr,
+                            _raw_stream(dev.index))
+    _checked(rc, "fba_window_bwd", check, dev)
     return dq, dk, dv
 
 
@@ -100,8 +102,7 @@ class SlidingWindowAttnFunc(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        q, k, v, o, lse = ctx.saved_tensors
-        return *backward_with_window(q, k, v, o, lse, dout, *ctx.args), None, None, None, None
+        return *backward_with_window(*ctx.saved_tensors, dout, *ctx.args), None, None, None, None
 
 
 def sliding_window_attn_func(q, k, v, window, sinks=0, softmax_scale=None):

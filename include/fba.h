@@ -325,7 +325,8 @@ int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, c
  *   page_size    16, 32, 64, 128 or 256; max_pages * page_size < 2^30
  * Lengths (`seq_lens`, int32 [B]) are read on the device.  A page number outside 0 .. n_pages - 1, or a length outside
  * 0 .. max_pages * page_size, is never followed: the kernel leaves out the rows concerned (holds the length to the limit)
- * and reports it in the status words; fba_check_status() then returns FBA_ERR_BAD_CACHE.  Pages that a call writes must
+ * and reports it in the status words (device memory, or pinned host memory that a
+ * caller can look at without a copy); fba_check_status(), which reads device memory, then returns FBA_ERR_BAD_CACHE.  Pages that a call writes must
  * belong to one sequence only; pages that are read may be shared.
  */
 typedef struct fba_paged {
