@@ -171,7 +171,7 @@ def lib() -> ctypes.CDLL:
     L.fba_paged_append.restype = i32
     L.fba_paged_append.argtypes = [paged, vp, vp, strides, strides, i32, i32] + [vp] * 6
     L.fba_paged_decode_workspace_bytes.restype = i32
-    L.fba_paged_decode_workspace_bytes.argtypes = [i32] * 6 + [ctypes.POINTER(ctypes.c_uint64)]
+    L.fba_paged_decode_workspace_bytes.argtypes = [i32] * 7 + [ctypes.POINTER(ctypes.c_uint64)]
     L.fba_paged_decode.restype = i32
     L.fba_paged_decode.argtypes = [paged, vp, strides, vp, vp, i32, i32, vp, i32, i32, ctypes.c_float, i32, vp,
                                    ctypes.c_uint64, vp, vp]

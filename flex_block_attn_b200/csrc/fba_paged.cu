@@ -97,8 +97,12 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedDev c, con
 // with K and V^T through ldmatrix from a swizzled ring and P^T turned in registers (movmatrix).  The running maximum is
 // raised, and O^T rescaled, only when a score exceeds it by 2^8.  P is rounded to bf16 for its product like the prompt
 // kernels' P; sums and statistics are fp32.
-// e4m3: bytes become bf16 exactly (shifts and a multiplication by 2^120); a row's K scale multiplies its scores, its V
-// scale its probabilities.
+// e4m3: bytes become fp16 exactly, one conversion a pair, and the products run in fp16.  q goes to fp16 with a power of two per
+// head that brings its largest element to 2^14 .. 2^15: bf16's 8 bits stay exact down to 2^-31 of that element.  A row's K
+// scale multiplies its scores.  Its V scale multiplies its probabilities, relative to a power of two that is at least the
+// largest V scale the warp has met (O^T is rescaled when a larger one comes) and times 2^7, so that they use fp16's range:
+// below 2^15, 11 bits down to 2^-21 of the largest weight, absolute error 2^-32 of it beyond, where bf16 would keep 8
+// bits.  (Bytes to bf16 by shifts and a multiplication by 2^120 took 288 of some 420 instructions a tile.)
 constexpr int kDecThreads = 128;
 constexpr int kTileKeys = 16;
 constexpr int kDecMinTiles = 16;      // tiles a CTA gets at least: 256 keys, four tiles a warp
@@ -108,12 +112,13 @@ template <bool kE4m3>
 struct DecShape {
     static constexpr int kRow = kE4m3 ? 128 : 256;                                     // bytes
     static constexpr int kStage = 2 * kTileKeys * kRow + (kE4m3 ? 2 * kTileKeys * 4 : 0);   // K, V, scales
-    static constexpr int kStages = kE4m3 ? 5 : 3;
+    static constexpr int kStages = 3;
+    static constexpr int kCtas = kE4m3 ? 3 : 2;                                        // resident on an SM
     static constexpr int kRing = 4 * kStages * kStage;
     static constexpr int kSmem = kRing + 4 * 8 * kOStride * 4 + 4 * 8 * 2 * 4 + 4 * 8 * 4;
 };
-static_assert(2 * (DecShape<false>::kSmem + 1024) <= 233472 && 2 * (DecShape<true>::kSmem + 1024) <= 233472,
-              "two CTAs of the decode kernel must fit into an SM's shared memory");
+static_assert(DecShape<false>::kCtas * (DecShape<false>::kSmem + 1024) <= 233472 &&
+              DecShape<true>::kCtas * (DecShape<true>::kSmem + 1024) <= 233472, "the CTAs must fit into an SM's shared memory");
 
 struct DecodeParams {
     const __nv_bfloat16* q;
@@ -146,49 +151,59 @@ __device__ __forceinline__ SeqTiles seq_tiles(int n, int window, int sinks) {
     return s;
 }
 
-// Sum over the sequences of their tiles, and where tile `at` of the list [sequence][head row][tile] falls.  Every lane of
-// the warp takes part and gets the answers.
-struct ListPlace {
-    int b, before;   // the sequence, and how many tiles a head row of the sequences ahead of it has in all
-};
-__device__ __forceinline__ int list_total(const PagedDev& c, const DecodeParams& p) {
-    const int lane = threadIdx.x & 31;
-    int sum = 0;
-    for (int b = lane; b < p.B; b += 32) sum += seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks).nt;
-    return __reduce_add_sync(0xffffffffu, sum);
+// Tiles a CTA takes.
+__device__ __forceinline__ long long list_piece(long long total, int n_ctas) {
+    const long long per = (total + n_ctas - 1) / n_ctas;
+    return per < kDecMinTiles ? kDecMinTiles : per;
 }
-// The last sequence whose tiles begin at or before `at` (a place in one head row's concatenation, scaled by `rows`).
-__device__ __forceinline__ ListPlace list_find(const PagedDev& c, const DecodeParams& p, long long at, int rows) {
+
+// Where a CTA's piece of the list [sequence][head row][tile] begins.  Every lane of the warp takes part and gets the
+// answers.
+struct ListPlace {
+    int b, length;       // the sequence, and its length in slots
+    long long in;        // tiles of the sequence's head rows ahead of the piece
+    long long count;     // tiles of the piece; 0: there is none
+};
+__device__ __forceinline__ ListPlace list_place(const PagedDev& c, const DecodeParams& p, int cta, int rows) {
     const int lane = threadIdx.x & 31;
-    ListPlace r = {0, 0};
+    auto load = [&](int base, int& n) {   // tiles of one head row of the lane's sequence
+        n = base + lane < p.B ? paged_length(c, p.seq_lens, base + lane, p.status) : 0;
+        return base + lane < p.B ? seq_tiles(n, p.window, p.sinks).nt : 0;
+    };
+    int n0, all = 0;
+    const int nt0 = load(0, n0);   // kept: with up to 32 sequences nothing is loaded twice
+    for (int base = 32; base < p.B; base += 32) {
+        int n;
+        all += load(base, n);
+    }
+    all = __reduce_add_sync(0xffffffffu, all + nt0);
+    const long long total = static_cast<long long>(all) * rows, per = list_piece(total, p.n_ctas), at = per * cta;
+    ListPlace r = {0, 0, 0, 0};
+    if (at >= total) return r;
+    r.count = min(per, total - at);
     int before = 0;
     for (int base = 0; base < p.B; base += 32) {
-        const int b = base + lane;
-        const int nt = b < p.B ? seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks).nt : 0;
+        int n = n0, nt = nt0;
+        if (base > 0) nt = load(base, n);
         int upto = nt;
 #pragma unroll
         for (int s = 1; s < 32; s <<= 1) {
             const int x = __shfl_up_sync(0xffffffffu, upto, s);
             if (lane >= s) upto += x;
         }
-        // sequences with tiles whose end lies behind `at`: the first of them is the place
+        // the first sequence with tiles whose end lies behind `at`
         const uint32_t hit = __ballot_sync(0xffffffffu, nt > 0 && static_cast<long long>(before + upto) * rows > at);
         if (hit) {
             const int first = __ffs(hit) - 1;
             r.b = base + first;
-            r.before = before + __shfl_sync(0xffffffffu, upto - nt, first);
+            r.length = __shfl_sync(0xffffffffu, n, first);
+            r.in = at - static_cast<long long>(before + __shfl_sync(0xffffffffu, upto - nt, first)) * rows;
             return r;
         }
         before += __shfl_sync(0xffffffffu, upto, 31);
     }
-    r.b = p.B;
-    r.before = before;
+    r.count = 0;   // not reached: the last tile lies behind `at`
     return r;
-}
-// Tiles a CTA takes.
-__device__ __forceinline__ long long list_piece(long long total, int n_ctas) {
-    const long long per = (total + n_ctas - 1) / n_ctas;
-    return per < kDecMinTiles ? kDecMinTiles : per;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
@@ -220,19 +235,30 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4],
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Four e4m3 bytes -> two bf16 pairs, exactly: (bytes 0, 2) and (bytes 1, 3).  Sign and the seven other bits moved to
-// their places in bf16 read as the value times 2^-120 (exponent bias 127 instead of 7), subnormals included.  The one
-// pattern that this does not cover is NaN (0x7f, 0xff), which reads as 480.
-__device__ __forceinline__ void e4m3_to_bf16(uint32_t r, uint32_t& even, uint32_t& odd) {
-    const uint32_t e = ((r << 8) & 0x80008000u) | ((r << 4) & 0x07f007f0u);
-    const uint32_t o = (r & 0x80008000u) | ((r >> 4) & 0x07f007f0u);
-    constexpr uint32_t k2p120 = 0x7b807b80u;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(even) : "r"(e), "r"(k2p120));
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(odd) : "r"(o), "r"(k2p120));
+// The same in fp16.
+__device__ __forceinline__ void mma_16816_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+// Four e4m3 bytes -> two fp16 pairs, exactly: (bytes 0, 1) and (bytes 2, 3).
+__device__ __forceinline__ void e4m3_to_f16(uint32_t r, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(r));
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// 2^e for e in -126 .. 127.
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+// Exponent of a positive finite number, rounded down (-127 for subnormals and 0).
+__device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23) - 127; }
 
 template <bool kE4m3, int NT>
-__global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const PagedDev c, const DecodeParams p) {
+__global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas : 2) paged_decode_kernel(const PagedDev c, const DecodeParams p) {
     using Sh = DecShape<kE4m3>;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_launch_dependents();
@@ -261,19 +287,14 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
         first.end = first.s.nt;
         first.left = 0;
     } else {
-        const long long total = static_cast<long long>(list_total(c, p)) * rows_per_seq;
-        const long long per = list_piece(total, p.n_ctas);
-        const long long at = per * blockIdx.x;
-        if (at >= total) return;
-        const ListPlace place = list_find(c, p, at, rows_per_seq);
+        const ListPlace place = list_place(c, p, blockIdx.x, rows_per_seq);
+        if (place.count == 0) return;
         first.b = place.b;
-        first.s = seq_tiles(paged_length(c, p.seq_lens, place.b, p.status), p.window, p.sinks);
-        const long long in = at - static_cast<long long>(place.before) * rows_per_seq;   // within the sequence
-        first.hr = static_cast<int>(in / first.s.nt);
-        first.i = static_cast<int>(in - static_cast<long long>(first.hr) * first.s.nt);
-        const long long mine = min(per, total - at);
-        first.end = static_cast<int>(min(static_cast<long long>(first.s.nt), first.i + mine));
-        first.left = mine - (first.end - first.i);
+        first.s = seq_tiles(place.length, p.window, p.sinks);
+        first.hr = static_cast<int>(place.in / first.s.nt);
+        first.i = static_cast<int>(place.in - static_cast<long long>(first.hr) * first.s.nt);
+        first.end = static_cast<int>(min(static_cast<long long>(first.s.nt), first.i + place.count));
+        first.left = place.count - (first.end - first.i);
     }
     // The next row's part of the piece; the caller has checked that tiles are left.
     auto next_row = [&](Cursor& r) {
@@ -361,25 +382,43 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
     while (true) {
         const int h = cur.hr / p.q_tiles, q0 = h * p.group + (cur.hr - h * p.q_tiles) * 8 * NT;   // first query head
         const int heads = min(8 * NT, (h + 1) * p.group - q0);
-        // q as the right operand: of k-step ks thread (g, t4) holds head g, two dims and two more 8 further on; with
-        // e4m3 the dims follow the byte order of e4m3_to_bf16.
+        // q as the right operand: of k-step ks thread (g, t4) holds head g, two dims and two more; with e4m3 the dims follow
+        // the order of a row's bytes: 4 t4 .. 4 t4 + 3.
         uint32_t qf[NT][16];
+        float q_mul[NT];   // e4m3: what undoes the power of two of head g
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             const bool real = 8 * nt + g < heads;
             const uint32_t* src = reinterpret_cast<const uint32_t*>(p.q + cur.b * p.qs[0] + (q0 + (real ? 8 * nt + g : 0)) * p.qs[1]);
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) {
-                if (kE4m3) {
-                    const uint32_t x = real ? src[ks * 8 + 2 * t4] : 0u, y = real ? src[ks * 8 + 2 * t4 + 1] : 0u;
-                    qf[nt][2 * ks] = __byte_perm(x, y, 0x5410);
-                    qf[nt][2 * ks + 1] = __byte_perm(x, y, 0x7632);
-                } else {
-                    qf[nt][2 * ks] = real ? src[ks * 8 + t4] : 0u;
-                    qf[nt][2 * ks + 1] = real ? src[ks * 8 + 4 + t4] : 0u;
-                }
+                qf[nt][2 * ks] = real ? src[ks * 8 + (kE4m3 ? 2 * t4 : t4)] : 0u;
+                qf[nt][2 * ks + 1] = real ? src[ks * 8 + (kE4m3 ? 2 * t4 + 1 : t4 + 4)] : 0u;
+            }
+            if (kE4m3) {
+                float most = 0.f;
+                auto lo = [](uint32_t x) { return __uint_as_float(x << 16); };
+                auto hi = [](uint32_t x) { return __uint_as_float(x & 0xffff0000u); };
+#pragma unroll
+                for (int x = 0; x < 16; ++x) most = max3(most, fabsf(lo(qf[nt][x])), fabsf(hi(qf[nt][x])));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+                most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+                // 14 minus its exponent, within what has a power of two and an inverse; infinities stay what they are
+                const int e = most > 0.f && most < INFINITY ? max(-112, min(112, 14 - exponent(most))) : 0;
+                const float up = pow2(e);
+                q_mul[nt] = pow2(-e);
+#pragma unroll
+                for (int x = 0; x < 16; ++x) qf[nt][x] = pack_f16x2(lo(qf[nt][x]) * up, hi(qf[nt][x]) * up);
             }
         }
+        // The scores' columns are heads 2 t4 and 2 t4 + 1.
+        float q_mul2[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                q_mul2[nt][x] = p.scale_log2 * (kE4m3 ? __shfl_sync(0xffffffffu, q_mul[nt], (2 * t4 + x) * 4) : 1.f);
+        float v_ref = 0.f, v_inv = 0.f;   // e4m3: the power of two that V scales are relative to, and 2^7 over it
         float acc[NT][8][4];
         float m[NT][2], l[NT][2];
 #pragma unroll
@@ -413,14 +452,14 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
                     for (int ci = 0; ci < 4; ++ci) {
                         uint32_t r[4], a[2][4];
                         ldmatrix_x4(r, row + (((2 * ci + hi) ^ sw) << 4));
-                        e4m3_to_bf16(r[0], a[0][0], a[0][2]);
-                        e4m3_to_bf16(r[1], a[0][1], a[0][3]);
-                        e4m3_to_bf16(r[2], a[1][0], a[1][2]);
-                        e4m3_to_bf16(r[3], a[1][1], a[1][3]);
+                        e4m3_to_f16(r[0], a[0][0], a[0][2]);
+                        e4m3_to_f16(r[1], a[0][1], a[0][3]);
+                        e4m3_to_f16(r[2], a[1][0], a[1][2]);
+                        e4m3_to_f16(r[3], a[1][1], a[1][3]);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma_16816(s2[nt][0], a[0], qf[nt][4 * ci], qf[nt][4 * ci + 1]);
-                            mma_16816(s2[nt][1], a[1], qf[nt][4 * ci + 2], qf[nt][4 * ci + 3]);
+                            mma_16816_f16(s2[nt][0], a[0], qf[nt][4 * ci], qf[nt][4 * ci + 1]);
+                            mma_16816_f16(s2[nt][1], a[1], qf[nt][4 * ci + 2], qf[nt][4 * ci + 3]);
                         }
                     }
                 } else {
@@ -439,21 +478,39 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
             }
             // Elements: (key g, head 2 t4), (g, + 1), (key g + 8, 2 t4), (g + 8, + 1).
             const uint32_t vis = ring_vis[stage];
-            float mul[2] = {p.scale_log2, p.scale_log2};
+            float mul[2] = {1.f, 1.f};
             float vs[2] = {1.f, 1.f};
             if (kE4m3) {
                 const float* sc = reinterpret_cast<const float*>(smem + (sk - smem_u32(smem)) + 2 * kTileKeys * Sh::kRow);
-                mul[0] *= sc[g];
-                mul[1] *= sc[g + 8];
+                mul[0] = sc[g];
+                mul[1] = sc[g + 8];
                 vs[0] = (vis >> g) & 1u ? sc[16 + g] : 0.f;   // the scales are loaded for all rows, whatever they hold
                 vs[1] = (vis >> (g + 8)) & 1u ? sc[24 + g] : 0.f;
+                const float most = fmaxf(vs[0], vs[1]);
+                if (__any_sync(0xffffffffu, most > v_ref && most < INFINITY)) {
+                    float top = most < INFINITY ? most : 0.f;
+#pragma unroll
+                    for (int sh = 4; sh < 32; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, sh));
+                    const int e = max(-119, min(126, exponent(top) + 1));
+                    const float down = v_ref * pow2(-e);   // below 1; 0 ahead of the first
+                    v_ref = pow2(e);
+                    v_inv = pow2(7 - e);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+#pragma unroll
+                            for (int x = 0; x < 4; ++x) acc[nt][j][x] *= down;
+                }
+                vs[0] *= v_inv;
+                vs[1] *= v_inv;
             }
             bool over = false;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    s[nt][e] = (vis >> (g + 8 * (e >> 1))) & 1u ? s[nt][e] * mul[e >> 1] : -INFINITY;
+                    s[nt][e] = (vis >> (g + 8 * (e >> 1))) & 1u ? s[nt][e] * (kE4m3 ? mul[e >> 1] * q_mul2[nt][e & 1] : q_mul2[nt][e & 1]) : -INFINITY;
                     over = over || s[nt][e] > m[nt][e & 1] + 8.f;
                 }
             }
@@ -496,8 +553,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
                     l[nt][e & 1] += e4[e];
                     if (kE4m3) e4[e] *= vs[e >> 1];
                 }
-                pb[nt][0] = movmatrix(pack_bf16x2(e4[0], e4[1]));
-                pb[nt][1] = movmatrix(pack_bf16x2(e4[2], e4[3]));
+                pb[nt][0] = movmatrix(kE4m3 ? pack_f16x2(e4[0], e4[1]) : pack_bf16x2(e4[0], e4[1]));
+                pb[nt][1] = movmatrix(kE4m3 ? pack_f16x2(e4[2], e4[3]) : pack_bf16x2(e4[2], e4[3]));
             }
             if (kE4m3) {
                 const uint32_t row = sv + (lane & 15) * Sh::kRow;
@@ -506,14 +563,17 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
                 for (int ci = 0; ci < 4; ++ci) {
                     uint32_t r[4], a[2][4];
                     ldmatrix_x4_trans(r, row + (((2 * ci + hi) ^ sw) << 4));
-                    e4m3_to_bf16(r[0], a[0][0], a[0][1]);
-                    e4m3_to_bf16(r[1], a[0][2], a[0][3]);
-                    e4m3_to_bf16(r[2], a[1][0], a[1][1]);
-                    e4m3_to_bf16(r[3], a[1][2], a[1][3]);
+                    // bytes: two dims of a key, then of the next; wanted: a dim's two keys
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) r[x] = __byte_perm(r[x], 0u, 0x3120);
+                    e4m3_to_f16(r[0], a[0][0], a[0][1]);
+                    e4m3_to_f16(r[1], a[0][2], a[0][3]);
+                    e4m3_to_f16(r[2], a[1][0], a[1][1]);
+                    e4m3_to_f16(r[3], a[1][2], a[1][3]);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma_16816(acc[nt][2 * ci], a[0], pb[nt][0], pb[nt][1]);
-                        mma_16816(acc[nt][2 * ci + 1], a[1], pb[nt][0], pb[nt][1]);
+                        mma_16816_f16(acc[nt][2 * ci], a[0], pb[nt][0], pb[nt][1]);
+                        mma_16816_f16(acc[nt][2 * ci + 1], a[1], pb[nt][0], pb[nt][1]);
                     }
                 }
             } else {
@@ -548,8 +608,9 @@ __global__ void __launch_bounds__(kDecThreads, 2) paged_decode_kernel(const Page
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     float* dst = ex_o + (warp * 8 + 2 * t4 + x) * kOStride + 16 * j;
-                    dst[kE4m3 ? 2 * g : g] = acc[nt][j][x];
-                    dst[kE4m3 ? 2 * g + 1 : g + 8] = acc[nt][j][x + 2];
+                    const float back = kE4m3 ? v_ref * 0.0078125f : 1.f;
+                    dst[kE4m3 ? 2 * g : g] = acc[nt][j][x] * back;
+                    dst[kE4m3 ? 2 * g + 1 : g + 8] = acc[nt][j][x + 2] * back;
                 }
             }
             __syncthreads();
@@ -624,19 +685,16 @@ __device__ __forceinline__ float part_scale(float m, float top) { return top == 
 // loads of a warp's parts are independent of one another.  (One block per row with its heads in turn and the sums carried
 // from part to part took 11 us for 64 sequences, 24 us for 16 of 8 heads a kv head, 36 us for two long ones.)
 template <int NT>
-__global__ void __launch_bounds__(128) paged_join_kernel(const PagedDev c, const DecodeParams p) {
+__device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, int b, int hr, int hq) {
     __shared__ float4 s_o[4][32];
     __shared__ float s_l[4];
-    const int rows_per_seq = c.Hkv * p.q_tiles;
-    const int b = blockIdx.x / rows_per_seq, hr = blockIdx.x - b * rows_per_seq;
     const int h = hr / p.q_tiles, q0 = h * p.group + (hr - h * p.q_tiles) * 8 * NT;
-    const int hq = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (hq >= min(8 * NT, (h + 1) * p.group - q0)) return;
     const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
     const RowParts r = row_parts(c, p, b, hr, s.nt);
     if (r.whole) return;
-    const long long slot0 = static_cast<long long>(blockIdx.x) * (8 * NT) + hq;   // a part x CTAs on is x * 8 NT slots on
+    const long long slot0 = (static_cast<long long>(b) * c.Hkv * p.q_tiles + hr) * (8 * NT) + hq;   // a part x CTAs on is x * 8 NT slots on
     const float top = parts_max(p, r, slot0, 8 * NT);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
@@ -665,30 +723,41 @@ __global__ void __launch_bounds__(128) paged_join_kernel(const PagedDev c, const
     if (p.lse && d == 0) p.lse[out] = some ? (top + log2f(sum)) * kLn2 : -INFINITY;
 }
 
-// Adds the probabilities to the weights, from the scores and the parts' sums.  blockIdx.x = row, blockIdx.y = a stretch of
-// kWeighSlots slots.
-constexpr int kWeighSlots = 1024;
+// Adds the probabilities to the weights, from the scores and the parts' sums: a block of the join's launch for each stretch of
+// kWeighSlots slots.  What does not depend on the sums is under way before they are looked at.
+constexpr int kWeighSlots = 256;
 template <int NT>
-__global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDev c, const DecodeParams p) {
+__device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, int b, int h, int stretch) {
     __shared__ float s_lse[8 * NT];   // in units of log2
-    const int rows_per_seq = c.Hkv;   // host-checked: q_tiles is 1
-    const int b = blockIdx.x / rows_per_seq, h = blockIdx.x - b * rows_per_seq;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    pdl_wait();
     const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
-    if (static_cast<int>(blockIdx.y) * kWeighSlots >= s.n) return;
-    const RowParts r = row_parts(c, p, b, h, s.nt);
+    const int j0 = stretch * kWeighSlots;
+    if (j0 >= s.n) return;
     const long long q0 = static_cast<long long>(b) * p.Hq + h * p.group;
-    for (int hq = warp; hq < p.group; hq += 8) {
+    constexpr int kSlots = kWeighSlots / 128;
+    long long row[kSlots];
+    float x[kSlots][8 * NT], old[kSlots];
+#pragma unroll
+    for (int u = 0; u < kSlots; ++u) {
+        const int j = j0 + u * 128 + threadIdx.x;
+        row[u] = j < s.n ? paged_row(c, b, h, j, p.status) : -1;
+#pragma unroll
+        for (int hq = 0; hq < 8 * NT; ++hq)
+            x[u][hq] = j < s.n && hq < p.group ? p.scores[(q0 + hq) * p.score_stride + j] : -INFINITY;
+    }
+#pragma unroll
+    for (int u = 0; u < kSlots; ++u) old[u] = row[u] >= 0 ? c.weight[row[u]] : 0.f;
+    const RowParts r = row_parts(c, p, b, h, s.nt);
+    for (int hq = warp; hq < p.group; hq += 4) {
         float lse;
         if (r.whole) {
             lse = p.lse[q0 + hq] * kLog2e;
         } else {
-            const long long slot0 = static_cast<long long>(blockIdx.x) * (8 * NT) + hq;
+            const long long slot0 = (static_cast<long long>(b) * c.Hkv + h) * (8 * NT) + hq;
             const float top = parts_max(p, r, slot0, 8 * NT);
             float l = 0.f;
-            for (int x = r.first + lane; x <= r.last; x += 32) {
-                const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[slot0 + static_cast<long long>(x) * (8 * NT)];
+            for (int part = r.first + lane; part <= r.last; part += 32) {
+                const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[slot0 + static_cast<long long>(part) * (8 * NT)];
                 l = fmaf(part_scale(ml.x, top), ml.y, l);
             }
 #pragma unroll
@@ -699,16 +768,26 @@ __global__ void __launch_bounds__(256) paged_weigh_kernel(const PagedDev c, cons
     }
     __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kWeighSlots / 256; ++u) {
-        const int j = blockIdx.y * kWeighSlots + u * 256 + threadIdx.x;
-        if (j >= s.n) continue;
-        const long long row = paged_row(c, b, h, j, p.status);
-        if (row < 0) continue;
+    for (int u = 0; u < kSlots; ++u) {
+        if (row[u] < 0) continue;
         float w = 0.f;
-#pragma unroll 8
-        for (int hq = 0; hq < p.group; ++hq) w += ex2_approx(p.scores[(q0 + hq) * p.score_stride + j] - s_lse[hq]);
-        c.weight[row] += w;
+#pragma unroll
+        for (int hq = 0; hq < 8 * NT; ++hq)
+            if (hq < p.group) w += ex2_approx(x[u][hq] - s_lse[hq]);
+        c.weight[row[u]] = old[u] + w;
     }
+}
+
+// The launch behind the decode kernel: blockIdx.x = row, blockIdx.y = a query head of it to join, or, behind those, a stretch
+// of its slots to weigh.
+template <int NT>
+__global__ void __launch_bounds__(128) paged_finish_kernel(const PagedDev c, const DecodeParams p, int heads) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int rows_per_seq = c.Hkv * p.q_tiles;
+    const int b = blockIdx.x / rows_per_seq, hr = blockIdx.x - b * rows_per_seq;
+    if (static_cast<int>(blockIdx.y) < heads) join<NT>(c, p, b, hr, blockIdx.y);
+    else weigh<NT>(c, p, b, hr, blockIdx.y - heads);   // host-checked: one group of query heads, so a row is a kv head
 }
 
 int paged_args(const char* who, const fba_paged_t* cache, int B, PagedDev* dev) {
@@ -783,16 +862,19 @@ struct DecodePlan {
     long long rows;
     uint64_t part_o, part_ml, scores;   // bytes of the workspace, each rounded up to 256
 };
-DecodePlan decode_plan(int B, int Hq, int Hkv, int page_size, int max_pages, bool accumulate) {
+DecodePlan decode_plan(int B, int Hq, int Hkv, int page_size, int max_pages, bool e4m3, bool accumulate) {
     DecodePlan d;
     const int group = Hq / Hkv;
     d.nt = group > 8 ? 2 : 1;
     d.q_tiles = (group + 8 * d.nt - 1) / (8 * d.nt);
     d.rows = static_cast<long long>(B) * Hkv * d.q_tiles;
     const long long tiles = static_cast<long long>(max_pages) * page_size / kTileKeys;   // a row has at most
-    // One CTA per row where a row is short: nothing is joined then.  Otherwise as many as are resident.
+    // One CTA per row where a row is short: nothing is joined then.  Otherwise as many as are resident.  (Two, three and four
+    // times as many, us: 64 sequences 183 -> 179, 178, 177; two long e4m3 ones 101 -> 105, 109, 115; 16 with a window 51 ->
+    // 55, 58, 60: a CTA's start and end cost about 4 us, uneven SMs less.)
     const long long pieces = (d.rows * tiles + kDecMinTiles - 1) / kDecMinTiles;
-    d.n_ctas = tiles <= 2 * kDecMinTiles ? 0 : static_cast<int>(pieces < 2 * 148 ? pieces : 2 * 148);
+    const long long want = 148 * (d.nt == 1 && e4m3 ? 3 : 2);
+    d.n_ctas = tiles <= 2 * kDecMinTiles ? 0 : static_cast<int>(pieces < want ? pieces : want);
     auto up = [](uint64_t n) { return (n + 255) / 256 * 256; };
     const uint64_t slots = d.n_ctas ? (d.n_ctas + d.rows) * 8 * d.nt : 0;
     d.part_o = up(slots * 128 * sizeof(float));
@@ -810,10 +892,10 @@ int launch_decode(const PagedDev& c, const DecodeParams& p, const DecodePlan& d,
     }
     const unsigned rows = static_cast<unsigned>(d.rows);
     int rc = launch_chained(paged_decode_kernel<kE4m3, NT>, dim3(d.n_ctas ? d.n_ctas : rows), kDecThreads, smem, stream, c, p);
-    if (rc == FBA_OK && d.n_ctas)
-        rc = launch_chained(paged_join_kernel<NT>, dim3(rows, p.group < 8 * NT ? p.group : 8 * NT), 128, 0, stream, c, p);
-    if (rc == FBA_OK && p.scores)
-        rc = launch_chained(paged_weigh_kernel<NT>, dim3(rows, (d.score_stride + kWeighSlots - 1) / kWeighSlots), 256, 0, stream, c, p);
+    const int heads = d.n_ctas == 0 ? 0 : p.group < 8 * NT ? p.group : 8 * NT;
+    const int stretches = p.scores ? (d.score_stride + kWeighSlots - 1) / kWeighSlots : 0;
+    if (rc == FBA_OK && heads + stretches > 0)
+        rc = launch_chained(paged_finish_kernel<NT>, dim3(rows, heads + stretches), 128, 0, stream, c, p, heads);
     return rc;
 }
 }  // namespace
@@ -828,12 +910,12 @@ static int decode_args(const char* who, int B, int Hq, int Hkv, int page_size, i
     return FBA_OK;
 }
 
-extern "C" int fba_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages, int accumulate,
-                                                uint64_t* bytes) {
+extern "C" int fba_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages, int e4m3,
+                                                int accumulate, uint64_t* bytes) {
     const int rc = decode_args("fba_paged_decode_workspace_bytes: bad size", B, Hq, Hkv, page_size, max_pages);
     if (rc != FBA_OK) return rc;
     if (!bytes) return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode_workspace_bytes: null pointer argument");
-    const DecodePlan d = decode_plan(B, Hq, Hkv, page_size, max_pages, accumulate != 0);
+    const DecodePlan d = decode_plan(B, Hq, Hkv, page_size, max_pages, e4m3 != 0, accumulate != 0);
     *bytes = d.part_o + d.part_ml + d.scores;
     return FBA_OK;
 }
@@ -853,13 +935,15 @@ extern "C" int fba_paged_decode(const fba_paged_t* cache, const void* q, const i
     if (window < 0 || sinks < 0) return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: window and sinks must not be negative");
     if (!(softmax_scale > 0.f) || !(softmax_scale < INFINITY))
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: softmax_scale must be positive and finite");
+    const DecodePlan d = decode_plan(B, Hq, c.Hkv, c.page_size, c.max_pages, cache->e4m3 != 0, accumulate != 0);
     if (accumulate && (!c.weight || window != 0 || !lse))
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: accumulation needs a cache with weights, lse, and no window");
+    if (accumulate && d.score_stride > 65000 * kWeighSlots)
+        return set_error(FBA_ERR_TOO_LARGE, "fba_paged_decode: accumulation takes tables of at most 16.6 million slots");
     if (accumulate && Hq / c.Hkv > 16)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: accumulation takes at most 16 query heads a kv head");
     if (reinterpret_cast<uintptr_t>(q) % 4 != 0 || q_strides[0] % 2 != 0 || q_strides[1] % 2 != 0)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: q must be 4-byte aligned, its strides multiples of 2");
-    const DecodePlan d = decode_plan(B, Hq, c.Hkv, c.page_size, c.max_pages, accumulate != 0);
     const uint64_t need = d.part_o + d.part_ml + d.scores;
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return set_error(FBA_ERR_BAD_ARG,

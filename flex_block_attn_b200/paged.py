@@ -187,7 +187,8 @@ def paged_decode_attn(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
     lens = _i32("seq_lens", seq_lens, B, dev)
     lib = _cabi.lib()
     n = ctypes.c_uint64(0)
-    rc = lib.fba_paged_decode_workspace_bytes(B, Hq, arg.Hkv, arg.page_size, arg.max_pages, accumulate, ctypes.byref(n))
+    rc = lib.fba_paged_decode_workspace_bytes(B, Hq, arg.Hkv, arg.page_size, arg.max_pages, arg.e4m3, accumulate,
+                                               ctypes.byref(n))
     _cabi.check(rc, "fba_paged_decode_workspace_bytes")
     poison, check = _debug_flags()
     ws = q.new_empty((n.value // 4,), dtype=torch.float32) if n.value else None

@@ -359,15 +359,15 @@ int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, con
  *   j < sinks (window 0: all).  q, o: bf16 [B, Hq, 128], q element (b, h, d) at b * q_strides[0] + h * q_strides[1] + d
  *   (multiples of 2), o contiguous; lse fp32 [B, Hq] or NULL.  n = 0: zeros, lse = -inf.
  * Rows outside what a query sees are not read: whatever they hold, NaN included, does not matter.
- * e4m3: a row stands for byte values times its scale; the NaN bytes 0x7f and 0xff read as 480 and -480 (a row that is not
- * finite is marked by its scale).
+ * e4m3: a row stands for its bytes' values times its scale.
  * accumulate != 0 (window 0, lse not NULL, at most 16 query heads a kv head): weight[slot] += the sum of the slot's
  * probabilities over the query heads of its kv head, in a fixed order.
  * The tiles of all sequences are divided evenly over the SMs; parts of one sequence are joined by a second kernel
  * through `workspace` (256-byte aligned, fba_paged_decode_workspace_bytes()).  Results do not depend on the order in which
  * CTAs run.  They may differ in the last bit with the other sequences' lengths, which move the seams.
  */
-int fba_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages, int accumulate, uint64_t* bytes);
+int fba_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages, int e4m3, int accumulate,
+                                     uint64_t* bytes);
 int fba_paged_decode(const fba_paged_t* cache, const void* q, const int64_t* q_strides, void* o, float* lse, int B, int Hq,
                      const int32_t* seq_lens, int window, int sinks, float softmax_scale, int accumulate, void* workspace,
                      uint64_t workspace_bytes, uint32_t* status, void* stream);

@@ -115,27 +115,28 @@ def test_c_decode_refuses_bad_arguments(lib):
     assert call(acc=1) == -1 and call(struct(**track), acc=1, window=5) == -1 and call(struct(**track), acc=1, lse=None) == -1
     assert call(struct(**track), acc=1, Hq=34) == -1
     long = {"max_pages": 1000}
-    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 1000, 0, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 1000, 0, 0, ctypes.byref(n)) == 0 and n.value > 0
     assert call(struct(**long), ws=None) == -1 and call(struct(**long), n=n.value - 1) == -1
     assert call(struct(**long), ws=ctypes.c_void_p(128)) == -1
     assert b"workspace" in lib.fba_last_error()
-    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 3, 0, ctypes.byref(n)) == 0 and n.value == 0
-    assert lib.fba_paged_decode_workspace_bytes(1, 4, 3, 16, 3, 0, ctypes.byref(n)) == -1
-    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 3, 0, None) == -1
-    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 2**26, 0, ctypes.byref(n)) == -5
-    assert lib.fba_paged_decode_workspace_bytes(65535, 4, 2, 256, 2**21, 0, ctypes.byref(n)) == -5
+    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 3, 0, 0, ctypes.byref(n)) == 0 and n.value == 0
+    assert lib.fba_paged_decode_workspace_bytes(1, 4, 3, 16, 3, 0, 0, ctypes.byref(n)) == -1
+    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 3, 0, 0, None) == -1
+    assert lib.fba_paged_decode_workspace_bytes(1, 4, 2, 16, 2**26, 0, 0, ctypes.byref(n)) == -5
+    assert lib.fba_paged_decode_workspace_bytes(65535, 4, 2, 256, 2**21, 0, 0, ctypes.byref(n)) == -5
 
 
+@pytest.mark.parametrize("e4m3", [0, 1])
 @pytest.mark.parametrize("B,Hq,Hkv,page,mp", [(1, 1, 1, 16, 40), (64, 32, 8, 64, 128), (300, 34, 2, 16, 100)])
-def test_workspace_holds_a_slot_for_every_seam(lib, B, Hq, Hkv, page, mp):
+def test_workspace_holds_a_slot_for_every_seam(lib, B, Hq, Hkv, page, mp, e4m3):
     """A CTA's part of a row goes to slot CTA + row; both count from 0."""
     n = ctypes.c_uint64()
-    assert lib.fba_paged_decode_workspace_bytes(B, Hq, Hkv, page, mp, 0, ctypes.byref(n)) == 0
+    assert lib.fba_paged_decode_workspace_bytes(B, Hq, Hkv, page, mp, e4m3, 0, ctypes.byref(n)) == 0
     group = Hq // Hkv
     nt = 2 if group > 8 else 1
     rows = B * Hkv * -(-group // (8 * nt))
     tiles = mp * page // 16
-    ctas = min(296, -(-rows * tiles // 16))
+    ctas = min(148 * (3 if e4m3 and nt == 1 else 2), -(-rows * tiles // 16))
     assert n.value >= (ctas + rows) * 8 * nt * (128 + 2) * 4
 
 

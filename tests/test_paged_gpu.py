@@ -2,7 +2,9 @@
 
 Tolerance of o: each probability is rounded to bf16 (relative u = 2^-8) for its product and the result once more, so an
 element is off by at most u * (sum p |v| + |o|); the rest is fp32: scores are sums of 128 products, off by at most
-128 * 2^-23 * scale * |q| |k| (dq below), which moves a probability by that share.
+128 * 2^-23 * scale * |q| |k| (dq below), which moves a probability by that share.  In an e4m3 cache a weight times its V scale is held in fp16 as a multiple of
+2^-7 R, where R is at most twice the largest V scale and the largest weight at least 1: below fp16's normal range it is
+off by at most 2^-25 of that, so n keys add at most n * 2^-32 * R * 448 to an element, whatever the key's own weight.
 """
 import math
 
@@ -30,6 +32,10 @@ def check(q, pools, table, lens, o, lse, window=None, sinks=0, scale=None):
     dq = 128 * 2.0**-23 * s * float(q.double().norm(dim=-1).max()) * kmax
     assert torch.isfinite(o.float()).all()
     bound = U * (around + want.abs()) + (2 * dq + 1e-6) * around + 1e-30
+    if "v_scale" in pools:
+        largest = [max([float(orc.rows_of(pools["v_scale"], table[b], int(n), h).max()) for h in range(pools["k"].shape[1])]) if n else 0.0
+                   for b, n in enumerate(lens)]
+        bound = bound + torch.tensor([int(n) * 2.0**-31 * x * 448 for n, x in zip(lens, largest)], dtype=torch.float64)[:, None, None]
     assert ((o.cpu().double() - want).abs() <= bound).all(), float(((o.cpu().double() - want).abs() / bound).max())
     if lse is not None:
         none = wl == -math.inf
