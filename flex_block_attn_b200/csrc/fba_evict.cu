@@ -167,7 +167,19 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
 
     // T, and how many tokens with a smaller key there are.
     uint32_t prefix = 0, below = 0;
-    if (leave > 0) {
+    if (leave == 1) {   // one token too many, as at every step of serving within a budget: the smallest key, in one round
+        uint32_t least = 0xffffffffu;
+        for (int i = begin + tid; i < end; i += kEvThreads) least = min(least, key_of(i));
+        least = __reduce_min_sync(0xffffffffu, least);
+        if (lane == 0) sh.scan[warp] = least;
+        __syncthreads();
+        prefix = __reduce_min_sync(0xffffffffu, sh.scan[lane]);
+        if (ctas > 1) {
+            if (tid == 0) sh.digit = prefix;
+            cluster.sync();
+            for (int r = 0; r < ctas; ++r) prefix = min(prefix, *cluster.map_shared_rank(&sh.digit, r));
+        }
+    } else if (leave > 1) {
         uint32_t rank_left = leave - 1;   // of the last token that leaves, among those that share the digits so far
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
@@ -365,11 +377,14 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     p.recent = recent;
     p.out_pages = out_pages;
     p.list = list;
-    // The keys of a CTA's slots stay in shared memory beside the histogram, with a cluster of up to 8 CTAs if need be.
+    // The keys of a CTA's slots stay in shared memory beside the histogram, with a cluster of up to 8 CTAs if need be; a
+    // cluster also where there are idle SMs and long stretches to go through (32 heads of up to 32768 slots, selection and
+    // copies: 80 us with one CTA a head, 64 with two, 55 with four).
     constexpr long long kMostKeys = 200 * 1024 / 4;
     const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
     int ctas = 1;
     while (ctas < 8 && cap > kMostKeys * ctas) ctas *= 2;
+    while (ctas < 8 && heads * ctas * 2 <= 148 && cap / (ctas * 2) >= 2048) ctas *= 2;
     const long long room = ((cap + ctas - 1) / ctas + 31) / 32 * 32;
     p.key_room = room <= kMostKeys ? static_cast<int>(room) : 0;
     // The most rows that a head can have to copy.
