@@ -104,8 +104,9 @@ struct BwdParams {
     int parts;             // 1: one CTA per (key tile, kv head); else the last tiles are split into this many CTAs each:
     int split_from;        //   those from this one on (kv head * n_ntiles + tile),
     int n_whole;           //   behind this many CTAs with whole groups
-    WindowDev win;         // fba_window_bwd alone (n_whole: its key tiles with sinks, which are split into `parts`)
-    int Sq;
+    WindowDev win;         // fba_window_bwd alone (n_whole: its key tiles with sinks, which are split into `parts`), as are:
+    int Sq, n_bhk;         //   kv heads in all
+    int heads_at_once;     //   kv heads whose tiles take turns in the grid
 };
 
 // ------------------------------------------------------------------------------------------
@@ -288,15 +289,22 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const int group = p.Hq / p.Hkv;
     int bhk = blockIdx.y, nt = blockIdx.x, part0 = 0, hr = group;   // bhk: b * Hkv + kv head
     float* partial = nullptr;
-    if constexpr (kWindow && kSplit) {
-        const int split_ctas = p.n_whole * p.parts;
-        if (nt < split_ctas) {
-            const int cta = nt;
-            nt = cta / p.parts;
-            part0 = cta - nt * p.parts;
-            partial = p.partial + (static_cast<long long>(bhk) * split_ctas + cta) * 32768;
+    if constexpr (kWindow) {
+        // One row of CTAs, the longest lists first: the tiles with sinks (or their parts), then the others, the first tiles
+        // of `heads_at_once` kv heads, their second ones, ...
+        const int sink_ctas = p.n_whole * (kSplit ? p.parts : 1), cta = blockIdx.x, body = cta - sink_ctas * p.n_bhk;
+        if (body < 0) {
+            bhk = cta / sink_ctas;
+            nt = cta - bhk * sink_ctas;
+            if (kSplit) {
+                part0 = nt % p.parts;
+                nt /= p.parts;
+                partial = p.partial + cta * 32768LL;
+            }
         } else {
-            nt -= split_ctas - p.n_whole;
+            const GridItem item = grid_item(body, p.n_ntiles - p.n_whole, p.n_bhk, p.heads_at_once);
+            bhk = item.head;
+            nt = p.n_whole + item.level;
         }
     } else if (kSplit) {
         const int cta = nt - p.n_whole;
@@ -1123,6 +1131,13 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     p.n_whole = sink_tiles;
     p.win = win;
     p.Sq = Sq;
+    p.n_bhk = static_cast<int>(n_bhk);
+    // As many kv heads take turns as have their rows of Q, dO and the dQ accumulator in L2 together.  Us, one at a time ->
+    // with this rule: causal, 8192 rows, 16 heads on 4: 873 -> 689 (2; all four: 701); causal, 4096 rows, 8 heads: 148 ->
+    // 112; causal, 4 x 4096, 32 on 8: 1512 -> 1396 (8; all 32: 1506); 12288 rows, window 4096, 16 on 4: 955 -> 941 (2);
+    // causal, 30720, 24 heads: 12311 -> 12604 (4; all 24: 17160).
+    const long long at_once = kGridL2 / (static_cast<long long>(Sq) * 1024 * (Hq / Hkv));
+    p.heads_at_once = static_cast<int>(at_once < 1 ? 1 : at_once < n_bhk ? at_once : n_bhk);
     auto kernel = parts > 1 ? fba_bwd_kernel<true, true, true> : fba_bwd_kernel<true, false, true>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBwdSmemBytes)) !=
         cudaSuccess) {
@@ -1130,7 +1145,7 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
         return set_error(FBA_ERR_LAUNCH, "fba_window_bwd: cannot raise the dynamic shared memory limit");
     }
     timing_mark(2, true, stream);
-    kernel<<<dim3(n_ntiles + (parts - 1) * sink_tiles, static_cast<unsigned>(n_bhk)), kBwdThreads, kBwdSmemBytes, stream>>>(
+    kernel<<<static_cast<unsigned>((n_ntiles + (parts - 1) * sink_tiles) * n_bhk), kBwdThreads, kBwdSmemBytes, stream>>>(
         tm_q, tm_k, tm_v, tm_do, tm_dk, tm_dv, p);
     rc = check_launch("fba_bwd_kernel");
     timing_mark(2, false, stream);

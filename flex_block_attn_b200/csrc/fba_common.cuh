@@ -34,6 +34,17 @@ inline ListDev to_dev(const fba_list_t& l) {
 struct WindowDev {
     int q_off, window, sinks;
 };
+// What heads that take turns may read and write in all; L2 holds 126 MB.
+constexpr long long kGridL2 = 128ll << 20;
+// The x-th of n_heads * levels work items: `at_once` heads at a time take turns, level by level.
+struct GridItem {
+    int head, level;
+};
+__device__ __forceinline__ GridItem grid_item(int x, int levels, int n_heads, int at_once) {
+    const int first = x / (levels * at_once) * at_once, in = x - first * levels;
+    const int heads = min(at_once, n_heads - first), level = in / heads;
+    return {first + in - level * heads, level};
+}
 // Checks the arguments of the window entry points and fills `win` (fba_api.cu).
 int window_args(const char* who, int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks, float softmax_scale,
                 WindowDev* win);

@@ -52,7 +52,9 @@ struct FwdParams {
     uint32_t* status;
     int n_mtiles, Sq, Hq, Hkv;
     float scale_log2;      // softmax scale * log2(e)
-    WindowDev win;         // fba_window_fwd alone
+    WindowDev win;         // fba_window_fwd alone, as are:
+    int n_pairs, n_bh;     //   pairs of query tiles per head, heads
+    int heads_at_once;     //   heads whose pairs take turns in the grid
 };
 
 // The key tiles of a pair of query tiles under a sliding window, without a list in memory.  Tile t (0: A, 1: B) sees
@@ -146,12 +148,17 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
 
     const int warp = warp_uniform(static_cast<int>(threadIdx.x >> 5));
     const int lane = threadIdx.x & 31;
-    const int bh = blockIdx.y;
+    int bh = blockIdx.y, window_pair = 0;
+    if constexpr (kWindow) {
+        // One row of CTAs, the longest lists first: the last pairs of `heads_at_once` heads, their last but one, ...
+        const GridItem item = grid_item(blockIdx.x, p.n_pairs, p.n_bh, p.heads_at_once);
+        bh = item.head;
+        window_pair = p.n_pairs - 1 - item.level;
+    }
     // Work item of this CTA: the blockIdx.x-th entry of the (batch, head)'s longest-first order when
     // one is given (CTAs are dispatched in blockIdx order, so the shortest items of the grid run
     // last and the tail of the launch stays short), else blockIdx.x itself.
-    // Under a window the later rows have the longer lists.
-    const int pair = kWindow ? static_cast<int>(gridDim.x - 1 - blockIdx.x)
+    const int pair = kWindow ? window_pair
                      : p.list.order
                          ? p.list.order[static_cast<long long>(p.list.bh_stride ? bh : 0) * gridDim.x + blockIdx.x]
                          : static_cast<int>(blockIdx.x);
@@ -645,6 +652,18 @@ static int launch_fwd(const void* q, const void* k, const void* v, void* o, floa
     p.Hkv = Hkv;
     p.scale_log2 = softmax_scale * kLog2e;
     dim3 grid((n_mtiles + 1) / 2, B * Hq);
+    p.n_pairs = p.n_bh = p.heads_at_once = 0;
+    if (win) {
+        p.n_pairs = static_cast<int>(grid.x);
+        p.n_bh = static_cast<int>(grid.y);
+        // As many heads take turns as have their keys and values in L2 together; one by one, each head's long lists come
+        // behind the short ones of the head before it, the last head's too.  Us, one head at a time -> with this rule: 12288
+        // rows, window 4096, 16 heads on 4: 320 -> 300; causal, 8192 rows, 16 on 4: 273 -> 226; causal, 4 x 4096, 32 on 8:
+        // 508 -> 482; causal, 30720, 24 heads: 4188 -> 4136 (8 at a time; all 24: 4275).
+        const long long kv_heads = kGridL2 / (static_cast<long long>(Skv) * 512), at_once = (kv_heads > 1 ? kv_heads : 1) * (Hq / Hkv);
+        p.heads_at_once = at_once < p.n_bh ? static_cast<int>(at_once) : p.n_bh;
+        grid = dim3(grid.x * grid.y);
+    }
     timing_mark(1, true, stream);
     kernel<<<grid, kFwdThreads, kFwdSmemBytes, stream>>>(tm_q, tm_k, tm_v, tm_o, p);
     rc = check_launch("fba_fwd_kernel");
