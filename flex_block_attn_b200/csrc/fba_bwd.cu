@@ -92,6 +92,12 @@ static_assert(kBwdSmemBytes <= 232448, "exceeds the 227 KiB shared memory of an 
 #define FBA_RED_SLEEP_NS 32
 #endif
 
+// Key tiles of a kv head whose steps are divided over several CTAs under a window: the first `sinks` tiles into
+// `sink_parts` each, the next `lead` ones into `lead_parts`.
+struct WindowSplit {
+    int sinks, sink_parts, lead, lead_parts;
+};
+
 struct BwdParams {
     ListDev list;          // key-major: rows = key tiles / rows_div, entries = query tiles / sub
     const float2* ld;      // [B*Hq, nMt, 2, 128]: per query tile 128 x (-lse*log2e), then 128 x (-delta*scale)
@@ -104,7 +110,8 @@ struct BwdParams {
     int parts;             // 1: one CTA per (key tile, kv head); else the last tiles are split into this many CTAs each:
     int split_from;        //   those from this one on (kv head * n_ntiles + tile),
     int n_whole;           //   behind this many CTAs with whole groups
-    WindowDev win;         // fba_window_bwd alone (n_whole: its key tiles with sinks, which are split into `parts`), as are:
+    WindowDev win;         // fba_window_bwd alone, as are:
+    WindowSplit wsplit;    //   which tiles' steps are divided
     int Sq, n_bhk;         //   kv heads in all
     int heads_at_once;     //   kv heads whose tiles take turns in the grid
 };
@@ -183,10 +190,11 @@ struct PartialSums {
     const float* partial;   // see BwdParams
     __nv_bfloat16 *dv, *dk;
     int first_row, n_blocks, split_from, parts, n_ntiles, Skv;
+    int tile0;              // of the n_ntiles tiles per kv head that the indices count
 };
 __device__ __forceinline__ void sum_partials(const PartialSums& s, int block, uint2* tile) {
     const int w = block & 3, z = (block >> 2) & 1, t = block >> 3;   // row group, dV / dK, split tile
-    const int bhk = (s.split_from + t) / s.n_ntiles, nt = s.split_from + t - bhk * s.n_ntiles;
+    const int bhk = (s.split_from + t) / s.n_ntiles, nt = s.split_from + t - bhk * s.n_ntiles + s.tile0;
     const float4* src = reinterpret_cast<const float4*>(s.partial) + (t * s.parts * 2LL + z) * 4096 + w * 256 + threadIdx.x;
     float4 v[4];   // column chunks of 32
 #pragma unroll
@@ -220,11 +228,12 @@ __device__ __forceinline__ void sum_partials(const PartialSums& s, int block, ui
 }
 
 __global__ void __launch_bounds__(256, 6) bwd_convert_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq,
-                                                            int Sq, int n_mtiles, PartialSums sums) {
+                                                            int Sq, int n_mtiles, PartialSums sums, PartialSums more) {
     __shared__ uint2 tile[128 * 33];
     if (static_cast<int>(blockIdx.y) >= sums.first_row) {
         const int block = (blockIdx.y - sums.first_row) * gridDim.x + blockIdx.x;
-        if (block < sums.n_blocks) sum_partials(sums, block, tile);
+        if (block < sums.n_blocks + more.n_blocks)
+            sum_partials(block < sums.n_blocks ? sums : more, block < sums.n_blocks ? block : block - sums.n_blocks, tile);
         return;
     }
     const int mt = blockIdx.x;
@@ -263,9 +272,9 @@ __device__ __forceinline__ void red_add_v4(float* addr, float a, float b, float 
 // (fba_bwd_dq.cu): no dQ GEMM, no drain, no reductions.  kSplit: some key tiles are split by query heads (SplitPlan);
 // decided at run time it cost every CTA some 200 clocks, 2 % of a call with lists of one entry.
 // kWindow: the query tiles of a key tile follow from a sliding window and sinks and are one range, the same for every head;
-// probabilities outside the mask become zero one by one.  A key tile with sinks is seen by every query behind it, and so
-// has a list many times the others' length: with kSplit its steps (query heads one after the other, query tiles in
-// order) are divided over `parts` CTAs at the front of the grid.
+// probabilities outside the mask become zero one by one.  With kSplit the steps of the tiles with the longest lists (query
+// heads one after the other, query tiles in order) are divided over several CTAs each, at the front of the grid
+// (window_split has the rule).
 template <bool kWithDq, bool kSplit, bool kWindow = false>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -288,23 +297,27 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     // split tiles.  Which tiles are split does not depend on the order, and so neither do the sums.
     const int group = p.Hq / p.Hkv;
     int bhk = blockIdx.y, nt = blockIdx.x, part0 = 0, hr = group;   // bhk: b * Hkv + kv head
+    int n_parts = 1;
     float* partial = nullptr;
     if constexpr (kWindow) {
-        // One row of CTAs, the longest lists first: the tiles with sinks (or their parts), then the others, the first tiles
-        // of `heads_at_once` kv heads, their second ones, ...
-        const int sink_ctas = p.n_whole * (kSplit ? p.parts : 1), cta = blockIdx.x, body = cta - sink_ctas * p.n_bhk;
-        if (body < 0) {
-            bhk = cta / sink_ctas;
-            nt = cta - bhk * sink_ctas;
-            if (kSplit) {
-                part0 = nt % p.parts;
-                nt /= p.parts;
-                partial = p.partial + cta * 32768LL;
-            }
+        // One row of CTAs, the longest lists first: the parts of divided tiles, then the others, the first tiles of
+        // `heads_at_once` kv heads, their second ones, ...
+        const WindowSplit& w = p.wsplit;
+        const int sink_ctas = w.sinks * w.sink_parts * p.n_bhk, lead_ctas = w.lead * w.lead_parts * p.n_bhk, cta = blockIdx.x;
+        if (kSplit && cta < sink_ctas + lead_ctas) {
+            const bool sink = cta < sink_ctas;
+            const int tiles = sink ? w.sinks : w.lead, in = sink ? cta : cta - sink_ctas;
+            n_parts = sink ? w.sink_parts : w.lead_parts;
+            bhk = in / (tiles * n_parts);
+            nt = in - bhk * (tiles * n_parts);
+            part0 = nt % n_parts;
+            nt = nt / n_parts + (sink ? 0 : w.sinks);
+            partial = p.partial + cta * 32768LL;
         } else {
-            const GridItem item = grid_item(body, p.n_ntiles - p.n_whole, p.n_bhk, p.heads_at_once);
+            const int split = kSplit ? w.sinks + w.lead : 0;
+            const GridItem item = grid_item(kSplit ? cta - sink_ctas - lead_ctas : cta, p.n_ntiles - split, p.n_bhk, p.heads_at_once);
             bhk = item.head;
-            nt = p.n_whole + item.level;
+            nt = split + item.level;
         }
     } else if (kSplit) {
         const int cta = nt - p.n_whole;
@@ -349,8 +362,8 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         n_total = cnt * group;
         win_cnt = max(cnt, 1);
         if (kSplit && partial != nullptr) {
-            win_step0 = static_cast<int>(static_cast<long long>(part0) * n_total / p.parts);
-            n_total = static_cast<int>(static_cast<long long>(part0 + 1) * n_total / p.parts) - win_step0;
+            win_step0 = static_cast<int>(static_cast<long long>(part0) * n_total / n_parts);
+            n_total = static_cast<int>(static_cast<long long>(part0 + 1) * n_total / n_parts) - win_step0;
         }
         hr = 1;   // one loop over all steps
     } else {
@@ -1035,11 +1048,11 @@ extern "C" int fba_bwd_split(const void* q, const void* k, const void* v, const 
         }
     }
     PartialSums sums = {partial, static_cast<__nv_bfloat16*>(dv), static_cast<__nv_bfloat16*>(dk), static_cast<int>(n_bhq),
-                        8 * split.tail, split.from, split.parts, n_ntiles, Skv};
+                        8 * split.tail, split.from, split.parts, n_ntiles, Skv, 0};
     if (qmajor) {
         if (split.parts > 1) {   // no dQ rows here: the query-major kernel writes them
             sums.first_row = 0;
-            bwd_convert_kernel<<<sums.n_blocks, 256, 0, stream>>>(nullptr, nullptr, Sq, n_mtiles, sums);
+            bwd_convert_kernel<<<sums.n_blocks, 256, 0, stream>>>(nullptr, nullptr, Sq, n_mtiles, sums, PartialSums{});
             if ((rc = check_launch("bwd_convert_kernel")) != FBA_OK) return rc;
         }
         return launch_bwd_dq(tm_q, tm_k, tm_v, tm_do, tm_dq, *q2k, lse_delta, status, n_mtiles, n_bhq, Hq, Hkv,
@@ -1047,31 +1060,72 @@ extern "C" int fba_bwd_split(const void* q, const void* k, const void* v, const 
     }
     {
         dim3 grid(n_mtiles, static_cast<unsigned>(n_bhq + (sums.n_blocks + n_mtiles - 1) / n_mtiles));
-        bwd_convert_kernel<<<grid, 256, 0, stream>>>(dq_accum, static_cast<__nv_bfloat16*>(dq), Sq, n_mtiles, sums);
+        bwd_convert_kernel<<<grid, 256, 0, stream>>>(dq_accum, static_cast<__nv_bfloat16*>(dq), Sq, n_mtiles, sums, PartialSums{});
         if ((rc = check_launch("bwd_convert_kernel")) != FBA_OK) return rc;
     }
     return FBA_OK;
 }
 
-// Split of the key tiles with sinks under a window: how many CTAs divide one such tile's steps.
+// Division of the longest lists under a window.
 //
-// Every query behind a sink sees it, so its tile has group * ceil(Sq / 128) steps where the others have about
-// group * (window / 128 + 1); unsplit it would be what the whole launch waits for.  A part gets no fewer steps than the
-// other tiles have, nor than half of an SM's share of all steps: shorter ones end no launch sooner.
-static int window_parts(int B, int Hq, int Hkv, int Sq, int Skv, const WindowDev& win) {
-    const int sink_tiles = (win.sinks + 127) / 128, n_ntiles = (Skv + 127) / 128;
-    if (sink_tiles == 0 || win.window >= Skv) return 1;   // no sinks, or a causal mask without a window
+// A CTA's list is group * (query tiles that see the key tile) steps: the whole sequence behind a tile with sinks, up to the
+// window for the others.  Where there are few kv heads, or many query heads to each, the others can be longer than an SM's
+// share of all steps, too: from one and a half times that share on they are divided into parts of about the share.  A tile
+// with sinks gets parts of the others' length (what they are divided into), or of half the share where that is longer.  No
+// part has fewer than kLeastSteps (a CTA's start and end cost about as much); 592 parts in all, 74 MB of partial sums.
+// Backward, us, undivided -> divided (sinks are in both columns): 16 heads on 1, 4096 rows, window 512: 241 -> 99; 8 on
+// 1, 2000 rows, causal: 312 -> 75; 1 head, 12000 rows, causal: 242 -> 171; 8 on 2, 1000 rows, window 300: 63 -> 40.  Parts of
+// half the share, and dividing from there on, lost as much where the tiles fill the chip: 8 heads, 4096 rows, causal: 112
+// -> 142; 16 on 4, 8192 rows, causal: 687 -> 738.
+constexpr int kLeastSteps = 6, kMostParts = 32, kMostWindowParts = 4 * kSms;
+static WindowSplit window_split(int B, int Hq, int Hkv, int Sq, int Skv, const WindowDev& win) {
     const long long group = Hq / Hkv, n_bhk = static_cast<long long>(B) * Hkv;
-    const int first = win.q_off < 0 ? -win.q_off / 128 : 0;   // rows ahead of every key see nothing
-    const long long sink_steps = group * ((Sq + 127) / 128 - first);
-    long long tile_steps = group * ((win.window + 254) / 128 + 1);
-    if (tile_steps > sink_steps) tile_steps = sink_steps;
-    const long long all = n_bhk * (sink_tiles * sink_steps + (n_ntiles - sink_tiles) * tile_steps);
-    const long long least = tile_steps > all / (2 * kSms) ? tile_steps : all / (2 * kSms);
-    long long parts = (sink_steps + least - 1) / least;
-    const long long room = 4 * kSms / (n_bhk * sink_tiles);   // at most 592 parts in all: 74 MB of partial sums
-    if (parts > room) parts = room;
-    return parts < 1 ? 1 : static_cast<int>(parts);
+    const int n_nt = (Skv + 127) / 128;
+    const int sinks = win.window < Skv ? (win.sinks + 127) / 128 : 0;   // without a window they change nothing
+    auto steps_of = [&](int nt) {   // of key tile nt, as the kernel counts them
+        const long long key = nt * 128ll, lo = key > win.q_off ? key - win.q_off : 0;
+        long long hi = nt < sinks ? Sq - 1 : key + 126 + win.window - win.q_off;
+        if (hi > Sq - 1) hi = Sq - 1;
+        return hi < lo ? 0ll : group * (hi / 128 - lo / 128 + 1);
+    };
+    // All steps; of long sequences every so many'th tile stands for its neighbours.
+    long long all = 0;
+    const int stride = n_nt > 4096 ? n_nt / 2048 : 1;
+    for (int nt = 0; nt < n_nt; nt += stride) all += steps_of(nt) * (nt < sinks ? 1 : stride);
+    all *= n_bhk;
+    auto parts_of = [](long long steps, long long share) {
+        const long long n = (steps + share - 1) / share;
+        return static_cast<int>(n < 1 ? 1 : n < kMostParts ? n : kMostParts);
+    };
+    WindowSplit w = {0, 1, 0, 1};
+    long long room = kMostWindowParts;
+    // The first tile without sinks has the longest list of those.
+    long long longest = sinks < n_nt ? steps_of(sinks) : 0, share = (all + kSms - 1) / kSms;
+    if (share < kLeastSteps) share = kLeastSteps;
+    const int lead_parts = 2 * longest > 3 * share ? parts_of(longest, share) : 1;
+    if (sinks > 0) {
+        long long least = (longest + lead_parts - 1) / lead_parts;
+        if (least < all / (2 * kSms)) least = all / (2 * kSms);
+        if (least < kLeastSteps) least = kLeastSteps;
+        const long long fit = room / (n_bhk * sinks);
+        int parts = parts_of(steps_of(0), least);
+        if (parts > fit) parts = static_cast<int>(fit);
+        if (parts > 1) {
+            w.sinks = sinks;
+            w.sink_parts = parts;
+            room -= n_bhk * sinks * parts;
+        }
+    }
+    if (lead_parts > 1 && w.sinks == sinks) {   // (the divided tiles are the first ones)
+        int lead = 0;
+        while (sinks + lead < n_nt && (lead + 1) * n_bhk * lead_parts <= room && 4 * steps_of(sinks + lead) > 5 * share) ++lead;
+        w.lead = lead;
+        w.lead_parts = lead ? lead_parts : 1;
+    }
+    return w;
+}
+static uint64_t window_partial_bytes_of(const WindowSplit& w, long long n_bhk) {
+    return static_cast<uint64_t>(n_bhk) * (w.sinks * w.sink_parts + w.lead * w.lead_parts) * 2 * 128 * 128 * sizeof(float);
 }
 
 extern "C" int fba_window_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks, uint64_t* bytes) {
@@ -1079,8 +1133,7 @@ extern "C" int fba_window_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv,
     const int rc = window_args("fba_window_partial_bytes", B, Hq, Hkv, Sq, Skv, window, sinks, 1.f, &win);
     if (rc != FBA_OK) return rc;
     if (!bytes) return set_error(FBA_ERR_BAD_ARG, "fba_window_partial_bytes: null pointer argument");
-    const int parts = window_parts(B, Hq, Hkv, Sq, Skv, win);
-    *bytes = parts == 1 ? 0 : static_cast<uint64_t>(B) * Hkv * ((win.sinks + 127) / 128) * parts * 2 * 128 * 128 * sizeof(float);
+    *bytes = window_partial_bytes_of(window_split(B, Hq, Hkv, Sq, Skv, win), static_cast<long long>(B) * Hkv);
     return FBA_OK;
 }
 
@@ -1095,15 +1148,14 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     WindowDev win;
     int rc = window_args("fba_window_bwd", B, Hq, Hkv, Sq, Skv, window, sinks, softmax_scale, &win);
     if (rc != FBA_OK) return rc;
-    uint64_t need = 0;
-    if ((rc = fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, window, sinks, &need)) != FBA_OK) return rc;
+    const long long n_bhq = static_cast<long long>(B) * Hq, n_bhk = static_cast<long long>(B) * Hkv;
+    const WindowSplit w = window_split(B, Hq, Hkv, Sq, Skv, win);
+    const uint64_t need = window_partial_bytes_of(w, n_bhk);
     if (need != 0 && (!partial || partial_bytes < need || reinterpret_cast<uintptr_t>(partial) % 16 != 0))
         return set_error(FBA_ERR_BAD_ARG, "fba_window_bwd: partial must be 16-byte aligned, of fba_window_partial_bytes() bytes");
-    const int n_mtiles = (Sq + 127) / 128, n_ntiles = (Skv + 127) / 128, sink_tiles = (win.sinks + 127) / 128;
-    const int parts = need ? window_parts(B, Hq, Hkv, Sq, Skv, win) : 1;
-    const long long n_bhq = static_cast<long long>(B) * Hq, n_bhk = static_cast<long long>(B) * Hkv;
-    const long long sum_blocks = parts > 1 ? 8 * n_bhk * sink_tiles : 0;
-    if (n_bhq + (sum_blocks + n_mtiles - 1) / n_mtiles > 65535)
+    const int n_mtiles = (Sq + 127) / 128, n_ntiles = (Skv + 127) / 128;
+    const long long n_split = n_bhk * (w.sinks + w.lead);   // divided tiles
+    if (n_bhq + (8 * n_split + n_mtiles - 1) / n_mtiles > 65535)
         return set_error(FBA_ERR_TOO_LARGE, "fba_window_bwd: B * Hq and the sums of the split tiles exceed 65535 rows of a grid");
 
     CUtensorMap tm_q, tm_k, tm_v, tm_do, tm_dk, tm_dv;
@@ -1127,9 +1179,8 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     p.scale = softmax_scale;
     p.partial = partial;
     p.n_ntiles = n_ntiles;
-    p.parts = parts;
-    p.n_whole = sink_tiles;
     p.win = win;
+    p.wsplit = w;
     p.Sq = Sq;
     p.n_bhk = static_cast<int>(n_bhk);
     // As many kv heads take turns as have their rows of Q, dO and the dQ accumulator in L2 together.  Us, one at a time ->
@@ -1138,22 +1189,29 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     // causal, 30720, 24 heads: 12311 -> 12604 (4; all 24: 17160).
     const long long at_once = kGridL2 / (static_cast<long long>(Sq) * 1024 * (Hq / Hkv));
     p.heads_at_once = static_cast<int>(at_once < 1 ? 1 : at_once < n_bhk ? at_once : n_bhk);
-    auto kernel = parts > 1 ? fba_bwd_kernel<true, true, true> : fba_bwd_kernel<true, false, true>;
+    auto kernel = n_split ? fba_bwd_kernel<true, true, true> : fba_bwd_kernel<true, false, true>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kBwdSmemBytes)) !=
         cudaSuccess) {
         cudaGetLastError();
         return set_error(FBA_ERR_LAUNCH, "fba_window_bwd: cannot raise the dynamic shared memory limit");
     }
     timing_mark(2, true, stream);
-    kernel<<<static_cast<unsigned>((n_ntiles + (parts - 1) * sink_tiles) * n_bhk), kBwdThreads, kBwdSmemBytes, stream>>>(
+    const long long ctas = n_bhk * (n_ntiles + w.sinks * (w.sink_parts - 1) + w.lead * (w.lead_parts - 1));
+    kernel<<<static_cast<unsigned>(ctas), kBwdThreads, kBwdSmemBytes, stream>>>(
         tm_q, tm_k, tm_v, tm_do, tm_dk, tm_dv, p);
     rc = check_launch("fba_bwd_kernel");
     timing_mark(2, false, stream);
     if (rc != FBA_OK) return rc;
     PartialSums sums = {partial, static_cast<__nv_bfloat16*>(dv), static_cast<__nv_bfloat16*>(dk), static_cast<int>(n_bhq),
-                        static_cast<int>(sum_blocks), 0, parts, sink_tiles, Skv};
-    dim3 grid(n_mtiles, static_cast<unsigned>(n_bhq + (sum_blocks + n_mtiles - 1) / n_mtiles));
-    bwd_convert_kernel<<<grid, 256, 0, stream>>>(dq_accum, static_cast<__nv_bfloat16*>(dq), Sq, n_mtiles, sums);
+                        static_cast<int>(8 * n_bhk * w.sinks), 0, w.sink_parts, w.sinks, Skv, 0};
+    PartialSums more = sums;
+    more.partial = partial + n_bhk * w.sinks * w.sink_parts * 32768;
+    more.n_blocks = static_cast<int>(8 * n_bhk * w.lead);
+    more.parts = w.lead_parts;
+    more.n_ntiles = w.lead;
+    more.tile0 = w.sinks;
+    dim3 grid(n_mtiles, static_cast<unsigned>(n_bhq + (8 * n_split + n_mtiles - 1) / n_mtiles));
+    bwd_convert_kernel<<<grid, 256, 0, stream>>>(dq_accum, static_cast<__nv_bfloat16*>(dq), Sq, n_mtiles, sums, more);
     return check_launch("bwd_convert_kernel");
 }
 

@@ -70,9 +70,9 @@ def test_c_entry_points_refuse_bad_arguments():
     assert fwd((1, 2, 1, 2**30, 2**30)) == _cabi.FBA_ERR_TOO_LARGE
     assert lib.fba_window_partial_bytes(1, 2, 1, 16, 16, 4, 0, None) == -1
     assert lib.fba_window_partial_bytes(1, 2, 1, 16, 16, -4, 0, ctypes.byref(n)) == -1
-    # no sinks, no window: nothing is split
+    # enough kv heads for the chip: nothing is split
     for window, sinks in ((100, 0), (0, 5), (5000, 5)):
-        assert lib.fba_window_partial_bytes(1, 8, 1, 5000, 5000, window, sinks, ctypes.byref(n)) == 0 and n.value == 0
+        assert lib.fba_window_partial_bytes(8, 64, 64, 5000, 5000, window, sinks, ctypes.byref(n)) == 0 and n.value == 0
     assert lib.fba_window_partial_bytes(1, 8, 1, 5000, 5000, 100, 5, ctypes.byref(n)) == 0
     assert 0 < n.value <= 592 * 2**17 and n.value % 2**17 == 0
     bwd = [some] * 9 + [1, 8, 1, 5000, 5000, 100, 5, 0.1, some, some]
