@@ -325,7 +325,10 @@ using namespace fba;
 namespace {
 // Up to so many rows a head are copied by the CTA that chose them; more by a kernel of their own, whose launch costs
 // less than leaving most SMs idle.
-constexpr int kMoveHere = 256;
+#ifndef MVH
+#define MVH 256
+#endif
+constexpr int kMoveHere = MVH;
 int evict_list(int page_size, int max_pages, int budget) {
     const long long cap = static_cast<long long>(max_pages) * page_size;
     return static_cast<int>(cap < budget ? cap : budget);

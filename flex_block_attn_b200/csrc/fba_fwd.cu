@@ -55,6 +55,7 @@ struct FwdParams {
     WindowDev win;         // fba_window_fwd alone, as are:
     int n_pairs, n_bh;     //   pairs of query tiles per head, heads
     int heads_at_once;     //   heads whose pairs take turns in the grid
+    int one_tile;          //   not 0: a CTA has one query tile instead of a pair
 };
 
 // The key tiles of a pair of query tiles under a sliding window, without a list in memory.  Tile t (0: A, 1: B) sees
@@ -166,13 +167,14 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
     const int bhk = (bh / p.Hq) * p.Hkv + (bh % p.Hq) / hr;
 
     // Per-tile list rows and lengths (identical in every thread).
-    const int mt0 = 2 * pair, mt1 = 2 * pair + 1;
-    const bool tile1_valid = mt1 < p.n_mtiles;
+    const bool one_tile = kWindow && p.one_tile != 0;
+    const int mt0 = one_tile ? pair : 2 * pair, mt1 = mt0 + 1;
+    const bool tile1_valid = mt1 < p.n_mtiles && !one_tile;
     long long lrow0 = 0, lrow1 = 0;
     int sub = 1, n0, n1;
     WindowWalk walk;
     if constexpr (kWindow) {
-        walk = window_walk(p.win, mt0, p.Sq);
+        walk = window_walk(p.win, mt0, one_tile ? min(p.Sq, mt0 * 128 + 128) : p.Sq);
         n0 = warp_uniform(walk.n[0]);
         n1 = warp_uniform(walk.n[1]);
     } else {
@@ -415,7 +417,7 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const int nt = t ? n1 : n0;
         const long long lrow = t ? lrow1 : lrow0;
         const uint32_t sQt = t ? sQ1 : sQ0;
-        const bool tile_valid = mt < p.n_mtiles;
+        const bool tile_valid = mt < p.n_mtiles && !(one_tile && t);
         const float c = p.scale_log2;
         const int g = row >> 4;
         const bool tracer = (warp & 3) == 0 && lane == 0;
@@ -652,8 +654,12 @@ static int launch_fwd(const void* q, const void* k, const void* v, void* o, floa
     p.Hkv = Hkv;
     p.scale_log2 = softmax_scale * kLog2e;
     dim3 grid((n_mtiles + 1) / 2, B * Hq);
-    p.n_pairs = p.n_bh = p.heads_at_once = 0;
+    p.n_pairs = p.n_bh = p.heads_at_once = p.one_tile = 0;
     if (win) {
+        // Where all tiles fit on the SMs by themselves, a tile's steps need not wait for another's.  Us, pairs -> tiles: 1
+        // head, 12000 rows, causal 152 -> 125; 8 heads, 2000 rows 33.7 -> 29.5; 8 heads, 1000 rows 18.4 -> 16.4.
+        p.one_tile = static_cast<long long>(n_mtiles) * B * Hq <= 148;
+        if (p.one_tile) grid.x = n_mtiles;
         p.n_pairs = static_cast<int>(grid.x);
         p.n_bh = static_cast<int>(grid.y);
         // As many heads take turns as have their keys and values in L2 together; one by one, each head's long lists come

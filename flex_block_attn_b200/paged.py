@@ -192,7 +192,7 @@ def paged_decode_attn(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
     _cabi.check(rc, "fba_paged_decode_workspace_bytes")
     poison, check = _debug_flags()
     ws = q.new_empty((n.value // 4,), dtype=torch.float32) if n.value else None
-    o = q.new_empty(shape)
+    o = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
     lse = q.new_empty((B, Hq), dtype=torch.float32) if need_lse or accumulate else None
     _poisoned(poison, *(x for x in (ws, o, lse) if x is not None))
     mon = _monitor(dev)
