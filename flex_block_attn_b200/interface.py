@@ -144,16 +144,12 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def _debug_flags() -> tuple[bool, bool]:
-    """(FBA_POISON_OUTPUTS, FBA_CHECK_STATUS), read once per call."""
-    env = os.environ
-    return env.get("FBA_POISON_OUTPUTS", "0") == "1", env.get("FBA_CHECK_STATUS", "0") == "1"
-
-
-def _poisoned(poison: bool, *tensors: torch.Tensor) -> None:
-    if poison:
+def _poisoned(*tensors: Optional[torch.Tensor]) -> None:
+    """What ``_new`` does under FBA_POISON_OUTPUTS=1, for several allocations with one look at the environment."""
+    if os.environ.get("FBA_POISON_OUTPUTS", "0") == "1":
         for t in tensors:
-            t.fill_(float("nan"))
+            if t is not None:
+                t.fill_(float("nan"))
 
 
 # The current stream of a device by its index, without building a Stream object (2 us of a call's 15).
@@ -161,11 +157,11 @@ _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_get
     lambda index: torch.cuda.current_stream(index).cuda_stream
 
 
-def _checked(rc: int, what: str, check: bool, device: torch.device) -> None:
+def _checked(rc: int, what: str, device: torch.device) -> None:
     """Behind a call that reports into the mapped words: raise its error, and check the status if asked to."""
     if rc != 0:
         _cabi.check(rc, what)
-    if check and not torch.cuda.is_current_stream_capturing():
+    if os.environ.get("FBA_CHECK_STATUS", "0") == "1" and not torch.cuda.is_current_stream_capturing():
         check_status(device)
 
 

@@ -17,7 +17,7 @@ import torch
 
 from . import _cabi
 from ._cabi import FbaPaged
-from .interface import HEAD_DIM, _checked, _debug_flags, _monitor, _poisoned, _ptr, _raw_stream, _scale_of
+from .interface import HEAD_DIM, _checked, _monitor, _poisoned, _ptr, _raw_stream, _scale_of
 from .window import _window_of
 
 _Strides3, _Strides2 = ctypes.c_int64 * 3, ctypes.c_int64 * 2
@@ -151,7 +151,7 @@ def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table
     rc = _cabi.lib().fba_paged_append(ctypes.byref(arg), k.data_ptr(), v.data_ptr(), _Strides3(*_strides("k", k, 3)),
                                       _Strides3(*_strides("v", v, 3)), B, shape[2], lens, new, pos, out.data_ptr(),
                                       mon.mapped_ptr, _raw_stream(dev.index))
-    _checked(rc, "fba_paged_append", _debug_flags()[1], dev)
+    _checked(rc, "fba_paged_append", dev)
     return out
 
 
@@ -190,17 +190,20 @@ def paged_decode_attn(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
     rc = lib.fba_paged_decode_workspace_bytes(B, Hq, arg.Hkv, arg.page_size, arg.max_pages, arg.e4m3, accumulate,
                                                ctypes.byref(n))
     _cabi.check(rc, "fba_paged_decode_workspace_bytes")
-    poison, check = _debug_flags()
-    ws = q.new_empty((n.value // 4,), dtype=torch.float32) if n.value else None
     o = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
-    lse = q.new_empty((B, Hq), dtype=torch.float32) if need_lse or accumulate else None
-    _poisoned(poison, *(x for x in (ws, o, lse) if x is not None))
+    lse = q.new_empty((B, Hq), dtype=torch.float32) if need_lse else None
+    # The workspace; with accumulation the kernels want the log-sum-exp, too, also where the caller does not.
+    words, own_lse = n.value // 4, accumulate and not need_lse
+    ws = q.new_empty((words + own_lse * B * Hq,), dtype=torch.float32) if words else None
+    _poisoned(ws, o, lse)
+    ws_ptr = _ptr(ws)
+    lse_ptr = ws_ptr + n.value if own_lse else _ptr(lse)
     mon = _monitor(dev)
     mon.poll_mapped()
-    rc = lib.fba_paged_decode(ctypes.byref(arg), q.data_ptr(), _Strides2(*_strides("q", q, 2)), o.data_ptr(), _ptr(lse), B, Hq,
-                              lens, w, s, _scale_of(softmax_scale), accumulate, _ptr(ws), n.value, mon.mapped_ptr,
+    rc = lib.fba_paged_decode(ctypes.byref(arg), q.data_ptr(), _Strides2(*_strides("q", q, 2)), o.data_ptr(), lse_ptr, B, Hq,
+                              lens, w, s, _scale_of(softmax_scale), accumulate, ws_ptr, n.value, mon.mapped_ptr,
                               _raw_stream(dev.index))
-    _checked(rc, "fba_paged_decode", check, dev)
+    _checked(rc, "fba_paged_decode", dev)
     return (o, lse) if need_lse else o
 
 
@@ -243,5 +246,5 @@ def evict_kv(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Ten
     mon.poll_mapped()
     rc = lib.fba_paged_evict(ctypes.byref(arg), B, lens, budget, sinks, recent, nxt, to, to_pages, out.data_ptr(),
                              ws.data_ptr(), n.value, mon.mapped_ptr, _raw_stream(dev.index))
-    _checked(rc, "fba_paged_evict", _debug_flags()[1], dev)
+    _checked(rc, "fba_paged_evict", dev)
     return out

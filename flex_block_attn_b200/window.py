@@ -13,7 +13,7 @@ from typing import Optional
 import torch
 
 from . import _cabi
-from .interface import _check_qkv, _checked, _debug_flags, _monitor, _poisoned, _ptr, _raw_stream, _scale_of
+from .interface import _check_qkv, _checked, _monitor, _poisoned, _ptr, _raw_stream, _scale_of
 
 
 def _window_of(window: Optional[int], sinks: int) -> tuple[int, int]:
@@ -41,15 +41,14 @@ def forward_with_window(q, k, v, window: Optional[int], sinks: int = 0, softmax_
     w, s = _window_of(window, sinks)
     B, Hq, Hkv, Sq, Skv = _sizes(q, k, v)
     dev = q.device
-    poison, check = _debug_flags()
     o = torch.empty_like(q)
     lse = q.new_empty((B, Hq, Sq), dtype=torch.float32) if need_lse else None
-    _poisoned(poison, o, *(() if lse is None else (lse,)))
+    _poisoned(o, lse)
     mon = _monitor(dev)
     mon.poll_mapped()
     rc = _cabi.lib().fba_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), B, Hq, Hkv, Sq, Skv, w,
                                     s, _scale_of(softmax_scale), mon.mapped_ptr, _raw_stream(dev.index))
-    _checked(rc, "fba_window_fwd", check, dev)
+    _checked(rc, "fba_window_fwd", dev)
     return o, lse
 
 
@@ -69,7 +68,6 @@ def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: in
     if not dout.device == o.device == lse.device == dev:
         raise RuntimeError("o, lse and dout must be on the device of q")
     lib = _cabi.lib()
-    poison, check = _debug_flags()
     n = ctypes.c_uint64(0)
     _cabi.check(lib.fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, w, s, ctypes.byref(n)), "fba_window_partial_bytes")
     # One buffer: row statistics, 2 floats a padded row; the dQ accumulator, 128; the partial sums.  All parts start at
@@ -77,7 +75,7 @@ def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: in
     rows = B * Hq * -(-Sq // 128) * 128
     scratch = q.new_empty((rows * 130 + n.value // 4,), dtype=torch.float32)
     dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
-    _poisoned(poison, scratch, dq, dk, dv)
+    _poisoned(scratch, dq, dk, dv)
     at = scratch.data_ptr()
     mon = _monitor(dev)
     mon.poll_mapped()
@@ -85,7 +83,7 @@ def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: in
                             dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Hq, Hkv, Sq, Skv, w, s, _scale_of(softmax_scale),
                             at, at + rows * 8, at + rows * 520 if n.value else None, n.value, mon.mapped_ptr,
                             _raw_stream(dev.index))
-    _checked(rc, "fba_window_bwd", check, dev)
+    _checked(rc, "fba_window_bwd", dev)
     return dq, dk, dv
 
 
