@@ -275,8 +275,8 @@ template <bool kE4m3, int NT>
 __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas : 2) paged_decode_kernel(const PagedDev c, const DecodeParams p) {
     using Sh = DecShape<kE4m3>;
     extern __shared__ __align__(128) uint8_t smem[];
-    pdl_launch_dependents();
     pdl_wait();
+    pdl_launch_dependents();   // in this order: the kernel behind reads lengths and tables ahead of its own wait
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t4 = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * Sh::kStages * Sh::kStage;
@@ -704,10 +704,10 @@ __device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, i
     __shared__ float s_l[4];
     const int h = hr / p.q_tiles, q0 = h * p.group + (hr - h * p.q_tiles) * 8 * NT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (hq >= min(8 * NT, (h + 1) * p.group - q0)) return;
     const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
     const RowParts r = row_parts(c, p, b, hr, s.nt);
-    if (r.whole) return;
+    pdl_wait();
+    if (r.whole || hq >= min(8 * NT, (h + 1) * p.group - q0)) return;
     const long long slot0 = (static_cast<long long>(b) * c.Hkv * p.q_tiles + hr) * (8 * NT) + hq;   // a part x CTAs on is x * 8 NT slots on
     const float top = parts_max(p, r, slot0, 8 * NT);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -746,7 +746,7 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
     const int j0 = stretch * kWeighSlots;
-    if (j0 >= s.n) return;
+    const RowParts r = j0 < s.n ? row_parts(c, p, b, h, s.nt) : RowParts{0, -1, false};
     const long long q0 = static_cast<long long>(b) * p.Hq + h * p.group;
     constexpr int kSlots = kWeighSlots / 128;
     long long row[kSlots];
@@ -755,13 +755,18 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
     for (int u = 0; u < kSlots; ++u) {
         const int j = j0 + u * 128 + threadIdx.x;
         row[u] = j < s.n ? paged_row(c, b, h, j, p.status) : -1;
+    }
+    pdl_wait();
+    if (j0 >= s.n) return;
+#pragma unroll
+    for (int u = 0; u < kSlots; ++u) {
+        const int j = j0 + u * 128 + threadIdx.x;
 #pragma unroll
         for (int hq = 0; hq < 8 * NT; ++hq)
             x[u][hq] = j < s.n && hq < p.group ? p.scores[(q0 + hq) * p.score_stride + j] : -INFINITY;
     }
 #pragma unroll
     for (int u = 0; u < kSlots; ++u) old[u] = row[u] >= 0 ? c.weight[row[u]] : 0.f;
-    const RowParts r = row_parts(c, p, b, h, s.nt);
     for (int hq = warp; hq < p.group; hq += 4) {
         float lse;
         if (r.whole) {
@@ -792,12 +797,11 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
     }
 }
 
-// The launch behind the decode kernel: blockIdx.x = row, blockIdx.y = a query head of it to join, or, behind those, a stretch
+// The launch behind the decode kernel, in whose shadow it reads the lengths and tables (that kernel lets it begin only when
+// those are there): blockIdx.x = row, blockIdx.y = a query head of it to join, or, behind those, a stretch
 // of its slots to weigh.
 template <int NT>
 __global__ void __launch_bounds__(128) paged_finish_kernel(const PagedDev c, const DecodeParams p, int heads) {
-    pdl_launch_dependents();
-    pdl_wait();
     const int rows_per_seq = c.Hkv * p.q_tiles;
     const int b = blockIdx.x / rows_per_seq, hr = blockIdx.x - b * rows_per_seq;
     if (static_cast<int>(blockIdx.y) < heads) join<NT>(c, p, b, hr, blockIdx.y);

@@ -43,7 +43,7 @@ __device__ __forceinline__ long long paged_row(const PagedDev& c, int b, int h, 
 
 // Programmatic dependent launch: a kernel of this family may be set up while the one before it in the stream still runs.  Each
 // waits for its predecessor's end (and with it, as the predecessor did the same, for all before) ahead of its first
-// access to memory, in every thread.
+// access to memory, in every thread (paged_finish_kernel but for what its predecessor reads as well).
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 template <class... Params, class... Args>

@@ -211,3 +211,56 @@ def test_two_streams_at_once():
         want = orc.masked_attention(q, k, v, orc.visible(900, 900, 100, 2, "cuda"), do)
         for g, w, what in zip(got, (want[0], *want[2:]), ("O", "dQ", "dK", "dV")):
             close(g, w, what)
+
+
+def test_training_step_captured_with_autograd():
+    """Forward and torch.autograd.grad inside a capture, as make_graphed_callables does it."""
+    import flex_block_attn_b200 as fba
+
+    bufs = [x.clone() for x in rand_qkv(1, 4, 2, 500, 500, seed=41, device="cuda")]
+    leaves = [x.requires_grad_() for x in bufs[:3]]
+
+    def step():
+        o = fba.sliding_window_attn_func(*leaves, 100, 4)
+        return (o.detach(), *torch.autograd.grad(o, leaves, bufs[3]))
+
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("FBA_POISON_OUTPUTS", "0")
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = step()
+    fresh = rand_qkv(1, 4, 2, 500, 500, seed=42, device="cuda")
+    with torch.no_grad():
+        for b, x in zip(bufs, fresh):
+            b.copy_(x)
+    graph.replay()
+    want = orc.masked_attention(*fresh[:3], orc.visible(500, 500, 100, 4, "cuda"), fresh[3])
+    for got, w, what in zip(outs, (want[0], *want[2:]), ("O", "dQ", "dK", "dV")):
+        close(got, w, what)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Skv,window,sinks", [(1, 16, 1, 1500, 1500, 300, 5), (1, 8, 1, 1100, 1300, None, 0),
+                                                          (1, 1, 1, 4000, 4000, None, 0), (2, 6, 1, 900, 700, 200, 3)])
+def test_divided_key_tiles(B, Hq, Hkv, Sq, Skv, window, sinks):
+    """Few kv heads: the steps of many key tiles are divided over CTAs; dK and dV stay reproducible."""
+    import ctypes
+
+    import flex_block_attn_b200 as fba
+    from flex_block_attn_b200 import _cabi
+
+    n = ctypes.c_uint64()
+    assert _cabi.lib().fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, window or 0, sinks, ctypes.byref(n)) == 0 and n.value > 0
+    q, k, v, do = rand_qkv(B, Hq, Hkv, Sq, Skv, seed=Sq, device="cuda")
+    want = orc.masked_attention(q, k, v, orc.visible(Sq, Skv, window, sinks, "cuda"), do)
+    o, lse = fba.forward_with_window(q, k, v, window, sinks)
+    grads = fba.backward_with_window(q, k, v, o, lse, do, window, sinks)
+    for got, w, what in zip((o, *grads), (want[0], *want[2:]), ("O", "dQ", "dK", "dV")):
+        close(got, w, what)
+    again = fba.backward_with_window(q, k, v, o, lse, do, window, sinks)
+    assert torch.equal(grads[1], again[1]) and torch.equal(grads[2], again[2])
