@@ -60,9 +60,10 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedDev c, con
         if (threadIdx.x == 0 && blockIdx.x == 0) report_paged(p.status, kBadLength, b, n);
         n = max(0, min(min(n, p.T), room));
     }
+    if (start != p.seq_lens[b]) n = 0;   // a length that is none: nothing is written anywhere
     if (p.out_lens && blockIdx.x == 0 && threadIdx.x == 0) p.out_lens[b] = start + n;
     const int pos0 = p.positions ? p.positions[b] : start;
-    const int rows = n * c.Hkv;   // host-checked: T * Hkv < 2^31
+    const int rows = n * c.Hkv;
     for (int r = (blockIdx.x * 256 + threadIdx.x) >> 3; r < rows; r += gridDim.x * 32) {
         const int tok = r / c.Hkv, h = r - tok * c.Hkv;
         const long long dst = paged_row(c, b, h, start + tok, p.status);
@@ -315,6 +316,11 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas 
         if (++r.hr == rows_per_seq) {
             r.hr = 0;
             do {   // sequences without a tile have no part in the list; one with tiles follows, as tiles are left
+                if (r.b + 1 >= p.B) {   // unless someone changes the lengths meanwhile
+                    r.i = r.end = 0;
+                    r.left = 0;
+                    return;
+                }
                 ++r.b;
                 r.s = seq_tiles(paged_length(c, p.seq_lens, r.b, p.status), p.window, p.sinks);
             } while (r.s.nt == 0);
@@ -680,7 +686,8 @@ __device__ __forceinline__ RowParts row_parts(const PagedDev& c, const DecodePar
     all = __reduce_add_sync(0xffffffffu, all);
     const long long per = list_piece(static_cast<long long>(all) * rows_per_seq, p.n_ctas);
     const long long at = static_cast<long long>(ahead) * rows_per_seq + static_cast<long long>(hr) * nt;
-    const int first = static_cast<int>(at / per), last = static_cast<int>((at + nt - 1) / per);
+    const int most = p.n_ctas - 1;   // beyond only if someone changes the lengths meanwhile
+    const int first = min(most, static_cast<int>(at / per)), last = min(most, static_cast<int>((at + nt - 1) / per));
     return {first, last, first == last};
 }
 // Largest maximum of the parts of a query head; every lane of the warp takes part.
@@ -852,8 +859,8 @@ extern "C" int fba_paged_append(const fba_paged_t* cache, const void* k, const v
     if (out_lens && out_lens == seq_lens)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: out_lens must not be seq_lens");
     if (T <= 0) return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: non-positive size");
-    if (static_cast<long long>(T) * c.Hkv > 0x7fffff00LL)
-        return set_error(FBA_ERR_TOO_LARGE, "fba_paged_append: more than 2^31 rows of a sequence");
+    if (static_cast<long long>(T) * c.Hkv > 1 << 30)   // rows, and rows plus a grid's, are counted in 31 bits
+        return set_error(FBA_ERR_TOO_LARGE, "fba_paged_append: more than 2^30 rows of a sequence");
     if (reinterpret_cast<uintptr_t>(k) % 16 != 0 || reinterpret_cast<uintptr_t>(v) % 16 != 0)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: k and v must be 16-byte aligned");
     AppendParams p = {static_cast<const __nv_bfloat16*>(k), static_cast<const __nv_bfloat16*>(v), {}, {}, seq_lens, new_lens,

@@ -347,7 +347,8 @@ typedef struct fba_paged {
  * elements and multiples of 8, bases 16-byte aligned.  e4m3: per row scale = max(max|x| * fp32(1/448), 2^-126) (1 for an
  * all-zero row, NaN for a row with a NaN or an infinity), byte = e4m3(x * (1 / scale)), round to nearest even.  With weight / position: 0 and positions[b] + t
  * (NULL: the slot).  out_lens (NULL, or int32 [B], not seq_lens itself) receives seq_lens[b] + new_lens[b].  Tokens that do not fit
- * into the table's row are left out, with the report above, and not counted.
+ * into the table's row are left out, with the report above, and not counted; so are all tokens of a sequence whose length
+ * is out of range.
  */
 int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, const int64_t* k_strides,
                      const int64_t* v_strides, int B, int T, const int32_t* seq_lens, const int32_t* new_lens,

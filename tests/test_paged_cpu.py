@@ -95,7 +95,7 @@ def test_c_append_refuses_bad_arguments(lib):
     assert call(out=some) == -1 and b"out_lens" in lib.fba_last_error()
     assert call(ks=(ctypes.c_int64 * 3)(8, 4, 8)) == -1 and call(vs=(ctypes.c_int64 * 3)(8, 8, 1)) == -1
     assert call(k=ctypes.c_void_p(264)) == -1
-    assert call(B=70000) == -5 and call(T=2**31 - 1) == -5
+    assert call(B=70000) == -5 and call(T=2**31 - 1) == -5 and call(T=2**29 + 1) == -5
     assert call(c=struct(max_pages=2**26)) == -5
 
 

@@ -297,6 +297,13 @@ def test_append_beyond_the_table_is_left_out_and_reported():
         for j in range(start, stop):
             pools["k"][table[b, j // 16], :, j % 16] = 1
     same(cache.k, pools["k"], "k")
+    with pytest.MonkeyPatch.context() as m:   # lengths that are none: nothing is written
+        m.setenv("FBA_CHECK_STATUS", "0")
+        got = fba.append_kv(cache, 2 * x, x, table.cuda(), torch.tensor([-1, 33], dtype=torch.int32).cuda())
+        assert got.tolist() == [0, 32]
+        with pytest.raises(RuntimeError, match="length"):
+            fba.check_status()
+    same(cache.k, pools["k"], "k")
 
 
 def test_prompt_then_tokens_equals_attention_over_the_whole():
