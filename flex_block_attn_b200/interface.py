@@ -33,6 +33,10 @@ from ._cabi import FbaList
 HEAD_DIM = 128
 TILE = 128
 
+# Whether the current stream is being captured; the C function itself, as every call asks.
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
+
+
 class _StatusMonitor:
     """Per-device status words (written by a kernel whose bounded wait gave up) and a pinned host
     mirror that is refreshed asynchronously after every call, so that a timeout is noticed at the
@@ -53,12 +57,12 @@ class _StatusMonitor:
     def poll_mapped(self) -> None:
         """Raise if a kernel has reported into the words in host memory."""
         if self._mapped_np[0]:
-            if not torch.cuda.is_current_stream_capturing():
+            if not _capturing():
                 torch.cuda.synchronize(self.device)   # all of the words are there
             self.raise_from(self.mapped.tolist())
 
     def after_call(self) -> None:
-        if torch.cuda.is_current_stream_capturing():   # a replay writes the words; check_status() or a later call sees them
+        if _capturing():   # a replay writes the words; check_status() or a later call sees them
             return
         self.host.copy_(self.buf, non_blocking=True)
         self.event.record(torch.cuda.current_stream(self.device))
@@ -66,7 +70,7 @@ class _StatusMonitor:
 
     def poll(self) -> None:
         """Raise if a mirror copy that has already completed shows a timed-out wait."""
-        if self.pending and not torch.cuda.is_current_stream_capturing() and self.event.query():
+        if self.pending and not _capturing() and self.event.query():
             self.pending = False
             if int(self.host[0]) != 0:
                 self.raise_from(self.host.tolist())
@@ -92,7 +96,7 @@ def _monitor(device: torch.device) -> _StatusMonitor:
     key = device.index if device.index is not None else torch.cuda.current_device()
     mon = _monitors.get(key)
     if mon is None:
-        if torch.cuda.is_current_stream_capturing():   # the words must not live in a graph's memory
+        if _capturing():   # the words must not live in a graph's memory
             raise RuntimeError("flex_block_attn_b200: make one call on this device before a stream capture")
         mon = _StatusMonitor(torch.device("cuda", key))
         _monitors[key] = mon
@@ -161,7 +165,7 @@ def _checked(rc: int, what: str, device: torch.device) -> None:
     """Behind a call that reports into the mapped words: raise its error, and check the status if asked to."""
     if rc != 0:
         _cabi.check(rc, what)
-    if os.environ.get("FBA_CHECK_STATUS", "0") == "1" and not torch.cuda.is_current_stream_capturing():
+    if os.environ.get("FBA_CHECK_STATUS", "0") == "1" and not _capturing():
         check_status(device)
 
 
