@@ -100,25 +100,29 @@ def _cache_arg(cache: PagedKVCache, block_table: torch.Tensor) -> tuple[FbaPaged
         raise ValueError("an e4m3 cache needs k_scale and v_scale")
     if (cache.weight is None) != (cache.position is None):
         raise ValueError("cache.weight and cache.position come together")
-    for what in ("k_scale", "v_scale", "weight", "position"):
-        x = getattr(cache, what)
-        if x is not None:
-            dtype = torch.int32 if what == "position" else torch.float32
-            if x.dtype != dtype or x.shape != shape[:3] or not x.is_contiguous():
-                raise ValueError(f"cache.{what} must be a contiguous {dtype} tensor, [pages, kv heads, page size]")
-            if x.device != dev:
-                raise RuntimeError("the cache's tensors must be on one device")
+    if e4m3 or cache.weight is not None:
+        rows = shape[:3]
+        for what in ("k_scale", "v_scale", "weight", "position"):
+            x = getattr(cache, what)
+            if x is not None:
+                dtype = torch.int32 if what == "position" else torch.float32
+                if x.dtype != dtype or x.shape != rows or not x.is_contiguous():
+                    raise ValueError(f"cache.{what} must be a contiguous {dtype} tensor, [pages, kv heads, page size]")
+                if x.device != dev:
+                    raise RuntimeError("the cache's tensors must be on one device")
     table, B, pages = _table("block_table", block_table, dev)
     return FbaPaged(k.data_ptr(), v.data_ptr(), _ptr(cache.k_scale), _ptr(cache.v_scale), _ptr(cache.weight),
                     _ptr(cache.position), table, shape[0], shape[1], shape[2], pages, e4m3), B, dev
 
 
-def _strides(name: str, x: torch.Tensor, n: int) -> list[int]:
-    """The strides of the first ``n`` dimensions; one that is never taken counts as 0."""
-    st = x.stride()
-    if st[n] != 1:
+def _strides(name: str, x: torch.Tensor, shape: torch.Size):
+    """The strides of all dimensions but the last, as the C entry points take them; one that is never taken counts as 0."""
+    *st, last = x.stride()
+    if last != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
-    return [s if d > 1 else 0 for s, d in zip(st[:n], x.shape)]
+    if 1 in shape:
+        st = [0 if d == 1 else s for s, d in zip(st, shape)]
+    return (_Strides3 if len(st) == 3 else _Strides2)(*st)
 
 
 def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
@@ -136,7 +140,8 @@ def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table
     """
     arg, B, dev = _cache_arg(cache, block_table)
     shape = k.shape
-    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or len(shape) != 4 or shape[:2] != (B, arg.Hkv) or shape[3] != HEAD_DIM:
+    if k.dtype != torch.bfloat16 or v.dtype != torch.bfloat16 or len(shape) != 4 or shape[0] != B or shape[1] != arg.Hkv or \
+            shape[3] != HEAD_DIM:
         raise ValueError("k and v must be torch.bfloat16, [batch, kv heads, tokens, 128]")
     if v.shape != shape:
         raise ValueError("k and v must have the same shape")
@@ -148,8 +153,8 @@ def append_kv(cache: PagedKVCache, k: torch.Tensor, v: torch.Tensor, block_table
     out = torch.empty_like(seq_lens)
     mon = _monitor(dev)
     mon.poll_mapped()
-    rc = _cabi.lib().fba_paged_append(ctypes.byref(arg), k.data_ptr(), v.data_ptr(), _Strides3(*_strides("k", k, 3)),
-                                      _Strides3(*_strides("v", v, 3)), B, shape[2], lens, new, pos, out.data_ptr(),
+    rc = _cabi.lib().fba_paged_append(ctypes.byref(arg), k.data_ptr(), v.data_ptr(), _strides("k", k, shape),
+                                      _strides("v", v, shape), B, shape[2], lens, new, pos, out.data_ptr(),
                                       mon.mapped_ptr, _raw_stream(dev.index))
     _checked(rc, "fba_paged_append", dev)
     return out
@@ -200,7 +205,7 @@ def paged_decode_attn(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
     lse_ptr = ws_ptr + n.value if own_lse else _ptr(lse)
     mon = _monitor(dev)
     mon.poll_mapped()
-    rc = lib.fba_paged_decode(ctypes.byref(arg), q.data_ptr(), _Strides2(*_strides("q", q, 2)), o.data_ptr(), lse_ptr, B, Hq,
+    rc = lib.fba_paged_decode(ctypes.byref(arg), q.data_ptr(), _strides("q", q, shape), o.data_ptr(), lse_ptr, B, Hq,
                               lens, w, s, _scale_of(softmax_scale), accumulate, ws_ptr, n.value, mon.mapped_ptr,
                               _raw_stream(dev.index))
     _checked(rc, "fba_paged_decode", dev)
