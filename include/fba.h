@@ -300,10 +300,11 @@ int fba_bwd_split(const void* q, const void* k, const void* v, const void* o, co
  * only tiles that hold visible pairs.  K and V must be finite: a NaN or infinity in a value row may also reach rows of
  * the same 128-row tiles that do not see it (0 * inf in the product).
  *
- * Backward: scratch buffers as fba_bwd's (fba_bwd_scratch_bytes), and `partial`, 16-byte aligned, of
- * fba_window_partial_bytes() bytes, at most 74 MB (0: NULL is accepted) for the fp32 dK / dV of the key tiles with sinks,
- * which every query sees and whose steps are therefore divided over several CTAs.  dK and dV are reproducible bit by bit;
- * dQ is summed in scheduling order, like fba_bwd's.
+ * Backward: scratch buffers as fba_bwd's (fba_bwd_scratch_bytes; dq_accum is zeroed by the call and 16-byte aligned), and
+ * `partial`, 16-byte aligned, of fba_window_partial_bytes() bytes, at most 74 MB (0: NULL is accepted), for the fp32 dK / dV
+ * of key tiles with long lists (sinks, which every query sees; all tiles where there are few kv heads), whose steps are
+ * divided over several CTAs.  dK and dV have the same bits in every call with the same sizes; a call on part of the batch
+ * or of the kv heads may divide other tiles and differ in the last bit.  dQ is summed in scheduling order, like fba_bwd's.
  */
 int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv, int Sq,
                    int Skv, int window, int sinks, float softmax_scale, uint32_t* status, void* stream);
@@ -325,9 +326,9 @@ int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, c
  *   page_size    16, 32, 64, 128 or 256; max_pages * page_size < 2^30
  * Lengths (`seq_lens`, int32 [B]) are read on the device.  A page number outside 0 .. n_pages - 1, or a length outside
  * 0 .. max_pages * page_size, is never followed: the kernel leaves out the rows concerned (holds the length to the limit)
- * and reports it in the status words (device memory, or pinned host memory that a
- * caller can look at without a copy); fba_check_status(), which reads device memory, then returns FBA_ERR_BAD_CACHE.  Pages that a call writes must
- * belong to one sequence only; pages that are read may be shared.
+ * and reports it in the status words (device memory, or pinned host memory that a caller can look at without a copy);
+ * fba_check_status(), which reads device memory, then returns FBA_ERR_BAD_CACHE.  Pages that a call writes must belong to
+ * one sequence only; pages that are read may be shared.
  */
 typedef struct fba_paged {
     void* k;
