@@ -272,6 +272,9 @@ __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) <
 // Exponent of a positive finite number, rounded down (-127 for subnormals and 0).
 __device__ __forceinline__ int exponent(float x) { return (__float_as_int(x) >> 23) - 127; }
 
+// Weight of a part with maximum m; where no part has a finite score, the sums (0, or NaN) stand as they are.
+__device__ __forceinline__ float part_scale(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
+
 template <bool kE4m3, int NT>
 __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas : 2) paged_decode_kernel(const PagedDev c, const DecodeParams p) {
     using Sh = DecShape<kE4m3>;
@@ -611,8 +614,9 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas 
             stage = stage + 1 == Sh::kStages ? 0 : stage + 1;
         }
 
-        // The four warps' parts of the row, eight heads at a time; thread = dim.
+        // The four warps' parts of the row, eight heads at a time: a warp joins two heads, a lane four dims.
         const int row_id = cur.b * rows_per_seq + cur.hr;
+        const float back = kE4m3 ? v_ref * 0.0078125f : 1.f;
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             if (8 * nt >= heads) break;
@@ -621,42 +625,54 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas 
                 float sum = l[nt][x];
 #pragma unroll
                 for (int sh = 4; sh < 32; sh <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, sh);
-                if (g == 0) {
-                    ex_ml[(warp * 8 + 2 * t4 + x) * 2] = m[nt][x];
-                    ex_ml[(warp * 8 + 2 * t4 + x) * 2 + 1] = sum;
-                }
+                if (g == 0)
+                    *reinterpret_cast<float2*>(ex_ml + (warp * 8 + 2 * t4 + x) * 2) = make_float2(m[nt][x], sum);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     float* dst = ex_o + (warp * 8 + 2 * t4 + x) * kOStride + 16 * j;
-                    const float back = kE4m3 ? v_ref * 0.0078125f : 1.f;
-                    dst[kE4m3 ? 2 * g : g] = acc[nt][j][x] * back;
-                    dst[kE4m3 ? 2 * g + 1 : g + 8] = acc[nt][j][x + 2] * back;
+                    const float a = acc[nt][j][x] * back, b = acc[nt][j][x + 2] * back;
+                    if (kE4m3) {
+                        *reinterpret_cast<float2*>(dst + 2 * g) = make_float2(a, b);
+                    } else {
+                        dst[g] = a;
+                        dst[g + 8] = b;
+                    }
                 }
             }
             __syncthreads();
-            const int d = threadIdx.x;
-            for (int hq = 0; hq < min(8, heads - 8 * nt); ++hq) {
-                float mw[4], top = -INFINITY;
 #pragma unroll
-                for (int w = 0; w < 4; ++w) top = fmaxf(top, mw[w] = ex_ml[(w * 8 + hq) * 2]);
-                float sum = 0.f, o = 0.f;
+            for (int x = 0; x < 2; ++x) {
+                const int hq = 2 * warp + x;
+                if (8 * nt + hq >= heads) break;
+                float2 ml[4];
+                float top = -INFINITY, sum = 0.f;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    const float a = top == -INFINITY ? 0.f : ex2_approx(mw[w] - top);
-                    sum = fmaf(a, ex_ml[(w * 8 + hq) * 2 + 1], sum);
-                    o = fmaf(a, ex_o[(w * 8 + hq) * kOStride + d], o);
+                    ml[w] = *reinterpret_cast<const float2*>(ex_ml + (w * 8 + hq) * 2);
+                    top = fmaxf(top, ml[w].x);
+                }
+                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const float a = part_scale(ml[w].x, top);
+                    const float4 v = *reinterpret_cast<const float4*>(ex_o + (w * 8 + hq) * kOStride + 4 * lane);
+                    sum = fmaf(a, ml[w].y, sum);
+                    o.x = fmaf(a, v.x, o.x);
+                    o.y = fmaf(a, v.y, o.y);
+                    o.z = fmaf(a, v.z, o.z);
+                    o.w = fmaf(a, v.w, o.w);
                 }
                 if (whole) {
+                    const bool some = sum > 0.f || isnan(sum);
+                    const float inv = some ? 1.f / sum : 0.f;
                     const long long out = static_cast<long long>(cur.b) * p.Hq + q0 + 8 * nt + hq;
-                    p.o[out * 128 + d] = __float2bfloat16(sum > 0.f || isnan(sum) ? o / sum : 0.f);
-                    if (p.lse && d == 0) p.lse[out] = sum > 0.f || isnan(sum) ? (top + log2f(sum)) * kLn2 : -INFINITY;
+                    reinterpret_cast<uint2*>(p.o)[out * 32 + lane] = some ? make_uint2(pack_bf16x2(o.x * inv, o.y * inv), pack_bf16x2(o.z * inv, o.w * inv))
+                                                                          : make_uint2(0u, 0u);
+                    if (p.lse && lane == 0) p.lse[out] = some ? (top + log2f(sum)) * kLn2 : -INFINITY;
                 } else {
                     const long long slot = (static_cast<long long>(blockIdx.x) + row_id) * (8 * NT) + 8 * nt + hq;
-                    p.part_o[slot * 128 + d] = o;
-                    if (d == 0) {
-                        p.part_ml[slot * 2] = top;
-                        p.part_ml[slot * 2 + 1] = sum;
-                    }
+                    reinterpret_cast<float4*>(p.part_o)[slot * 32 + lane] = o;
+                    if (lane == 0) reinterpret_cast<float2*>(p.part_ml)[slot] = make_float2(top, sum);
                 }
             }
             __syncthreads();
@@ -698,17 +714,14 @@ __device__ __forceinline__ float parts_max(const DecodeParams& p, const RowParts
     for (int s = 16; s > 0; s >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, s));
     return top;
 }
-// Weight of a part with maximum m; where no part has a finite score, the sums (0, or NaN) stand as they are.
-__device__ __forceinline__ float part_scale(float m, float top) { return top == -INFINITY ? 1.f : ex2_approx(m - top); }
-
 // Joins the parts of the rows that several CTAs share, and gives the rows without a tile their zeros.  One block per row
-// and query head; the four warps take the parts in turn, a lane four dims.  Latency-bound: a few KB per block, so the
+// and query head; the warps take the parts in turn, a lane four dims.  Latency-bound: a few KB per block, so the
 // loads of a warp's parts are independent of one another.  (One block per row with its heads in turn and the sums carried
 // from part to part took 11 us for 64 sequences, 24 us for 16 of 8 heads a kv head, 36 us for two long ones.)
-template <int NT>
+template <int NT, int kWarps>
 __device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, int b, int hr, int hq) {
-    __shared__ float4 s_o[4][32];
-    __shared__ float s_l[4];
+    __shared__ float4 s_o[kWarps][32];
+    __shared__ float s_l[kWarps];
     const int h = hr / p.q_tiles, q0 = h * p.group + (hr - h * p.q_tiles) * 8 * NT;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
@@ -720,7 +733,7 @@ __device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, i
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
 #pragma unroll 8
-    for (int x = r.first + warp; x <= r.last; x += 4) {
+    for (int x = r.first + warp; x <= r.last; x += kWarps) {
         const long long slot = slot0 + static_cast<long long>(x) * (8 * NT);
         const float2 ml = reinterpret_cast<const float2*>(p.part_ml)[slot];
         const float4 v = reinterpret_cast<const float4*>(p.part_o)[slot * 32 + lane];
@@ -735,9 +748,14 @@ __device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, i
     if (lane == 0) s_l[warp] = l;
     __syncthreads();
     const int d = threadIdx.x;
+    if (d >= 128) return;
     const float* so = reinterpret_cast<const float*>(s_o);
-    const float sum = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-    const float x = (so[d] + so[128 + d]) + (so[256 + d] + so[384 + d]);
+    float sum = 0.f, x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        sum += s_l[w];
+        x += so[128 * w + d];
+    }
     const bool some = sum > 0.f || isnan(sum);
     const long long out = static_cast<long long>(b) * p.Hq + q0 + hq;
     p.o[out * 128 + d] = __float2bfloat16(some ? x / sum : 0.f);
@@ -747,7 +765,7 @@ __device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, i
 // Adds the probabilities to the weights, from the scores and the parts' sums: a block of the join's launch for each stretch of
 // kWeighSlots slots.  What does not depend on the sums is under way before they are looked at.
 constexpr int kWeighSlots = 256;
-template <int NT>
+template <int NT, int kWarps>
 __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, int b, int h, int stretch) {
     __shared__ float s_lse[8 * NT];   // in units of log2
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -755,26 +773,26 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
     const int j0 = stretch * kWeighSlots;
     const RowParts r = j0 < s.n ? row_parts(c, p, b, h, s.nt) : RowParts{0, -1, false};
     const long long q0 = static_cast<long long>(b) * p.Hq + h * p.group;
-    constexpr int kSlots = kWeighSlots / 128;
+    constexpr int kSlots = kWarps == 4 ? 2 : 1;   // a thread; with more than 8 warps some have none
     long long row[kSlots];
     float x[kSlots][8 * NT], old[kSlots];
 #pragma unroll
     for (int u = 0; u < kSlots; ++u) {
-        const int j = j0 + u * 128 + threadIdx.x;
-        row[u] = j < s.n ? paged_row(c, b, h, j, p.status) : -1;
+        const int j = j0 + u * 128 + threadIdx.x, end = min(s.n, j0 + kWeighSlots);
+        row[u] = j < end ? paged_row(c, b, h, j, p.status) : -1;
     }
     pdl_wait();
     if (j0 >= s.n) return;
 #pragma unroll
     for (int u = 0; u < kSlots; ++u) {
-        const int j = j0 + u * 128 + threadIdx.x;
+        const int j = j0 + u * 128 + threadIdx.x, end = min(s.n, j0 + kWeighSlots);
 #pragma unroll
         for (int hq = 0; hq < 8 * NT; ++hq)
-            x[u][hq] = j < s.n && hq < p.group ? p.scores[(q0 + hq) * p.score_stride + j] : -INFINITY;
+            x[u][hq] = j < end && hq < p.group ? p.scores[(q0 + hq) * p.score_stride + j] : -INFINITY;
     }
 #pragma unroll
     for (int u = 0; u < kSlots; ++u) old[u] = row[u] >= 0 ? c.weight[row[u]] : 0.f;
-    for (int hq = warp; hq < p.group; hq += 4) {
+    for (int hq = warp; hq < p.group; hq += kWarps) {
         float lse;
         if (r.whole) {
             lse = p.lse[q0 + hq] * kLog2e;
@@ -807,12 +825,12 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
 // The launch behind the decode kernel, in whose shadow it reads the lengths and tables (that kernel lets it begin only when
 // those are there): blockIdx.x = row, blockIdx.y = a query head of it to join, or, behind those, a stretch
 // of its slots to weigh.
-template <int NT>
-__global__ void __launch_bounds__(128) paged_finish_kernel(const PagedDev c, const DecodeParams p, int heads) {
+template <int NT, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32) paged_finish_kernel(const PagedDev c, const DecodeParams p, int heads) {
     const int rows_per_seq = c.Hkv * p.q_tiles;
     const int b = blockIdx.x / rows_per_seq, hr = blockIdx.x - b * rows_per_seq;
-    if (static_cast<int>(blockIdx.y) < heads) join<NT>(c, p, b, hr, blockIdx.y);
-    else weigh<NT>(c, p, b, hr, blockIdx.y - heads);   // host-checked: one group of query heads, so a row is a kv head
+    if (static_cast<int>(blockIdx.y) < heads) join<NT, kWarps>(c, p, b, hr, blockIdx.y);
+    else weigh<NT, kWarps>(c, p, b, hr, blockIdx.y - heads);   // host-checked: one group of query heads, so a row is a kv head
 }
 
 int paged_args(const char* who, const fba_paged_t* cache, int B, PagedDev* dev) {
@@ -919,7 +937,9 @@ int launch_decode(const PagedDev& c, const DecodeParams& p, const DecodePlan& d,
     const int heads = d.n_ctas == 0 ? 0 : p.group < 8 * NT ? p.group : 8 * NT;
     const int stretches = p.scores ? (d.score_stride + kWeighSlots - 1) / kWeighSlots : 0;
     if (rc == FBA_OK && heads + stretches > 0)
-        rc = launch_chained(paged_finish_kernel<NT>, dim3(rows, heads + stretches), 128, 0, stream, c, p, heads);
+        // A row may have many parts where there are few rows: more warps take them then.
+        rc = d.n_ctas > 16 * d.rows ? launch_chained(paged_finish_kernel<NT, 16>, dim3(rows, heads + stretches), 512, 0, stream, c, p, heads)
+                                    : launch_chained(paged_finish_kernel<NT, 4>, dim3(rows, heads + stretches), 128, 0, stream, c, p, heads);
     return rc;
 }
 }  // namespace
