@@ -148,7 +148,8 @@ struct DecodeParams {
     int score_stride;
     int B, Hq, group, q_tiles;      // query heads a kv head; groups of 8 NT of them
     int window, sinks;              // window 0: none
-    int n_ctas;                     // 0: one CTA per row, nothing to join
+    int splits;                     // CTAs per row, each with an equal part of the row's own tiles; 0: the list of all tiles
+    int n_ctas;                     //   is cut into this many pieces
     float scale_log2;
 };
 
@@ -297,12 +298,15 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas 
         SeqTiles s;
     };
     Cursor first;
-    if (p.n_ctas == 0) {
-        first.b = blockIdx.x / rows_per_seq;
-        first.hr = blockIdx.x - first.b * rows_per_seq;
+    if (p.splits > 0) {
+        const int row = blockIdx.x / p.splits, part = blockIdx.x - row * p.splits;
+        first.b = row / rows_per_seq;
+        first.hr = row - first.b * rows_per_seq;
         first.s = seq_tiles(paged_length(c, p.seq_lens, first.b, p.status), p.window, p.sinks);
-        first.i = 0;
-        first.end = first.s.nt;
+        const int per = static_cast<int>(list_piece(first.s.nt, p.splits));
+        first.i = part * per;
+        if (part > 0 && first.i >= first.s.nt) return;   // (part 0 of a row without a tile writes its zeros)
+        first.end = min(first.s.nt, first.i + per);
         first.left = 0;
     } else {
         const ListPlace place = list_place(c, p, blockIdx.x, rows_per_seq);
@@ -670,7 +674,7 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas 
                                                                           : make_uint2(0u, 0u);
                     if (p.lse && lane == 0) p.lse[out] = some ? (top + log2f(sum)) * kLn2 : -INFINITY;
                 } else {
-                    const long long slot = (static_cast<long long>(blockIdx.x) + row_id) * (8 * NT) + 8 * nt + hq;
+                    const long long slot = (static_cast<long long>(blockIdx.x) + (p.splits > 0 ? 0 : row_id)) * (8 * NT) + 8 * nt + hq;
                     reinterpret_cast<float4*>(p.part_o)[slot * 32 + lane] = o;
                     if (lane == 0) reinterpret_cast<float2*>(p.part_ml)[slot] = make_float2(top, sum);
                 }
@@ -683,15 +687,20 @@ __global__ void __launch_bounds__(kDecThreads, NT == 1 ? DecShape<kE4m3>::kCtas 
     cp_async_wait<0>();
 }
 
-// A row's tiles are in the pieces of CTAs first .. last; `whole`: of one, which wrote the result itself.  No tile: none.
+// A row's parts: slots base + first .. base + last; `whole`: there is one, whose CTA wrote the result itself.  No tile: none.
 struct RowParts {
     int first, last;
     bool whole;
+    long long base;
 };
 __device__ __forceinline__ RowParts row_parts(const PagedDev& c, const DecodeParams& p, int b, int hr, int nt) {
-    if (p.n_ctas == 0) return {0, 0, true};
-    if (nt == 0) return {0, -1, false};
     const int rows_per_seq = c.Hkv * p.q_tiles;
+    const long long row = static_cast<long long>(b) * rows_per_seq + hr;
+    if (p.splits > 0) {
+        const int per = static_cast<int>(list_piece(nt, p.splits)), last = nt == 0 ? 0 : (nt - 1) / per;
+        return {0, last, last == 0, row * p.splits};
+    }
+    if (nt == 0) return {0, -1, false, row};
     int ahead = 0, all = 0;   // tiles of the sequences before b, and of all
     for (int x = threadIdx.x & 31; x < p.B; x += 32) {
         const int n = seq_tiles(paged_length(c, p.seq_lens, x, p.status), p.window, p.sinks).nt;
@@ -704,7 +713,7 @@ __device__ __forceinline__ RowParts row_parts(const PagedDev& c, const DecodePar
     const long long at = static_cast<long long>(ahead) * rows_per_seq + static_cast<long long>(hr) * nt;
     const int most = p.n_ctas - 1;   // beyond only if someone changes the lengths meanwhile
     const int first = min(most, static_cast<int>(at / per)), last = min(most, static_cast<int>((at + nt - 1) / per));
-    return {first, last, first == last};
+    return {first, last, first == last, row};
 }
 // Largest maximum of the parts of a query head; every lane of the warp takes part.
 __device__ __forceinline__ float parts_max(const DecodeParams& p, const RowParts& r, long long slot0, int step) {
@@ -728,7 +737,7 @@ __device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, i
     const RowParts r = row_parts(c, p, b, hr, s.nt);
     pdl_wait();
     if (r.whole || hq >= min(8 * NT, (h + 1) * p.group - q0)) return;
-    const long long slot0 = (static_cast<long long>(b) * c.Hkv * p.q_tiles + hr) * (8 * NT) + hq;   // a part x CTAs on is x * 8 NT slots on
+    const long long slot0 = r.base * (8 * NT) + hq;
     const float top = parts_max(p, r, slot0, 8 * NT);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float l = 0.f;
@@ -771,7 +780,7 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const SeqTiles s = seq_tiles(paged_length(c, p.seq_lens, b, p.status), p.window, p.sinks);
     const int j0 = stretch * kWeighSlots;
-    const RowParts r = j0 < s.n ? row_parts(c, p, b, h, s.nt) : RowParts{0, -1, false};
+    const RowParts r = j0 < s.n ? row_parts(c, p, b, h, s.nt) : RowParts{0, -1, false, 0};
     const long long q0 = static_cast<long long>(b) * p.Hq + h * p.group;
     constexpr int kSlots = kWarps == 4 ? 2 : 1;   // a thread; with more than 8 warps some have none
     long long row[kSlots];
@@ -797,7 +806,7 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
         if (r.whole) {
             lse = p.lse[q0 + hq] * kLog2e;
         } else {
-            const long long slot0 = (static_cast<long long>(b) * c.Hkv + h) * (8 * NT) + hq;
+            const long long slot0 = r.base * (8 * NT) + hq;
             const float top = parts_max(p, r, slot0, 8 * NT);
             float l = 0.f;
             for (int part = r.first + lane; part <= r.last; part += 32) {
@@ -900,7 +909,7 @@ extern "C" int fba_paged_append(const fba_paged_t* cache, const void* k, const v
 namespace {
 // How a decode call is cut up.
 struct DecodePlan {
-    int nt, q_tiles, n_ctas, score_stride;
+    int nt, q_tiles, splits, n_ctas, score_stride;   // n_ctas: of the grid
     long long rows;
     uint64_t part_o, part_ml, scores;   // bytes of the workspace, each rounded up to 256
 };
@@ -911,14 +920,26 @@ DecodePlan decode_plan(int B, int Hq, int Hkv, int page_size, int max_pages, boo
     d.q_tiles = (group + 8 * d.nt - 1) / (8 * d.nt);
     d.rows = static_cast<long long>(B) * Hkv * d.q_tiles;
     const long long tiles = static_cast<long long>(max_pages) * page_size / kTileKeys;   // a row has at most
-    // One CTA per row where a row is short: nothing is joined then.  Otherwise as many as are resident.  (Two, three and four
-    // times as many, us: 64 sequences 183 -> 179, 178, 177; two long e4m3 ones 101 -> 105, 109, 115; 16 with a window 51 ->
-    // 55, 58, 60: a CTA's start and end cost about 4 us, uneven SMs less.)
-    const long long pieces = (d.rows * tiles + kDecMinTiles - 1) / kDecMinTiles;
-    const long long want = 148 * (d.nt == 1 && e4m3 ? 3 : 2);
-    d.n_ctas = tiles <= 2 * kDecMinTiles ? 0 : static_cast<int>(pieces < want ? pieces : want);
+    // Many rows: a CTA per row, or per equal part of a row where that makes four waves of them and leaves parts of 2048 keys.
+    // The order in which CTAs end evens out lengths and SMs, and a row in one part needs no join.  Few rows: the list of all
+    // tiles in as many pieces as are resident at a time.  Us, list -> rows: 256 sequences of 600 tokens and 8 kv heads 126 ->
+    // 100, of 1 - 1000 126 -> 84, 64 of 2048 95 -> 83 (1 part), of 512 - 8192 182 -> 170 (3 parts); e4m3, 64 of 1 - 2048 63 ->
+    // 41, of 2048 58 -> 68.  Rows that barely fill the chip: 40 sequences of 1500 50 -> 54.
+    // (The list in two, three and four waves: 64 sequences of 512 - 8192 183 -> 179, 178, 177; two long e4m3 ones 101 ->
+    // 105, 109, 115: a CTA's start and end cost a few us.)
+    const long long resident = 148 * (d.nt == 1 && e4m3 ? 3 : 2), four_waves = 4 * 2 * 148;
+    const long long most = (tiles + kDecMinTiles - 1) / kDecMinTiles;   // pieces of a row
+    d.splits = 0;
+    if (tiles <= 2 * kDecMinTiles || d.rows >= four_waves) {
+        d.splits = 1;
+    } else if (2 * d.rows >= 3 * 2 * 148) {
+        const long long want = (four_waves + d.rows - 1) / d.rows, room = tiles / (8 * kDecMinTiles);
+        d.splits = static_cast<int>(room < 1 ? 1 : want < room ? want : room);
+    }
+    const long long pieces = d.splits ? d.rows * d.splits : d.rows * most;
+    d.n_ctas = static_cast<int>(d.splits || pieces < resident ? pieces : resident);
     auto up = [](uint64_t n) { return (n + 255) / 256 * 256; };
-    const uint64_t slots = d.n_ctas ? (d.n_ctas + d.rows) * 8 * d.nt : 0;
+    const uint64_t slots = d.splits == 1 ? 0 : (d.n_ctas + (d.splits ? 0 : d.rows)) * 8ull * d.nt;
     d.part_o = up(slots * 128 * sizeof(float));
     d.part_ml = up(slots * 2 * sizeof(float));
     d.score_stride = static_cast<int>(tiles * kTileKeys);
@@ -933,12 +954,12 @@ int launch_decode(const PagedDev& c, const DecodeParams& p, const DecodePlan& d,
         return set_error(FBA_ERR_LAUNCH, "fba_paged_decode: cannot raise the dynamic shared memory limit");
     }
     const unsigned rows = static_cast<unsigned>(d.rows);
-    int rc = launch_chained(paged_decode_kernel<kE4m3, NT>, dim3(d.n_ctas ? d.n_ctas : rows), kDecThreads, smem, stream, c, p);
-    const int heads = d.n_ctas == 0 ? 0 : p.group < 8 * NT ? p.group : 8 * NT;
+    int rc = launch_chained(paged_decode_kernel<kE4m3, NT>, dim3(static_cast<unsigned>(d.n_ctas)), kDecThreads, smem, stream, c, p);
+    const int heads = d.splits == 1 ? 0 : p.group < 8 * NT ? p.group : 8 * NT;
     const int stretches = p.scores ? (d.score_stride + kWeighSlots - 1) / kWeighSlots : 0;
     if (rc == FBA_OK && heads + stretches > 0)
         // A row may have many parts where there are few rows: more warps take them then.
-        rc = d.n_ctas > 16 * d.rows ? launch_chained(paged_finish_kernel<NT, 16>, dim3(rows, heads + stretches), 512, 0, stream, c, p, heads)
+        rc = d.splits == 0 && d.n_ctas > 16 * d.rows ? launch_chained(paged_finish_kernel<NT, 16>, dim3(rows, heads + stretches), 512, 0, stream, c, p, heads)
                                     : launch_chained(paged_finish_kernel<NT, 4>, dim3(rows, heads + stretches), 128, 0, stream, c, p, heads);
     return rc;
 }
@@ -1015,6 +1036,7 @@ extern "C" int fba_paged_decode(const fba_paged_t* cache, const void* q, const i
     p.q_tiles = d.q_tiles;
     p.window = window;
     p.sinks = sinks;
+    p.splits = d.splits;
     p.n_ctas = d.n_ctas;
     p.scale_log2 = softmax_scale * kLog2e;
     if (cache->e4m3) return d.nt == 1 ? launch_decode<true, 1>(c, p, d, stream) : launch_decode<true, 2>(c, p, d, stream);

@@ -127,17 +127,23 @@ def test_c_decode_refuses_bad_arguments(lib):
 
 
 @pytest.mark.parametrize("e4m3", [0, 1])
-@pytest.mark.parametrize("B,Hq,Hkv,page,mp", [(1, 1, 1, 16, 40), (64, 32, 8, 64, 128), (300, 34, 2, 16, 100)])
-def test_workspace_holds_a_slot_for_every_seam(lib, B, Hq, Hkv, page, mp, e4m3):
-    """A CTA's part of a row goes to slot CTA + row; both count from 0."""
+@pytest.mark.parametrize("B,Hq,Hkv,page,mp", [(1, 1, 1, 16, 40), (30, 32, 8, 64, 128), (64, 32, 8, 64, 128), (200, 34, 2, 16, 400),
+                                              (300, 34, 2, 16, 100)])
+def test_workspace_holds_a_slot_for_every_part(lib, B, Hq, Hkv, page, mp, e4m3):
+    """Few rows: a CTA's part of a row goes to slot CTA + row, both counted from 0.  Many: parts of a row side by side."""
     n = ctypes.c_uint64()
     assert lib.fba_paged_decode_workspace_bytes(B, Hq, Hkv, page, mp, e4m3, 0, ctypes.byref(n)) == 0
     group = Hq // Hkv
     nt = 2 if group > 8 else 1
     rows = B * Hkv * -(-group // (8 * nt))
     tiles = mp * page // 16
-    ctas = min(148 * (3 if e4m3 and nt == 1 else 2), -(-rows * tiles // 16))
-    assert n.value >= (ctas + rows) * 8 * nt * (128 + 2) * 4
+    slots = min(148 * (3 if e4m3 and nt == 1 else 2), -(-rows * tiles // 16)) + rows
+    if rows >= 444:
+        slots = rows * max(1, min(-(-1184 // rows), tiles // 128))
+        if slots == rows:
+            assert n.value == 0   # nothing to join
+            return
+    assert n.value >= slots * 8 * nt * (128 + 2) * 4
 
 
 def test_oracle_evict_by_hand():
