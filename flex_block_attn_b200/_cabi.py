@@ -180,11 +180,11 @@ def lib() -> ctypes.CDLL:
     L.fba_paged_evict.restype = i32
     L.fba_paged_evict.argtypes = [paged, i32, vp, i32, i32, i32, vp, vp, i32, vp, vp, ctypes.c_uint64, vp, vp]
     L.fba_window_fwd.restype = i32
-    L.fba_window_fwd.argtypes = [vp] * 5 + [i32] * 7 + [ctypes.c_float, vp, vp]
+    L.fba_window_fwd.argtypes = [vp] * 6 + [i32] * 7 + [ctypes.c_float, vp, vp]
     L.fba_window_partial_bytes.restype = i32
     L.fba_window_partial_bytes.argtypes = [i32] * 7 + [ctypes.POINTER(ctypes.c_uint64)]
     L.fba_window_bwd.restype = i32
-    L.fba_window_bwd.argtypes = [vp] * 9 + [i32] * 7 + [ctypes.c_float, vp, vp, vp, ctypes.c_uint64, vp, vp]
+    L.fba_window_bwd.argtypes = [vp] * 10 + [i32] * 7 + [ctypes.c_float, vp, vp, vp, ctypes.c_uint64, vp, vp]
     L.fba_bwd_static_scratch_max_rows.restype = ctypes.c_uint64
     L.fba_bwd_static_scratch_max_rows.argtypes = []
     L.fba_bwd_static_scratch.restype = i32

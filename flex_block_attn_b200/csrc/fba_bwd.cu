@@ -118,13 +118,14 @@ struct BwdParams {
 
 // ------------------------------------------------------------------------------------------
 // kZero: also the zeros in the dQ accumulator, 512 bytes a row, instead of a memset behind it (under a window: the backward
-// takes 4 us less, at 1531 rows 48 instead of 52).
+// takes 4 us less, at 1531 rows 48 instead of 52); and O with what its rounding left, if there is that.
 template <bool kZero>
 __global__ void __launch_bounds__(256) bwd_prep_kernel(const __nv_bfloat16* __restrict__ o,
                                                       const __nv_bfloat16* __restrict__ dout,
                                                       const float* __restrict__ lse,
                                                       float2* __restrict__ ld, uint32_t Sq, uint32_t rows_pad,
-                                                      uint32_t total_rows, float scale, float4* __restrict__ accum) {
+                                                      uint32_t total_rows, float scale, float4* __restrict__ accum,
+                                                      const __nv_bfloat16* __restrict__ o_rest) {
     // A half-warp per row (16 bytes of O and of dO per lane), two rows per half-warp in flight, a
     // grid-stride loop over groups of four rows per warp.  Row counts fit 32 bits (host-checked):
     // 64-bit divisions per row would cost more than the row's memory traffic.
@@ -135,7 +136,7 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(const __nv_bfloat16* __re
     for (uint32_t base = warp * 4; base < total_rows; base += n_warps * 4) {
         uint32_t w[2];
         bool live[2];
-        uint4 a[2], b[2];
+        uint4 a[2], b[2], rest[2];
         float l[2];
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -143,13 +144,14 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(const __nv_bfloat16* __re
             const uint32_t bh = w[u] / rows_pad;
             const uint32_t r = w[u] - bh * rows_pad;
             live[u] = w[u] < total_rows && r < Sq;
-            a[u] = b[u] = make_uint4(0u, 0u, 0u, 0u);
+            a[u] = b[u] = rest[u] = make_uint4(0u, 0u, 0u, 0u);
             l[u] = -INFINITY;
             if (live[u]) {
                 const unsigned long long row = static_cast<unsigned long long>(bh) * Sq + r;
                 a[u] = reinterpret_cast<const uint4*>(o + row * 128)[l16];
                 b[u] = reinterpret_cast<const uint4*>(dout + row * 128)[l16];
                 l[u] = lse[row];
+                if (kZero && o_rest) rest[u] = reinterpret_cast<const uint4*>(o_rest + row * 128)[l16];
             }
             if (kZero && w[u] < total_rows) {
                 accum[w[u] * 32ull + l16] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -163,8 +165,9 @@ __global__ void __launch_bounds__(256) bwd_prep_kernel(const __nv_bfloat16* __re
             float s = 0.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float2 x = __bfloat1622float2(a2[j]);
+                float2 x = __bfloat1622float2(a2[j]);
                 const float2 y = __bfloat1622float2(b2[j]);
+                if (kZero) x = add2(x, __bfloat1622float2(reinterpret_cast<const __nv_bfloat162*>(&rest[u])[j]));
                 s = fmaf(x.x, y.x, s);
                 s = fmaf(x.y, y.y, s);
             }
@@ -921,7 +924,7 @@ extern "C" int fba_bwd_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv, ui
 }
 
 // Row statistics, and zeros in the dQ accumulator (null: none is used), by the same kernel with `fused`.
-static int launch_prep(const void* o, const void* dout, const float* lse, float* lse_delta, float* dq_accum, int Sq,
+static int launch_prep(const void* o, const void* o_rest, const void* dout, const float* lse, float* lse_delta, float* dq_accum, int Sq,
                        long long n_bhq, float scale, bool fused, cudaStream_t stream) {
     const int rows_pad = (Sq + 127) / 128 * 128;
     const long long total_rows = n_bhq * rows_pad;
@@ -932,7 +935,8 @@ static int launch_prep(const void* o, const void* dout, const float* lse, float*
     kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(
         static_cast<const __nv_bfloat16*>(o), static_cast<const __nv_bfloat16*>(dout), lse,
         reinterpret_cast<float2*>(lse_delta), static_cast<uint32_t>(Sq), static_cast<uint32_t>(rows_pad),
-        static_cast<uint32_t>(total_rows), scale, reinterpret_cast<float4*>(dq_accum));
+        static_cast<uint32_t>(total_rows), scale, reinterpret_cast<float4*>(dq_accum),
+        static_cast<const __nv_bfloat16*>(o_rest));
     const int rc = check_launch("bwd_prep_kernel");
     if (rc != FBA_OK) return rc;
     if (dq_accum && !fused &&
@@ -1017,7 +1021,7 @@ extern "C" int fba_bwd_split(const void* q, const void* k, const void* v, const 
     if ((rc = make_tmap_bf16(&tm_dv, dv, Skv, n_bhk, 128)) != FBA_OK) return rc;
     if (qmajor && (rc = make_tmap_bf16(&tm_dq, dq, Sq, n_bhq, 128)) != FBA_OK) return rc;
 
-    rc = launch_prep(o, dout, lse, lse_delta, qmajor ? nullptr : dq_accum, Sq, n_bhq, softmax_scale, false, stream);
+    rc = launch_prep(o, nullptr, dout, lse, lse_delta, qmajor ? nullptr : dq_accum, Sq, n_bhq, softmax_scale, false, stream);
     if (rc != FBA_OK) return rc;
     {
         BwdParams p;
@@ -1145,8 +1149,8 @@ extern "C" int fba_window_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv,
     return FBA_OK;
 }
 
-extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                              const void* dout, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq, int Skv,
+extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest,
+                              const float* lse, const void* dout, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq, int Skv,
                               int window, int sinks, float softmax_scale, float* lse_delta, float* dq_accum,
                               float* partial, uint64_t partial_bytes, uint32_t* status, void* stream_) {
     ProfRange range("fba_window_bwd");
@@ -1156,6 +1160,8 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     WindowDev win;
     int rc = window_args("fba_window_bwd", B, Hq, Hkv, Sq, Skv, window, sinks, softmax_scale, &win);
     if (rc != FBA_OK) return rc;
+    if (reinterpret_cast<uintptr_t>(o_rest) % 16 != 0)
+        return set_error(FBA_ERR_BAD_ARG, "fba_window_bwd: o_rest must be 16-byte aligned");
     const long long n_bhq = static_cast<long long>(B) * Hq, n_bhk = static_cast<long long>(B) * Hkv;
     const WindowSplit w = window_split(B, Hq, Hkv, Sq, Skv, win);
     const uint64_t need = window_partial_bytes_of(w, n_bhk);
@@ -1175,7 +1181,7 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     if ((rc = make_tmap_bf16(&tm_do, dout, Sq, n_bhq, 128)) != FBA_OK) return rc;
     if ((rc = make_tmap_bf16(&tm_dk, dk, Skv, n_bhk, 128)) != FBA_OK) return rc;
     if ((rc = make_tmap_bf16(&tm_dv, dv, Skv, n_bhk, 128)) != FBA_OK) return rc;
-    if ((rc = launch_prep(o, dout, lse, lse_delta, dq_accum, Sq, n_bhq, softmax_scale, true, stream)) != FBA_OK) return rc;
+    if ((rc = launch_prep(o, o_rest, dout, lse, lse_delta, dq_accum, Sq, n_bhq, softmax_scale, true, stream)) != FBA_OK) return rc;
 
     BwdParams p = {};
     p.ld = reinterpret_cast<const float2*>(lse_delta);

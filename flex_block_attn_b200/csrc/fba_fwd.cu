@@ -53,6 +53,7 @@ struct FwdParams {
     int n_mtiles, Sq, Hq, Hkv;
     float scale_log2;      // softmax scale * log2(e)
     WindowDev win;         // fba_window_fwd alone, as are:
+    __nv_bfloat16* o_rest; //   null, or what the rounding of O to bf16 leaves, rounded as well: [B, Hq, Sq, 128]
     int n_pairs, n_bh;     //   pairs of query tiles per head, heads
     int heads_at_once;     //   heads whose pairs take turns in the grid
     int one_tile;          //   not 0: a CTA has one query tile instead of a pair
@@ -581,6 +582,21 @@ fba_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
                                            static_cast<uint32_t>(row) * 128u +
                                            (static_cast<uint32_t>((chunk & 7) ^ (row & 7)) << 4);
                         *reinterpret_cast<uint4*>(stage + o) = w;
+                        if constexpr (kWindow) {
+                            // A thread writes its own row here: with no wait behind it, unlike a second trip through the
+                            // staging buffer.
+                            if (p.o_rest != nullptr && mt * 128 + row < p.Sq) {
+                                const uint32_t hi[4] = {w.x, w.y, w.z, w.w};
+                                uint32_t lo[4];
+#pragma unroll
+                                for (int j = 0; j < 4; ++j)
+                                    lo[j] = pack_bf16x2(
+                                        fmaf(__uint_as_float(v[8 * q4 + 2 * j]), inv_l, -__uint_as_float(hi[j] << 16)),
+                                        fmaf(__uint_as_float(v[8 * q4 + 2 * j + 1]), inv_l, -__uint_as_float(hi[j] & 0xffff0000u)));
+                                reinterpret_cast<uint4*>(p.o_rest)[(static_cast<long long>(bh) * p.Sq + mt * 128 + row) * 16 + chunk] =
+                                    make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                            }
+                        }
                     }
                 }
                 const int grow = mt * 128 + row;
@@ -620,8 +636,8 @@ static int check_list(const fba_list_t* l, const char* who) {
 }
 
 // Launches the kernel over lists (q2k) or under a window (win); the arguments have been checked.
-static int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv, int Sq,
-                      int Skv, const fba_list_t* q2k, const WindowDev* win, float softmax_scale, uint32_t* status,
+static int launch_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest, int B, int Hq, int Hkv,
+                      int Sq, int Skv, const fba_list_t* q2k, const WindowDev* win, float softmax_scale, uint32_t* status,
                       cudaStream_t stream) {
     int rc;
     const int n_mtiles = (Sq + 127) / 128;
@@ -646,6 +662,7 @@ static int launch_fwd(const void* q, const void* k, const void* v, void* o, floa
     FwdParams p;
     p.list = win ? ListDev{} : to_dev(*q2k);
     p.win = win ? *win : WindowDev{};
+    p.o_rest = static_cast<__nv_bfloat16*>(o_rest);
     p.lse = lse;
     p.status = status;
     p.n_mtiles = n_mtiles;
@@ -705,18 +722,20 @@ static int fwd_impl(const void* q, const void* k, const void* v, void* o, float*
                          "fba_fwd: ceil(Skv/128) must be a multiple of q2k->sub and ceil(Sq/128) of q2k->rows_div");
     if (static_cast<long long>(B) * Hq > 65535)
         return set_error(FBA_ERR_TOO_LARGE, "fba_fwd: B * Hq exceeds 65535");
-    return launch_fwd(q, k, v, o, lse, B, Hq, Hkv, Sq, Skv, q2k, nullptr, softmax_scale, status, stream);
+    return launch_fwd(q, k, v, o, lse, nullptr, B, Hq, Hkv, Sq, Skv, q2k, nullptr, softmax_scale, status, stream);
 }
 
-extern "C" int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv,
-                              int Sq, int Skv, int window, int sinks, float softmax_scale, uint32_t* status,
+extern "C" int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest, int B, int Hq,
+                              int Hkv, int Sq, int Skv, int window, int sinks, float softmax_scale, uint32_t* status,
                               void* stream) {
     ProfRange range("fba_window_fwd");
     if (!q || !k || !v || !o || !status) return set_error(FBA_ERR_BAD_ARG, "fba_window_fwd: null pointer argument");
     WindowDev win;
     int rc = window_args("fba_window_fwd", B, Hq, Hkv, Sq, Skv, window, sinks, softmax_scale, &win);
     if (rc != FBA_OK) return rc;
-    return launch_fwd(q, k, v, o, lse, B, Hq, Hkv, Sq, Skv, nullptr, &win, softmax_scale, status,
+    if (reinterpret_cast<uintptr_t>(o_rest) % 16 != 0)
+        return set_error(FBA_ERR_BAD_ARG, "fba_window_fwd: o_rest must be 16-byte aligned");
+    return launch_fwd(q, k, v, o, lse, o_rest, B, Hq, Hkv, Sq, Skv, nullptr, &win, softmax_scale, status,
                       static_cast<cudaStream_t>(stream));
 }
 

@@ -35,26 +35,30 @@ def _sizes(q, k, v) -> tuple[int, int, int, int, int]:
     return B, Hq, Hkv, Sq, Skv
 
 
-def forward_with_window(q, k, v, window: Optional[int], sinks: int = 0, softmax_scale=None, need_lse: bool = True):
-    """Forward kernel alone; returns (o bf16 [B, Hq, Sq, 128], lse fp32 [B, Hq, Sq] or None).  A row that sees no key
-    (possible when Sq > Skv) is zero, its lse -inf."""
+def forward_with_window(q, k, v, window: Optional[int], sinks: int = 0, softmax_scale=None, need_lse: bool = True,
+                        need_rest: bool = False):
+    """Forward kernel alone; returns (o bf16 [B, Hq, Sq, 128], lse fp32 [B, Hq, Sq] or None), and with ``need_rest`` what the
+    rounding of o left, for ``backward_with_window``.  A row that sees no key (possible when Sq > Skv) is zero, its lse
+    -inf."""
     w, s = _window_of(window, sinks)
     B, Hq, Hkv, Sq, Skv = _sizes(q, k, v)
     dev = q.device
     o = torch.empty_like(q)
     lse = q.new_empty((B, Hq, Sq), dtype=torch.float32) if need_lse else None
-    _poisoned(o, lse)
+    rest = torch.empty_like(q) if need_rest else None
+    _poisoned(o, lse, rest)
     mon = _monitor(dev)
     mon.poll_mapped()
-    rc = _cabi.lib().fba_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), B, Hq, Hkv, Sq, Skv, w,
-                                    s, _scale_of(softmax_scale), mon.mapped_ptr, _raw_stream(dev.index))
+    rc = _cabi.lib().fba_window_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(lse), _ptr(rest), B, Hq, Hkv, Sq,
+                                    Skv, w, s, _scale_of(softmax_scale), mon.mapped_ptr, _raw_stream(dev.index))
     _checked(rc, "fba_window_fwd", dev)
-    return o, lse
+    return (o, lse, rest) if need_rest else (o, lse)
 
 
-def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: int = 0, softmax_scale=None):
-    """Backward kernels; ``o`` and ``lse`` are the forward's.  Returns (dq, dk, dv) in bf16.  dK and dV are reproducible
-    bit by bit; dQ is summed in fp32 in scheduling order."""
+def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: int = 0, softmax_scale=None, rest=None):
+    """Backward kernels; ``o``, ``lse`` and, if it was asked for, ``rest`` are the forward's.  Returns (dq, dk, dv) in bf16.
+    dK and dV are reproducible bit by bit; dQ is summed in fp32 in scheduling order.  ``rest`` makes the gradients more
+    exact, those of rows that see few keys most."""
     w, s = _window_of(window, sinks)
     B, Hq, Hkv, Sq, Skv = _sizes(q, k, v)
     dev = q.device
@@ -65,8 +69,10 @@ def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: in
         raise TypeError("lse must be torch.float32")
     if dout.shape != q.shape or o.shape != q.shape or o.dtype != torch.bfloat16:
         raise ValueError("o and dout must have the shape of q, and o its type")
-    if not dout.device == o.device == lse.device == dev:
-        raise RuntimeError("o, lse and dout must be on the device of q")
+    if rest is not None and (rest.shape != q.shape or rest.dtype != torch.bfloat16 or not rest.is_contiguous()):
+        raise ValueError("rest must be the forward's")
+    if not dout.device == o.device == lse.device == dev or (rest is not None and rest.device != dev):
+        raise RuntimeError("o, lse, rest and dout must be on the device of q")
     lib = _cabi.lib()
     n = ctypes.c_uint64(0)
     _cabi.check(lib.fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, w, s, ctypes.byref(n)), "fba_window_partial_bytes")
@@ -79,8 +85,8 @@ def backward_with_window(q, k, v, o, lse, dout, window: Optional[int], sinks: in
     at = scratch.data_ptr()
     mon = _monitor(dev)
     mon.poll_mapped()
-    rc = lib.fba_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), lse.data_ptr(), dout.data_ptr(),
-                            dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Hq, Hkv, Sq, Skv, w, s, _scale_of(softmax_scale),
+    rc = lib.fba_window_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _ptr(rest), lse.data_ptr(),
+                            dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, Hq, Hkv, Sq, Skv, w, s, _scale_of(softmax_scale),
                             at, at + rows * 8, at + rows * 520 if n.value else None, n.value, mon.mapped_ptr,
                             _raw_stream(dev.index))
     _checked(rc, "fba_window_bwd", dev)
@@ -91,16 +97,18 @@ class SlidingWindowAttnFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, softmax_scale, is_grad_enabled):
         is_grad = is_grad_enabled and any(x.requires_grad for x in (q, k, v))
-        o, lse = forward_with_window(q, k, v, window, sinks, softmax_scale, need_lse=is_grad)
-        if is_grad:
-            ctx.save_for_backward(q, k, v, o, lse)
-            ctx.args = (window, sinks, softmax_scale)
+        if not is_grad:
+            return forward_with_window(q, k, v, window, sinks, softmax_scale, need_lse=False)[0]
+        o, lse, rest = forward_with_window(q, k, v, window, sinks, softmax_scale, need_rest=True)
+        ctx.save_for_backward(q, k, v, o, lse, rest)
+        ctx.args = (window, sinks, softmax_scale)
         return o
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout):
-        return *backward_with_window(*ctx.saved_tensors, dout, *ctx.args), None, None, None, None
+        *saved, rest = ctx.saved_tensors
+        return *backward_with_window(*saved, dout, *ctx.args, rest), None, None, None, None
 
 
 def sliding_window_attn_func(q, k, v, window, sinks=0, softmax_scale=None):

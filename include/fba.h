@@ -300,17 +300,21 @@ int fba_bwd_split(const void* q, const void* k, const void* v, const void* o, co
  * only tiles that hold visible pairs.  K and V must be finite: a NaN or infinity in a value row may also reach rows of
  * the same 128-row tiles that do not see it (0 * inf in the product).
  *
+ * o_rest (bf16 like o, 16-byte aligned, or NULL): the forward writes what the rounding of o left, the backward adds it to o
+ * where it forms rowsum(dO * O).  Rows that see few keys need it: dS is the difference of nearly equal values there (two
+ * keys: dQ 0.7 % off without, 0.3 % with it); in long rows it is worth a quarter of the error.
+ *
  * Backward: scratch buffers as fba_bwd's (fba_bwd_scratch_bytes; dq_accum is zeroed by the call and 16-byte aligned), and
  * `partial`, 16-byte aligned, of fba_window_partial_bytes() bytes, at most 74 MB (0: NULL is accepted), for the fp32 dK / dV
  * of key tiles with long lists (sinks, which every query sees; all tiles where there are few kv heads), whose steps are
  * divided over several CTAs.  dK and dV have the same bits in every call with the same sizes; a call on part of the batch
  * or of the kv heads may divide other tiles and differ in the last bit.  dQ is summed in scheduling order, like fba_bwd's.
  */
-int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, int B, int Hq, int Hkv, int Sq,
-                   int Skv, int window, int sinks, float softmax_scale, uint32_t* status, void* stream);
+int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest, int B, int Hq, int Hkv,
+                   int Sq, int Skv, int window, int sinks, float softmax_scale, uint32_t* status, void* stream);
 int fba_window_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks, uint64_t* bytes);
-int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* dout,
-                   void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks,
+int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, const void* o_rest, const float* lse,
+                   const void* dout, void* dq, void* dk, void* dv, int B, int Hq, int Hkv, int Sq, int Skv, int window, int sinks,
                    float softmax_scale, float* lse_delta, float* dq_accum, float* partial, uint64_t partial_bytes,
                    uint32_t* status, void* stream);
 

@@ -58,9 +58,9 @@ def test_c_entry_points_refuse_bad_arguments():
     sizes = (1, 2, 1, 16, 16)
 
     def fwd(sizes=sizes, window=4, sinks=0, scale=0.1):
-        return lib.fba_window_fwd(some, some, some, some, None, *sizes, window, sinks, scale, some, None)
+        return lib.fba_window_fwd(some, some, some, some, None, None, *sizes, window, sinks, scale, some, None)
 
-    assert lib.fba_window_fwd(None, some, some, some, None, *sizes, 4, 0, 0.1, some, None) == -1
+    assert lib.fba_window_fwd(None, some, some, some, None, None, *sizes, 4, 0, 0.1, some, None) == -1
     for bad in ((0, 2, 1, 16, 16), (1, 2, 1, 0, 16), (1, 2, 1, 16, 0), (1, 3, 2, 16, 16)):
         assert fwd(bad) == -1
     assert fwd(window=-1) == -1 and fwd(sinks=-1) == -1
@@ -75,7 +75,8 @@ def test_c_entry_points_refuse_bad_arguments():
         assert lib.fba_window_partial_bytes(8, 64, 64, 5000, 5000, window, sinks, ctypes.byref(n)) == 0 and n.value == 0
     assert lib.fba_window_partial_bytes(1, 8, 1, 5000, 5000, 100, 5, ctypes.byref(n)) == 0
     assert 0 < n.value <= 592 * 2**17 and n.value % 2**17 == 0
-    bwd = [some] * 9 + [1, 8, 1, 5000, 5000, 100, 5, 0.1, some, some]
+    assert lib.fba_window_fwd(some, some, some, some, None, ctypes.c_void_p(8), *sizes, 4, 0, 0.1, some, None) == -1   # o_rest
+    bwd = [some] * 10 + [1, 8, 1, 5000, 5000, 100, 5, 0.1, some, some]
     assert lib.fba_window_bwd(*bwd, None, 0, some, None) == -1                       # the partial buffer is missing,
     assert lib.fba_window_bwd(*bwd, some, n.value - 1, some, None) == -1             # too small,
     assert lib.fba_window_bwd(*bwd, ctypes.c_void_p(8), n.value, some, None) == -1   # misaligned

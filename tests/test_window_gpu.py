@@ -264,3 +264,30 @@ def test_divided_key_tiles(B, Hq, Hkv, Sq, Skv, window, sinks):
         close(got, w, what)
     again = fba.backward_with_window(q, k, v, o, lse, do, window, sinks)
     assert torch.equal(grads[1], again[1]) and torch.equal(grads[2], again[2])
+
+
+@pytest.mark.parametrize("S,window,sinks", [(2, None, 0), (3, None, 0), (300, 2, 0), (300, 2, 1), (300, 5, 0)])
+def test_gradients_of_rows_that_see_few_keys(S, window, sinks):
+    """dS is the difference of nearly equal values there; what the rounding of O left keeps it exact.  Element by element:
+    dS and the result are rounded (u each), and dP - delta is off by the rounding of P in O = P V (u of each p |dO V|; O's own
+    rounding would add u |dO| |O|) and of fp32 sums of 128 products and O's second part (2^-16 of |dO| |V| + |dO| |O|),
+    times P, the scale and a key (a query)."""
+    import flex_block_attn_b200 as fba
+
+    q, k, v, do = rand_qkv(2, 4, 2, S, S, seed=S + (window or 0), device="cuda")
+    mask = orc.visible(S, S, window, sinks, "cuda")
+    _, lse, dq, dk, _ = orc.masked_attention(q, k, v, mask, do)
+    o = orc.masked_attention(q, k, v, mask)[0]
+    ke, ve = (x.double().repeat_interleave(2, 1) for x in (k, v))
+    scale, Q, dO = 128**-0.5, q.double(), do.double()
+    p = ((Q @ ke.transpose(-1, -2) * scale).masked_fill(~mask, -math.inf) - lse[..., None]).exp()
+    dp = dO @ ve.transpose(-1, -2)
+    ds = p * (dp - (dO * o).sum(-1, keepdim=True)) * scale
+    norm = lambda x: x.norm(dim=-1)  # noqa: E731
+    noise = p * scale * 2.0**-16 * norm(dO)[..., None] * (norm(ve)[..., None, :] + norm(o)[..., None])
+    off = (U + 2.0**-18) * ds.abs() + U * scale * p * (p * dp.abs()).sum(-1, keepdim=True) + noise
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    got = torch.autograd.grad(fba.sliding_window_attn_func(*leaves, window, sinks), leaves, do)
+    around = (off @ ke.abs(), (off.transpose(-1, -2) @ Q.abs()).unflatten(1, (2, 2)).sum(2))
+    for g, w, a, what in zip(got, (dq, dk), around, ("dQ", "dK")):
+        assert ((g.double() - w).abs() <= (1 + U) * a + U * w.abs()).all(), what
