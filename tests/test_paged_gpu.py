@@ -337,3 +337,58 @@ def test_prompt_then_tokens_equals_attention_over_the_whole():
         for b in range(2):
             assert (o[b].double() - want[b][:, prompt[b] + step]).abs().max() <= 8 * U * most
     fba.check_status()
+
+
+def test_c_callers_with_status_words_on_the_device():
+    """The entry points report into device memory as well; fba_check_status reads and clears it."""
+    import ctypes
+
+    from flex_block_attn_b200 import _cabi, paged
+
+    lib = _cabi.lib()
+    pools, table = make([40], 1, 16, seed=3)
+    table[0, 1] = 12345
+    tab = table.cuda()
+    arg, B, dev = paged._cache_arg(to_gpu(pools), tab)
+    status = torch.zeros(8, dtype=torch.int32, device="cuda")
+    q, n = queries(1, 2, 3).cuda(), torch.tensor([40], dtype=torch.int32).cuda()
+    o = torch.empty_like(q)
+    stream = torch.cuda.current_stream().cuda_stream
+    rc = lib.fba_paged_decode(ctypes.byref(arg), q.data_ptr(), (ctypes.c_int64 * 2)(256, 128), o.data_ptr(), None, 1, 2,
+                              n.data_ptr(), 0, 0, 0.1, 0, None, 0, status.data_ptr(), stream)
+    assert rc == 0
+    assert lib.fba_check_status(status.data_ptr(), stream) == _cabi.FBA_ERR_BAD_CACHE
+    assert b"page number 12345 for sequence 0" in lib.fba_last_error()
+    assert lib.fba_check_status(status.data_ptr(), stream) == 0
+    check(q.cpu(), pools, torch.cat((table[:, :1], table[:, 2:]), 1), [24], o, None, scale=0.1)
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+def test_pools_beyond_32_bit_offsets(e4m3):
+    """The highest pages of pools of 9 (4.6) GB each: writer, attention and eviction reach the rows they mean."""
+    import flex_block_attn_b200 as fba
+
+    n_pages, Hkv, page = 70000, 2, 256
+    shape = (n_pages, Hkv, page)
+    new = lambda dtype, *more: torch.empty((*shape, *more), dtype=dtype, device="cuda")  # noqa: E731
+    kind = torch.uint8 if e4m3 else torch.bfloat16
+    cache = fba.PagedKVCache(new(kind, 128), new(kind, 128), weight=new(torch.float32), position=new(torch.int32))
+    if e4m3:
+        cache.k_scale, cache.v_scale = new(torch.float32), new(torch.float32)
+    table = torch.tensor([[n_pages - 1, n_pages - 3, 5]], dtype=torch.int32, device="cuda")
+    g = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((1, Hkv, 700, 128), generator=g).bfloat16().cuda() for _ in "kv")
+    lens = fba.append_kv(cache, k, v, table, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    small = fba.new_paged_cache(3, Hkv, page, e4m3, track=True)   # the same in a small pool
+    near = torch.tensor([[2, 0, 1]], dtype=torch.int32, device="cuda")
+    fba.append_kv(small, k, v, near, torch.zeros(1, dtype=torch.int32, device="cuda"))
+    q = queries(1, 8, 2).cuda()
+    for step in range(2):
+        assert torch.equal(fba.paged_decode_attn(q, cache, table, lens, accumulate=True),
+                           fba.paged_decode_attn(q, small, near, lens, accumulate=True))
+        for name in ("k", "v", "weight", "position") + (("k_scale", "v_scale") if e4m3 else ()):
+            for p, m in zip(table[0].tolist(), near[0].tolist()):
+                rows = max(0, min(page, int(lens[0]) - table[0].tolist().index(p) * page))
+                assert torch.equal(getattr(cache, name)[p, :, :rows], getattr(small, name)[m, :, :rows]), name
+        lens, fewer = fba.evict_kv(cache, table, lens, 300, 4, 10), fba.evict_kv(small, near, lens, 300, 4, 10)
+        assert torch.equal(lens, fewer)
