@@ -325,10 +325,7 @@ using namespace fba;
 namespace {
 // Up to so many rows a head are copied by the CTA that chose them; more by a kernel of their own, whose launch costs
 // less than leaving most SMs idle.
-#ifndef MVH
-#define MVH 256
-#endif
-constexpr int kMoveHere = MVH;
+constexpr int kMoveHere = 256;
 int evict_list(int page_size, int max_pages, int budget) {
     const long long cap = static_cast<long long>(max_pages) * page_size;
     return static_cast<int>(cap < budget ? cap : budget);
@@ -418,6 +415,7 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     // Blocks for all of a head's entries while the grid stays within a few waves; a warp takes further batches beyond.
     long long blocks = (most + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
     const long long enough = (148 * 16 + heads - 1) / heads;
-    return launch_chained(cache->e4m3 ? paged_move_kernel<true> : paged_move_kernel<false>, dim3(static_cast<unsigned>(blocks < enough ? blocks : enough), static_cast<unsigned>(heads)),
-                          kMoveWarps * 32, 0, static_cast<cudaStream_t>(stream), c, p);
+    const dim3 grid(static_cast<unsigned>(blocks < enough ? blocks : enough), static_cast<unsigned>(heads));
+    return launch_chained(cache->e4m3 ? paged_move_kernel<true> : paged_move_kernel<false>, grid, kMoveWarps * 32, 0,
+                          static_cast<cudaStream_t>(stream), c, p);
 }

@@ -331,8 +331,8 @@ int fba_window_bwd(const void* q, const void* k, const void* v, const void* o, c
  * Lengths (`seq_lens`, int32 [B]) are read on the device.  A page number outside 0 .. n_pages - 1, or a length outside
  * 0 .. max_pages * page_size, is never followed: the kernel leaves out the rows concerned (holds the length to the limit)
  * and reports it in the status words (device memory, or pinned host memory that a caller can look at without a copy);
- * fba_check_status(), which reads device memory, then returns FBA_ERR_BAD_CACHE.  Pages that a call writes must belong to
- * one sequence only; pages that are read may be shared.
+ * fba_check_status(), which reads device memory, then returns FBA_ERR_BAD_CACHE.  A page that a call writes (keys, weights
+ * or positions) must stand in the tables once only; pages that are only read may be shared.
  */
 typedef struct fba_paged {
     void* k;
