@@ -38,11 +38,12 @@ struct EvictParams {
 };
 
 struct EvictShared {
-    uint32_t hist[kEvBins];
+    uint32_t hist[2][kEvBins];     // in turns, so that one may be filled while other CTAs still read the other
     uint32_t scan[kEvWarps];
+    uint2 least[kEvWarps], least_cta;   // smallest key and its slot
     uint2 count[2][kEvWarps];      // per warp: ties, then holes and moves
     uint2 total[2];                // of the CTA
-    uint32_t digit, below;         // of the bin that holds the wanted rank: its number, and how many keys lie before it
+    uint32_t digit, below, inside; // of the bin that holds the wanted rank: its number, how many keys lie before it and in it
 };
 
 __device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int pos, float weight, long long recent_from) {
@@ -69,51 +70,61 @@ __device__ __forceinline__ void copy_rows(const PagedDev& c, const EvictParams& 
     }
     uint4* pool = reinterpret_cast<uint4*>(kv ? c.v : c.k);
     for (int base = i0; base < total; base += stride) {
-        long long src = -1, dst = -1;
+        int src = -1, dst = -1;   // 32 bits do: 2^31 rows of keys and values are 512 GB
         if (base + lane < total) {
-            src = paged_row(c, b, h, from[base + lane], p.status);
-            dst = paged_row(dst_c, b, h, p.out_table ? base + lane : to[base + lane], p.status);
-            if (src < 0 || dst < 0) {
-                dst = -1;   // a page that is not there
+            const int f = from[base + lane], t = p.out_table ? base + lane : to[base + lane];
+            const int f_page = paged_page(c, b, f), t_page = paged_page(dst_c, b, t);
+            src = static_cast<int>(paged_row_in(c, f_page, h, f));
+            dst = static_cast<int>(paged_row_in(dst_c, t_page, h, t));
+            if (src < 0 || dst < 0) {   // a page that is not there
+                report_paged(p.status, kBadPage, b, src < 0 ? f_page : t_page);
+                dst = -1;
             } else {   // what there is one of per row
+                float ks, vs;
                 if (e4m3) {
-                    const float ks = c.k_scale[src], vs = c.v_scale[src];
-                    c.k_scale[dst] = ks;
-                    c.v_scale[dst] = vs;
+                    ks = c.k_scale[src];
+                    vs = c.v_scale[src];
                 }
                 const float w = c.weight[src];
                 const int pos = c.position[src];
                 c.weight[dst] = w;
                 c.position[dst] = pos;
+                if (e4m3) {
+                    c.k_scale[dst] = ks;
+                    c.v_scale[dst] = vs;
+                }
             }
         }
         const int n = min(32, total - base);
         constexpr int kFlight = 8;   // rows a lane has under way
         for (int j0 = 0; j0 < n; j0 += kFlight * tokens) {
             uint4 x[kFlight];
-            long long d[kFlight];
+            int d[kFlight];
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) {
                 const int j = j0 + u * tokens + sub;   // below 32 + 16; lanes repeat modulo 32
-                const long long s = __shfl_sync(0xffffffffu, src, j & 31);
+                const int s = __shfl_sync(0xffffffffu, src, j & 31);
                 d[u] = __shfl_sync(0xffffffffu, dst, j & 31);
                 if (j >= n) d[u] = -1;
-                if (d[u] >= 0) x[u] = pool[s * lanes + l];
+                if (d[u] >= 0) x[u] = pool[static_cast<long long>(s) * lanes + l];
             }
 #pragma unroll
             for (int u = 0; u < kFlight; ++u)
-                if (d[u] >= 0) pool[d[u] * lanes + l] = x[u];
+                if (d[u] >= 0) pool[static_cast<long long>(d[u]) * lanes + l] = x[u];
         }
     }
 }
 
+// kCtas: CTAs a head, one cluster.
+template <int kCtas>
 __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev c, const EvictParams p) {
-    extern __shared__ uint32_t keys[];
+    extern __shared__ __align__(16) uint32_t keys[];
     __shared__ EvictShared sh;
     pdl_launch_dependents();
     pdl_wait();
     cg::cluster_group cluster = cg::this_cluster();
-    const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    constexpr int ctas = kCtas;
+    const int rank = ctas > 1 ? static_cast<int>(cluster.block_rank()) : 0;
     auto sync_all = [&]() {
         if (ctas > 1) cluster.sync();
         else __syncthreads();
@@ -129,27 +140,33 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     }
     const long long recent_from = static_cast<long long>(p.next_positions ? p.next_positions[b] : n) - p.recent;
 
-    // This CTA's slots, and of them this warp's; both multiples of 32 long.
+    // This CTA's slots, and of them this warp's; but for the last, multiples of 32 and 128 long.
     const int per_cta = ((n + ctas - 1) / ctas + 31) / 32 * 32;
     const int begin = min(n, rank * per_cta), end = min(n, begin + per_cta);
-    const int per_warp = ((end - begin + kEvWarps - 1) / kEvWarps + 31) / 32 * 32;
+    const int per_warp = ((end - begin + kEvWarps - 1) / kEvWarps + 127) / 128 * 128;
     const int w_begin = min(end, begin + warp * per_warp), w_end = min(end, w_begin + per_warp);
     const bool cached = per_cta <= p.key_room;
     if (cached) {
         constexpr int kFlight = 8;
+        int bad_page = 0;
+        bool bad = false;
         for (int i0 = begin + tid; i0 < end; i0 += kFlight * kEvThreads) {
-            long long row[kFlight];
+            int page[kFlight];
+            int row[kFlight];
             float w[kFlight];
             int pos[kFlight];
 #pragma unroll
+            for (int u = 0; u < kFlight; ++u) page[u] = paged_page(c, b, min(i0 + u * kEvThreads, end - 1));
+#pragma unroll
             for (int u = 0; u < kFlight; ++u) {
-                const int i = i0 + u * kEvThreads;
-                row[u] = i < end ? paged_row(c, b, h, i, p.status) : -1;
+                row[u] = static_cast<int>(paged_row_in(c, page[u], h, min(i0 + u * kEvThreads, end - 1)));
+                if (row[u] < 0) bad_page = page[u], bad = true;
             }
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) {
-                w[u] = row[u] >= 0 ? c.weight[row[u]] : 0.f;
-                pos[u] = row[u] >= 0 ? c.position[row[u]] : 0;
+                const bool is = row[u] >= 0 && i0 + u * kEvThreads < end;
+                w[u] = is ? c.weight[row[u]] : 0.f;
+                pos[u] = is ? c.position[row[u]] : 0;
             }
 #pragma unroll
             for (int u = 0; u < kFlight; ++u) {
@@ -157,7 +174,9 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
                 if (i < end) keys[i - begin] = row[u] >= 0 ? evict_key(p, pos[u], w[u], recent_from) : 0u;
             }
         }
+        if (bad) report_paged(p.status, kBadPage, b, bad_page);
     }
+    for (int i = tid; i < 2 * kEvBins; i += kEvThreads) sh.hist[0][i] = 0;
     __syncthreads();
     auto key_of = [&](int i) {
         if (cached) return keys[i - begin];
@@ -166,41 +185,68 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
     };
 
     // T, and how many tokens with a smaller key there are.
+    int32_t* from = p.from + static_cast<long long>(head) * p.list;
+    int32_t* to = p.to + static_cast<long long>(head) * p.list;
     uint32_t prefix = 0, below = 0;
+    bool no_ties = leave == 0;   // all tokens with the key T leave
+    int total = -1;              // entries of the lists
     if (leave == 1) {   // one token too many, as at every step of serving within a budget: the smallest key, in one round
-        uint32_t least = 0xffffffffu;
-        for (int i = begin + tid; i < end; i += kEvThreads) least = min(least, key_of(i));
-        least = __reduce_min_sync(0xffffffffu, least);
-        if (lane == 0) sh.scan[warp] = least;
+        uint2 least = make_uint2(0xffffffffu, 0xffffffffu);
+        auto smaller = [](uint2 x, uint2 y) { return y.x < x.x || (y.x == x.x && y.y < x.y) ? y : x; };
+        auto least_of_warp = [](uint2 x) {
+            const uint32_t key = __reduce_min_sync(0xffffffffu, x.x);
+            return make_uint2(key, __reduce_min_sync(0xffffffffu, x.x == key ? x.y : 0xffffffffu));
+        };
+        for (int i = begin + tid; i < end; i += kEvThreads) least = smaller(least, make_uint2(key_of(i), i));
+        least = least_of_warp(least);
+        if (lane == 0) sh.least[warp] = least;
         __syncthreads();
-        prefix = __reduce_min_sync(0xffffffffu, sh.scan[lane]);
+        least = least_of_warp(sh.least[lane]);
         if (ctas > 1) {
-            if (tid == 0) sh.digit = prefix;
+            if (tid == 0) sh.least_cta = least;
             cluster.sync();
-            for (int r = 0; r < ctas; ++r) prefix = min(prefix, *cluster.map_shared_rank(&sh.digit, r));
+#pragma unroll
+            for (int r = 0; r < ctas; ++r) least = smaller(least, *cluster.map_shared_rank(&sh.least_cta, r));
+            cluster.sync();
         }
+        if (!p.out_table) {   // the last token takes the slot of the one that leaves, unless it is that one
+            total = static_cast<int>(least.y) < left;
+            if (rank == 0 && tid == 0) {   // whose warp copies it
+                from[0] = left;
+                to[0] = static_cast<int>(least.y);
+            }
+            __syncwarp();
+        }
+        prefix = least.x;
     } else if (leave > 1) {
         uint32_t rank_left = leave - 1;   // of the last token that leaves, among those that share the digits so far
 #pragma unroll
         for (int pass = 0; pass < 3; ++pass) {
             constexpr int kShift[3] = {21, 10, 0}, kBits[3] = {11, 11, 10};
             const int shift = kShift[pass], bins = 1 << kBits[pass];
-            for (int i = tid; i < bins; i += kEvThreads) sh.hist[i] = 0;
-            __syncthreads();
+            uint32_t* hist = sh.hist[pass & 1];
             for (int i = begin + tid; i < end; i += kEvThreads) {
                 const uint32_t k = key_of(i);
-                if (pass == 0 || (k >> kShift[pass ? pass - 1 : 0]) == prefix) atomicAdd(&sh.hist[(k >> shift) & (bins - 1)], 1u);
+                if (pass == 0 || (k >> kShift[pass ? pass - 1 : 0]) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1u);
             }
             sync_all();
+            if (pass == 1)   // for the third pass: all have read what it held
+                for (int i = tid; i < kEvBins; i += kEvThreads) sh.hist[0][i] = 0;
             // Thread t: bins 2 t and 2 t + 1 (t alone in the last pass) of all CTAs.
             constexpr int kPer = kEvBins / kEvThreads;
+            static_assert(kPer == 2, "a thread reads two bins at once");
             uint32_t mine[kPer] = {}, sum = 0;
             const int per = bins / kEvThreads;
-            for (int r = 0; r < ctas; ++r) {
-                const uint32_t* other = cluster.map_shared_rank(sh.hist, r);
 #pragma unroll
-                for (int x = 0; x < kPer; ++x)
-                    if (x < per) mine[x] += other[tid * per + x];
+            for (int r = 0; r < ctas; ++r) {
+                const uint32_t* other = ctas > 1 ? cluster.map_shared_rank(hist, r) : hist;
+                if (per == 2) {
+                    const uint2 y = reinterpret_cast<const uint2*>(other)[tid];
+                    mine[0] += y.x;
+                    mine[1] += y.y;
+                } else {
+                    mine[0] += other[tid];
+                }
             }
 #pragma unroll
             for (int x = 0; x < kPer; ++x) sum += mine[x];
@@ -212,92 +258,141 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
             }
             if (lane == 31) sh.scan[warp] = upto;
             __syncthreads();
-            uint32_t before = upto - sum;
-            for (int w = 0; w < warp; ++w) before += sh.scan[w];
+            uint32_t before = upto - sum + __reduce_add_sync(0xffffffffu, lane < warp ? sh.scan[lane] : 0u);
             if (rank_left >= before && rank_left < before + sum) {
 #pragma unroll
                 for (int x = 0; x < kPer; ++x) {
                     if (rank_left >= before && rank_left < before + mine[x]) {
                         sh.digit = tid * per + x;
                         sh.below = before;
+                        sh.inside = mine[x];
                     }
                     before += mine[x];
                 }
             }
-            sync_all();   // all have read the histograms, and `digit` is there
+            __syncthreads();
             prefix = (prefix << kBits[pass]) | sh.digit;
             below += sh.below;
             rank_left -= sh.below;
-        }
-    }
-    const uint32_t T = prefix, ties_leave = leave - below;   // of the tokens with key T the first so many leave
-
-    // Sums of a pair of counts over the warps ahead of this one, in this CTA and in those before it, and over the cluster.
-    static_assert(kEvWarps == 32, "a lane reads a warp's counts");
-    auto place = [&](int what, uint2 count, uint2& all) {
-        if (lane == 0) sh.count[what][warp] = count;
-        __syncthreads();
-        const uint2 x = sh.count[what][lane];
-        uint2 before = make_uint2(__reduce_add_sync(0xffffffffu, lane < warp ? x.x : 0u),
-                                  __reduce_add_sync(0xffffffffu, lane < warp ? x.y : 0u));
-        all = make_uint2(__reduce_add_sync(0xffffffffu, x.x), __reduce_add_sync(0xffffffffu, x.y));
-        if (ctas > 1) {
-            if (tid == 0) sh.total[what] = all;
-            cluster.sync();
-            all = make_uint2(0, 0);
-            for (int r = 0; r < ctas; ++r) {
-                const uint2 y = *cluster.map_shared_rank(&sh.total[what], r);
-                all.x += y.x;
-                all.y += y.y;
-                if (r < rank) {
-                    before.x += y.x;
-                    before.y += y.y;
-                }
+            if (sh.inside == rank_left + 1) {   // the whole bin leaves: its upper end will do for T
+                prefix = (prefix << shift) | ((1u << shift) - 1u);
+                no_ties = true;
+                break;
             }
         }
-        return before;
-    };
-    uint32_t ties = 0;
-    for (int i = w_begin + lane; i < w_end; i += 32) ties += key_of(i) == T;
-    ties = __reduce_add_sync(0xffffffffu, ties);
-    uint2 unused;
-    const uint32_t ties_before = place(0, make_uint2(ties, 0), unused).x;
-    // Calls f(slot, stays) for the warp's slots, a full warp at a time.
-    auto for_slots = [&](auto f) {
-        uint32_t tie = ties_before;
-        for (int base = w_begin; base < w_end; base += 32) {
-            const int i = base + lane;
-            const uint32_t k = i < w_end ? key_of(i) : 0u;
-            const uint32_t eq = __ballot_sync(0xffffffffu, i < w_end && k == T);
-            const bool goes = leave > 0 && (k < T || (k == T && tie + __popc(eq & ((1u << lane) - 1u)) < ties_leave));
-            tie += __popc(eq);
-            f(i, i < w_end && !goes, i < w_end && goes);
-        }
-    };
-    // With an out_table every token that stays is "moved", to its place among them.
-    const bool out = p.out_table != nullptr;
-    uint32_t n_holes = 0, n_moves = 0;
-    for_slots([&](int i, bool stays, bool goes) {
-        n_moves += __popc(__ballot_sync(0xffffffffu, stays && (out || i >= left)));
-        n_holes += __popc(__ballot_sync(0xffffffffu, goes && i < left));
-    });
-    uint2 all;
-    const uint2 at = place(1, make_uint2(n_holes, n_moves), all);
-    uint32_t hole = at.x, move = at.y;
-    int32_t* from = p.from + static_cast<long long>(head) * p.list;
-    int32_t* to = p.to + static_cast<long long>(head) * p.list;
-    for_slots([&](int i, bool stays, bool goes) {
-        const uint32_t mv = __ballot_sync(0xffffffffu, stays && (out || i >= left));
-        const uint32_t hl = __ballot_sync(0xffffffffu, goes && i < left);
-        const uint32_t ahead = (1u << lane) - 1u;
-        if ((mv >> lane) & 1u) from[move + __popc(mv & ahead)] = i;
-        if (!out && ((hl >> lane) & 1u)) to[hole + __popc(hl & ahead)] = i;
-        move += __popc(mv);
-        hole += __popc(hl);
-    });
-    sync_all();   // the lists are written, and no CTA's shared memory is read any more
+    }
+    if (total < 0) {
+        // Of the tokens with the key T the first so many leave.
+        const uint32_t T = prefix, ties_leave = no_ties ? 0xffffffffu : leave - below;
 
-    const int total = static_cast<int>(all.y);
+        // Sums of a pair of counts over the warps ahead of this one, in this CTA and in those before it, and over the cluster.
+        static_assert(kEvWarps == 32, "a lane reads a warp's counts");
+        auto place = [&](int what, uint2 count, uint2& all) {
+            if (lane == 0) sh.count[what][warp] = count;
+            __syncthreads();
+            const uint2 x = sh.count[what][lane];
+            uint2 before = make_uint2(__reduce_add_sync(0xffffffffu, lane < warp ? x.x : 0u),
+                                      __reduce_add_sync(0xffffffffu, lane < warp ? x.y : 0u));
+            all = make_uint2(__reduce_add_sync(0xffffffffu, x.x), __reduce_add_sync(0xffffffffu, x.y));
+            if (ctas > 1) {
+                if (tid == 0) sh.total[what] = all;
+                cluster.sync();
+                all = make_uint2(0, 0);
+#pragma unroll
+                for (int r = 0; r < ctas; ++r) {
+                    const uint2 y = *cluster.map_shared_rank(&sh.total[what], r);
+                    all.x += y.x;
+                    all.y += y.y;
+                    if (r < rank) {
+                        before.x += y.x;
+                        before.y += y.y;
+                    }
+                }
+            }
+            return before;
+        };
+        uint32_t ties_before = 0;
+        if (!no_ties) {
+            uint32_t ties = 0;
+            for (int i = w_begin + lane; i < w_end; i += 32) ties += key_of(i) == T;
+            ties = __reduce_add_sync(0xffffffffu, ties);
+            uint2 unused;
+            ties_before = place(0, make_uint2(ties, 0), unused).x;
+        }
+        // Calls f(i, slots to be moved, slots that come free), as bits, for a lane's four slots from i on, the warp's slots 128
+        // at a time.  With an out_table every token that stays is "moved", to its place among them.
+        const bool out = p.out_table != nullptr;
+        auto lanes_below = [&](uint32_t x, uint32_t& all) {   // sum of x over the lanes ahead, and over all
+            uint32_t upto = x;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, upto, s);
+                if (lane >= s) upto += y;
+            }
+            all = __shfl_sync(0xffffffffu, upto, 31);
+            return upto - x;
+        };
+        auto for_slots = [&](auto f) {
+            uint32_t tie = ties_before;
+            for (int base = w_begin; base < w_end; base += 128) {
+                const int i = base + 4 * lane;
+                uint32_t k[4] = {}, less = 0, equal = 0;
+                if (cached) {
+                    if (i < w_end) {   // the room for keys is a multiple of 4
+                        const uint4 x = *reinterpret_cast<const uint4*>(keys + (i - begin));
+                        k[0] = x.x, k[1] = x.y, k[2] = x.z, k[3] = x.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (i + j < w_end) k[j] = key_of(i + j);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    less |= (k[j] < T ? 1u : 0u) << j;
+                    equal |= (k[j] == T ? 1u : 0u) << j;
+                }
+                const uint32_t there = (1u << max(0, min(4, w_end - i))) - 1u;
+                uint32_t goes = no_ties ? less | equal : less;
+                equal &= there;
+                if (!no_ties && __any_sync(0xffffffffu, equal != 0)) {
+                    uint32_t sum;
+                    const uint32_t ahead = tie + lanes_below(__popc(equal), sum);
+                    tie += sum;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (ahead + __popc(equal & ((1u << j) - 1u)) < ties_leave) goes |= equal & (1u << j);
+                }
+                goes = leave > 0 ? goes & there : 0u;
+                const uint32_t before = (1u << max(0, min(4, left - i))) - 1u;   // the budget
+                f(i, there & ~goes & (out ? 15u : ~before), goes & before);
+            }
+        };
+        uint32_t n_holes = 0, n_moves = 0;
+        for_slots([&](int, uint32_t moves, uint32_t holes) {
+            n_moves += __popc(moves);
+            n_holes += __popc(holes);
+        });
+        uint2 all;
+        const uint2 at = place(1, make_uint2(__reduce_add_sync(0xffffffffu, n_holes), __reduce_add_sync(0xffffffffu, n_moves)), all);
+        uint32_t hole = at.x, move = at.y;
+        for_slots([&](int i, uint32_t moves, uint32_t holes) {
+            uint32_t sum;
+            const uint32_t ahead = lanes_below(__popc(moves) | __popc(holes) << 16, sum);
+            int32_t* f = from + move + (ahead & 0xffffu);
+            int32_t* t = to + hole + (ahead >> 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if ((moves >> j) & 1u) *f++ = i + j;
+                if (!out && ((holes >> j) & 1u)) *t++ = i + j;
+            }
+            move += sum & 0xffffu;
+            hole += sum >> 16;
+        });
+        sync_all();   // the lists are written, and no CTA's shared memory is read any more
+
+        total = static_cast<int>(all.y);
+    }
     if (p.moves) {
         if (rank == 0 && tid == 0) p.moves[head] = total;
         return;
@@ -393,7 +488,8 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
 
     DeviceGuard guard;
     if ((rc = guard.bind(cache->k)) != FBA_OK) return rc;
-    if (cudaFuncSetAttribute(paged_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
+    auto kernel = ctas == 1 ? paged_evict_kernel<1> : ctas == 2 ? paged_evict_kernel<2> : ctas == 4 ? paged_evict_kernel<4> : paged_evict_kernel<8>;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
         cudaGetLastError();
         return set_error(FBA_ERR_LAUNCH, "fba_paged_evict: cannot raise the dynamic shared memory limit");
     }
@@ -410,7 +506,7 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attr;
     config.numAttrs = 2;
-    cudaLaunchKernelEx(&config, paged_evict_kernel, c, p);
+    cudaLaunchKernelEx(&config, kernel, c, p);
     if ((rc = check_launch("paged_evict_kernel")) != FBA_OK || !p.moves) return rc;
     // Blocks for all of a head's entries while the grid stays within a few waves; a warp takes further batches beyond.
     long long blocks = (most + kMoveWarps * 32 - 1) / (kMoveWarps * 32);

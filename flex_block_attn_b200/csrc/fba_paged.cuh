@@ -31,14 +31,21 @@ __device__ __forceinline__ int paged_length(const PagedDev& c, const int32_t* se
     return n < 0 ? 0 : most;
 }
 
-// Row of the pools that slot `slot` of sequence b and kv head h lives in, or -1 when the table names no page there.
-__device__ __forceinline__ long long paged_row(const PagedDev& c, int b, int h, int slot, uint32_t* status) {
-    const int page = c.table[static_cast<long long>(b) * c.max_pages + (slot >> c.page_shift)];
-    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.n_pages)) {
-        report_paged(status, kBadPage, b, page);
-        return -1;
-    }
+// Page that the table names for slot `slot` of sequence b, and the row of the pools that the slot of kv head h has in it, or
+// -1 where there is no such page.  Apart, so that a thread may look up several pages at a time.
+__device__ __forceinline__ int paged_page(const PagedDev& c, int b, int slot) {
+    return c.table[static_cast<long long>(b) * c.max_pages + (slot >> c.page_shift)];
+}
+__device__ __forceinline__ long long paged_row_in(const PagedDev& c, int page, int h, int slot) {
+    if (static_cast<uint32_t>(page) >= static_cast<uint32_t>(c.n_pages)) return -1;
     return (static_cast<long long>(page) * c.Hkv + h) * c.page_size + (slot & (c.page_size - 1));
+}
+// Both, with a report.
+__device__ __forceinline__ long long paged_row(const PagedDev& c, int b, int h, int slot, uint32_t* status) {
+    const int page = paged_page(c, b, slot);
+    const long long row = paged_row_in(c, page, h, slot);
+    if (row < 0) report_paged(status, kBadPage, b, page);
+    return row;
 }
 
 // Programmatic dependent launch: a kernel of this family may be set up while the one before it in the stream still runs.  Each
