@@ -4,13 +4,15 @@
 // One CTA per (sequence, kv head), or a cluster where the keys of its slots do not fit into one CTA's shared memory:
 //   1. weights become 32-bit keys in their order, protected tokens the largest key;
 //   2. the key T of the last token that leaves is found from its digits, 11 + 11 + 10 bits from the top: a histogram of a
-//      digit per CTA, all of them added up by every CTA through distributed shared memory;
+//      digit per CTA, all of them added up by every CTA through distributed shared memory (reads of all the CTAs in
+//      flight at once, as are those of pages and weights in step 1: one after the other they cost 9 us of 55);
 //   3. counts per warp (tokens with the key T; slots that come free; tokens to be moved), exchanged the same way, give
 //      every warp the place of its entries in the lists of slots to move from and to, which are in slot order
 //      therefore, whatever the timing;
 //   4. the rows on the lists are copied, by a second kernel where there can be many.
-// In place, the i-th staying token behind slot `budget` goes to the i-th slot that came free before it: only as many rows move as
-// tokens leave from there, and no row is both read and written.
+// In place, the i-th staying token behind slot `budget` goes to the i-th slot that came free before it: only as many rows
+// move as tokens leave from there, and no row is both read and written.  Where one token is too many, as at every step of
+// serving within a budget, the smallest key is all there is to find: 128 heads of 2049 slots take 10 us, 16 with lists.
 // What bounds it: the rows copied, and with few rows the latency of the steps before.
 #include <math.h>
 #include <stdio.h>
@@ -402,9 +404,11 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
 }
 
 // The copies, a warp per 32 entries of a head's lists.
+// Seven CTAs an SM have 72 registers a thread; eight, of 64, spill: 32 heads of 4096 rows 48 us instead of 46, 512 of 2048
+// 247 instead of 228.
 constexpr int kMoveWarps = 4;
 template <bool e4m3>
-__global__ void __launch_bounds__(kMoveWarps * 32, 8) paged_move_kernel(const PagedDev c, const EvictParams p) {
+__global__ void __launch_bounds__(kMoveWarps * 32, 7) paged_move_kernel(const PagedDev c, const EvictParams p) {
     pdl_launch_dependents();
     pdl_wait();
     const int head = blockIdx.y, b = head / c.Hkv, h = head - b * c.Hkv;
@@ -474,7 +478,7 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     p.list = list;
     // The keys of a CTA's slots stay in shared memory beside the histogram, with a cluster of up to 8 CTAs if need be; a
     // cluster also where there are idle SMs and long stretches to go through (32 heads of up to 32768 slots, selection and
-    // copies: 80 us with one CTA a head, 64 with two, 55 with four).
+    // copies: 80 us with one CTA a head, 64 with two, 55 with four; with the loads of step 2 in parallel 46).
     constexpr long long kMostKeys = 200 * 1024 / 4;
     const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
     int ctas = 1;
@@ -488,7 +492,10 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
 
     DeviceGuard guard;
     if ((rc = guard.bind(cache->k)) != FBA_OK) return rc;
-    auto kernel = ctas == 1 ? paged_evict_kernel<1> : ctas == 2 ? paged_evict_kernel<2> : ctas == 4 ? paged_evict_kernel<4> : paged_evict_kernel<8>;
+    auto kernel = ctas == 1   ? paged_evict_kernel<1>
+                  : ctas == 2 ? paged_evict_kernel<2>
+                  : ctas == 4 ? paged_evict_kernel<4>
+                              : paged_evict_kernel<8>;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024) != cudaSuccess) {
         cudaGetLastError();
         return set_error(FBA_ERR_LAUNCH, "fba_paged_evict: cannot raise the dynamic shared memory limit");
@@ -508,9 +515,10 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     config.numAttrs = 2;
     cudaLaunchKernelEx(&config, kernel, c, p);
     if ((rc = check_launch("paged_evict_kernel")) != FBA_OK || !p.moves) return rc;
-    // Blocks for all of a head's entries while the grid stays within a few waves; a warp takes further batches beyond.
+    // Blocks for all of a head's entries while the grid stays within 10 waves; a warp takes further batches beyond.  With 2.3
+    // waves as the limit 320 heads of 2000 rows took 106 us instead of 97, 512 of 2048 228 instead of 216.
     long long blocks = (most + kMoveWarps * 32 - 1) / (kMoveWarps * 32);
-    const long long enough = (148 * 16 + heads - 1) / heads;
+    const long long enough = (148 * 64 + heads - 1) / heads;
     const dim3 grid(static_cast<unsigned>(blocks < enough ? blocks : enough), static_cast<unsigned>(heads));
     return launch_chained(cache->e4m3 ? paged_move_kernel<true> : paged_move_kernel<false>, grid, kMoveWarps * 32, 0,
                           static_cast<cudaStream_t>(stream), c, p);

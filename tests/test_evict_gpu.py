@@ -69,6 +69,30 @@ def test_equal_special_and_negative_weights(lens, budget):
     run(pools, table, lens, budget, 0, 0)
 
 
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("n,max_pages", [(2, 1), (300, 5), (300, 40), (6000, 94), (18001, 283)])   # one to four CTAs a head
+def test_one_token_too_many(n, max_pages, e4m3):
+    """The one that leaves first, last, in between and among equals."""
+    pools, table = make([n], 2, 64, e4m3, track=True, seed=11, max_pages=max_pages)
+    for slots in ([0], [n - 1], [n // 2], [n - 1, n // 2], range(n)):
+        for h in range(2):   # of the second head always the slot before the last
+            for s in slots if h == 0 else [n - 2]:
+                pools["weight"][table[0, s // 64], h, s % 64] = -2.0
+        run(pools, table, [n], n - 1, 0, 0)
+
+
+@pytest.mark.parametrize("lens", [[300], [18001]])
+def test_weights_of_few_leading_digits(lens):
+    """Distinct weights that agree in their first 11 or 22 bits, where the last to leave shares them with others, and where
+    it does not."""
+    for step in (2.0**-23, 2.0**-12, 2.0**-2):
+        pools, table = make(lens, 2, 64, track=True, seed=12)
+        g = torch.Generator().manual_seed(13)
+        pools["weight"] = 1.0 + step * torch.randint(0, 400, pools["weight"].shape, generator=g)
+        for budget in (lens[0] - 3, lens[0] // 2, 7):
+            run({k: x.clone() for k, x in pools.items()}, table, lens, budget, 2, 3)
+
+
 def test_a_cut_cache_is_cut_again_by_positions():
     """Slots in no order of positions; duplicates that protect more than the budget holds."""
     lens, page = [200, 130], 16
