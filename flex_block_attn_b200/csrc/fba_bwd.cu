@@ -1090,6 +1090,85 @@ extern "C" int fba_bwd_split(const void* q, const void* k, const void* v, const 
 // half the share, and dividing from there on, lost as much where the tiles fill the chip: 8 heads, 4096 rows, causal: 112
 // -> 142; 16 on 4, 8192 rows, causal: 687 -> 738.
 constexpr int kLeastSteps = 6, kMostParts = 32, kMostWindowParts = 4 * kSms;
+
+// Where the lists are long but within one and a half shares, and there are one to three an SM, SMs that take them in the
+// grid's order end far apart: the last lists begin late.  With the first few tiles divided the SMs' ends are apart from early
+// on, and the lists that follow fit together better.  Which division is best follows from no simple rule, so the end of the
+// last list is worked out on the host for 24 of them, with 2 steps for a CTA's start and end and 1 for partial sums (the
+// time of 25 measured divisions is 2.9 to 3.2 us a step of it), and the best one is taken if it ends 4 % sooner.  Backward,
+// us, undivided -> divided: 12288 rows, window 4096, 4 sinks, 16 heads on 4: 1056 -> 932; 16384 rows, window 2048, 16 on 2:
+// 873 -> 764; 16384 rows, window 4096, 128 sinks, 24 on 3: 2274 -> 2043; 9500 rows, window 700, 100 sinks, 32 on 2: 690 ->
+// 507; causal, 8192 rows, 16 on 4: 766 -> 730.  With more lists an SM there is nothing to gain (16384 rows, window 2048,
+// 24 on 8, 7 lists: 1225 -> 1215 to 1303), and below 100 steps an SM not enough for the host's time (0.3 ms, once for sizes
+// that are among the last 16 a thread asked for).
+constexpr int kPackLists = 3 * kSms, kPackSteps = 100;
+struct PackKey {
+    int n_bhk, group, Sq, Skv, window, sinks;
+    bool operator==(const PackKey& o) const {
+        return n_bhk == o.n_bhk && group == o.group && Sq == o.Sq && Skv == o.Skv && window == o.window && sinks == o.sinks;
+    }
+};
+// Where the last list ends, in steps; steps: of the key tiles of a kv head.
+static int last_end(const int* steps, int n_nt, int n_bhk, const WindowSplit& w) {
+    int end[kSms] = {};   // a heap, the SM that is free first in front
+    auto take = [&](int tile, int parts) {
+        const int cost = (steps[tile] + parts - 1) / parts + (parts > 1 ? 3 : 2);
+        for (int i = 0; i < parts * n_bhk; ++i) {
+            const int x = end[0] + cost;
+            int at = 0;
+            for (int next = 1; next < kSms; next = 2 * at + 1) {
+                if (next + 1 < kSms && end[next + 1] < end[next]) ++next;
+                if (end[next] >= x) break;
+                end[at] = end[next];
+                at = next;
+            }
+            end[at] = x;
+        }
+    };
+    for (int nt = 0; nt < n_nt; ++nt) take(nt, nt < w.sinks ? w.sink_parts : nt < w.sinks + w.lead ? w.lead_parts : 1);
+    int last = 0;
+    for (int x : end) last = x > last ? x : last;
+    return last;
+}
+// Adds the best lead tiles to w.
+static void pack_lists(const int* steps, int n_nt, const PackKey& key, long long room, WindowSplit& w) {
+    struct Known {
+        PackKey key;
+        int lead, parts;
+    };
+    static thread_local Known known[16] = {};
+    static thread_local unsigned next = 0;
+    for (const Known& k : known)
+        if (k.key == key) {
+            w.lead = k.lead;
+            w.lead_parts = k.parts;
+            return;
+        }
+    const int undivided = last_end(steps, n_nt, key.n_bhk, w);
+    int best = undivided - undivided / 25;
+    Known found = {key, 0, 1};
+    for (int parts = 2; parts <= 4; ++parts) {
+        int most = kSms / key.n_bhk, before = 0;
+        if (most > n_nt - w.sinks) most = n_nt - w.sinks;
+        if (most > room / (key.n_bhk * parts)) most = static_cast<int>(room / (key.n_bhk * parts));
+        for (int i = 1; i <= 8; ++i) {
+            WindowSplit t = w;
+            t.lead = (most * i + 7) / 8;
+            t.lead_parts = parts;
+            if (t.lead == before) continue;
+            before = t.lead;
+            const int end = last_end(steps, n_nt, key.n_bhk, t);
+            if (end >= best) continue;
+            best = end;
+            found.lead = t.lead;
+            found.parts = parts;
+        }
+    }
+    known[next++ % 16] = found;
+    w.lead = found.lead;
+    w.lead_parts = found.parts;
+}
+
 static WindowSplit window_split(int B, int Hq, int Hkv, int Sq, int Skv, const WindowDev& win) {
     const long long group = Hq / Hkv, n_bhk = static_cast<long long>(B) * Hkv;
     const int n_nt = (Skv + 127) / 128;
@@ -1133,6 +1212,11 @@ static WindowSplit window_split(int B, int Hq, int Hkv, int Sq, int Skv, const W
         while (sinks + lead < n_nt && (lead + 1) * n_bhk * lead_parts <= room && 4 * steps_of(sinks + lead) > 5 * share) ++lead;
         w.lead = lead;
         w.lead_parts = lead ? lead_parts : 1;
+    }
+    if (w.lead == 0 && n_bhk * n_nt > kSms && n_bhk * n_nt <= kPackLists && all >= kPackSteps * kSms && all < 1 << 28) {
+        int steps[kPackLists];
+        for (int nt = 0; nt < n_nt; ++nt) steps[nt] = static_cast<int>(steps_of(nt));
+        pack_lists(steps, n_nt, {static_cast<int>(n_bhk), static_cast<int>(group), Sq, Skv, win.window, win.sinks}, room, w);
     }
     return w;
 }

@@ -92,3 +92,33 @@ def test_partial_sums_stay_within_their_limit(B, Hq, Hkv, Sq, Skv, window, sinks
     n = ctypes.c_uint64()
     assert _cabi.lib().fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, window, sinks, ctypes.byref(n)) == 0
     assert n.value <= 592 * 2**17
+
+
+def test_the_same_sizes_are_always_divided_alike():
+    """Whatever was asked for in between, and in another thread."""
+    import random
+    import threading
+
+    from flex_block_attn_b200 import _cabi
+
+    lib, rng = _cabi.lib(), random.Random(5)
+
+    def parts(sizes):
+        n = ctypes.c_uint64()
+        assert lib.fba_window_partial_bytes(*sizes, ctypes.byref(n)) == 0
+        assert n.value <= 592 * 2**17
+        return n.value // 2**17
+
+    def draw():
+        heads, group = rng.choice([1, 2, 3, 4, 8]), rng.choice([1, 2, 4, 12, 16])
+        rows = rng.randint(150, 444) * 128 // heads
+        return 1, heads * group, heads, rows - rng.randint(0, 127), rows, rng.choice([0, rows // 4, rows // 9]), rng.choice([0, 4, 150])
+
+    sizes = [draw() for _ in range(60)]
+    first = [parts(x) for x in sizes]
+    assert any(first) and first == [parts(x) for x in sizes]
+    other = []
+    thread = threading.Thread(target=lambda: other.extend(parts(x) for x in reversed(sizes)))
+    thread.start()
+    thread.join()
+    assert first == other[::-1]

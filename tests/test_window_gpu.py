@@ -266,6 +266,32 @@ def test_divided_key_tiles(B, Hq, Hkv, Sq, Skv, window, sinks):
     assert torch.equal(grads[1], again[1]) and torch.equal(grads[2], again[2])
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,Sq,Skv,window,sinks", [(1, 48, 4, 4900, 4900, 1000, 3), (2, 40, 2, 4700, 4700, None, 0),
+                                                          (1, 96, 3, 6500, 6500, 500, 140)])
+def test_key_tiles_divided_to_pack_the_grid(B, Hq, Hkv, Sq, Skv, window, sinks):
+    """Long lists, one to three an SM: the first few tiles of every kv head are divided."""
+    import ctypes
+
+    import flex_block_attn_b200 as fba
+    from flex_block_attn_b200 import _cabi
+
+    n = ctypes.c_uint64()
+    assert _cabi.lib().fba_window_partial_bytes(B, Hq, Hkv, Sq, Skv, window or 0, sinks, ctypes.byref(n)) == 0 and n.value > 0
+    q, k, v, do = rand_qkv(B, Hq, Hkv, Sq, Skv, seed=Sq, device="cuda")
+    o, lse, rest = fba.forward_with_window(q, k, v, window, sinks, need_rest=True)
+    grads = fba.backward_with_window(q, k, v, o, lse, do, window, sinks, rest=rest)
+    mask, group = orc.visible(Sq, Skv, window, sinks, "cuda"), Hq // Hkv
+    for b in range(B):
+        for h in range(Hkv):
+            ours, one = (slice(b, b + 1), slice(h * group, (h + 1) * group)), (slice(b, b + 1), slice(h, h + 1))
+            want = orc.masked_attention(q[ours], k[one], v[one], mask, do[ours])
+            for got, w, what in zip((o[ours], grads[0][ours], grads[1][one], grads[2][one]), (want[0], *want[2:]),
+                                    ("O", "dQ", "dK", "dV")):
+                close(got, w, what)
+    again = fba.backward_with_window(q, k, v, o, lse, do, window, sinks, rest=rest)
+    assert torch.equal(grads[1], again[1]) and torch.equal(grads[2], again[2])
+
+
 @pytest.mark.parametrize("S,window,sinks", [(2, None, 0), (3, None, 0), (300, 2, 0), (300, 2, 1), (300, 5, 0)])
 def test_gradients_of_rows_that_see_few_keys(S, window, sinks):
     """dS is the difference of nearly equal values there; what the rounding of O left keeps it exact.  Element by element:
