@@ -147,7 +147,7 @@ struct DecodeParams {
     float* scores;       // accumulate: [B, Hq, score_stride] in units of log2, else null
     int score_stride;
     int B, Hq, group, q_tiles;      // query heads a kv head; groups of 8 NT of them
-    int window, sinks;              // window 0: none
+    int window, sinks;              // window 0: none; sinks: at most a row's slots (host-clamped: they are rounded up to tiles)
     int splits;                     // CTAs per row, each with an equal part of the row's own tiles; 0: the list of all tiles
     int n_ctas;                     //   is cut into this many pieces
     float scale_log2;
@@ -1035,7 +1035,8 @@ extern "C" int fba_paged_decode(const fba_paged_t* cache, const void* q, const i
     p.group = Hq / c.Hkv;
     p.q_tiles = d.q_tiles;
     p.window = window;
-    p.sinks = sinks;
+    const int cap = c.max_pages * c.page_size;   // below 2^30
+    p.sinks = sinks < cap ? sinks : cap;
     p.splits = d.splits;
     p.n_ctas = d.n_ctas;
     p.scale_log2 = softmax_scale * kLog2e;
