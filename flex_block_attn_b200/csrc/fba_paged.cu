@@ -1009,6 +1009,7 @@ extern "C" int fba_paged_decode(const fba_paged_t* cache, const void* q, const i
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: accumulation takes at most 16 query heads a kv head");
     if (reinterpret_cast<uintptr_t>(q) % 4 != 0 || q_strides[0] % 2 != 0 || q_strides[1] % 2 != 0)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: q must be 4-byte aligned, its strides multiples of 2");
+    if (reinterpret_cast<uintptr_t>(o) % 8 != 0) return set_error(FBA_ERR_BAD_ARG, "fba_paged_decode: o must be 8-byte aligned");
     const uint64_t need = d.part_o + d.part_ml + d.scores;
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256 != 0))
         return set_error(FBA_ERR_BAD_ARG,

@@ -363,7 +363,7 @@ int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, con
  * Attention of one new token per sequence over its cached rows, the token's own (the last) among them:
  *   o[b, h] = softmax(softmax_scale * q[b, h] . K) V over the slots j < n = seq_lens[b] with n - 1 - j < window or
  *   j < sinks (window 0: all).  q, o: bf16 [B, Hq, 128], q element (b, h, d) at b * q_strides[0] + h * q_strides[1] + d
- *   (multiples of 2), o contiguous; lse fp32 [B, Hq] or NULL.  n = 0: zeros, lse = -inf.
+ *   (multiples of 2; q 4-byte aligned), o contiguous and 8-byte aligned; lse fp32 [B, Hq] or NULL.  n = 0: zeros, lse = -inf.
  * Rows outside what a query sees are not read: whatever they hold, NaN included, does not matter.
  * e4m3: a row stands for its bytes' values times its scale.
  * accumulate != 0 (window 0, lse not NULL, at most 16 query heads a kv head): weight[slot] += the sum of the slot's
