@@ -923,6 +923,12 @@ extern "C" int fba_bwd_partial_bytes(int B, int Hq, int Hkv, int Sq, int Skv, ui
     return FBA_OK;
 }
 
+// Pointers that kernels follow 16 bytes at a time (lse_delta by bulk copies) and no tensor map covers; null is as good.
+static bool rows_aligned(const void* o, const void* o_rest, const void* dq, const void* lse_delta, const void* dq_accum) {
+    for (const void* x : {o, o_rest, dq, lse_delta, dq_accum})
+        if (reinterpret_cast<uintptr_t>(x) % 16 != 0) return false;
+    return true;
+}
 // Row statistics, and zeros in the dQ accumulator (null: none is used), by the same kernel with `fused`.
 static int launch_prep(const void* o, const void* o_rest, const void* dout, const float* lse, float* lse_delta, float* dq_accum, int Sq,
                        long long n_bhq, float scale, bool fused, cudaStream_t stream) {
@@ -1244,8 +1250,8 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     WindowDev win;
     int rc = window_args("fba_window_bwd", B, Hq, Hkv, Sq, Skv, window, sinks, softmax_scale, &win);
     if (rc != FBA_OK) return rc;
-    if (reinterpret_cast<uintptr_t>(o_rest) % 16 != 0)
-        return set_error(FBA_ERR_BAD_ARG, "fba_window_bwd: o_rest must be 16-byte aligned");
+    if (!rows_aligned(o, o_rest, dq, lse_delta, dq_accum))
+        return set_error(FBA_ERR_BAD_ARG, "fba_window_bwd: o, o_rest, dq, lse_delta and dq_accum must be 16-byte aligned");
     const long long n_bhq = static_cast<long long>(B) * Hq, n_bhk = static_cast<long long>(B) * Hkv;
     const WindowSplit w = window_split(B, Hq, Hkv, Sq, Skv, win);
     const uint64_t need = window_partial_bytes_of(w, n_bhk);

@@ -304,11 +304,12 @@ int fba_bwd_split(const void* q, const void* k, const void* v, const void* o, co
  * where it forms rowsum(dO * O).  Rows that see few keys need it: dS is the difference of nearly equal values there (two
  * keys: dQ 0.7 % off without, 0.3 % with it); in long rows it is worth a quarter of the error.
  *
- * Backward: scratch buffers as fba_bwd's (fba_bwd_scratch_bytes; dq_accum is zeroed by the call and 16-byte aligned), and
- * `partial`, 16-byte aligned, of fba_window_partial_bytes() bytes, at most 74 MB (0: NULL is accepted), for the fp32 dK / dV
- * of key tiles with long lists (sinks, which every query sees; all tiles where there are few kv heads), whose steps are
- * divided over several CTAs.  dK and dV have the same bits in every call with the same sizes; a call on part of the batch
- * or of the kv heads may divide other tiles and differ in the last bit.  dQ is summed in scheduling order, like fba_bwd's.
+ * Backward: scratch buffers as fba_bwd's (fba_bwd_scratch_bytes; dq_accum is zeroed by the call); o, dq, lse_delta and
+ * dq_accum are 16-byte aligned.  `partial`, 16-byte aligned, of fba_window_partial_bytes() bytes, at most 74 MB (0: NULL is
+ * accepted), holds the fp32 dK / dV of key tiles with long lists (sinks, which every query sees; all tiles where there are
+ * few kv heads), whose steps are divided over several CTAs.  dK and dV have the same bits in every call with the same
+ * sizes; a call on part of the batch or of the kv heads may divide other tiles and differ in the last bit.  dQ is summed in
+ * scheduling order, like fba_bwd's.
  */
 int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest, int B, int Hq, int Hkv,
                    int Sq, int Skv, int window, int sinks, float softmax_scale, uint32_t* status, void* stream);
