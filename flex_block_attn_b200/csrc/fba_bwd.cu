@@ -974,6 +974,8 @@ extern "C" int fba_bwd_split(const void* q, const void* k, const void* v, const 
     if (!q || !k || !v || !o || !lse || !dout || !dq || !dk || !dv || !lse_delta || !status ||
         (!qmajor && !dq_accum))
         return set_error(FBA_ERR_BAD_ARG, "fba_bwd: null pointer argument");
+    if (!rows_aligned(o, nullptr, dq, lse_delta, qmajor ? nullptr : dq_accum))
+        return set_error(FBA_ERR_BAD_ARG, "fba_bwd: o, dq, lse_delta and dq_accum must be 16-byte aligned");
     if (qmajor) {
         if (!q2k || !q2k->idx || !q2k->cnt || q2k->stride <= 0 || q2k->rows_per_bh <= 0 || q2k->rows_div <= 0 ||
             q2k->sub <= 0 || (q2k->bh_stride != 0 && q2k->bh_stride != q2k->rows_per_bh))

@@ -229,7 +229,8 @@ int fba_fwd_fp8kv(const void* q, const uint8_t* k8, const uint8_t* v8t, const fl
  *   k2q      : key-major list (entries are query tiles)
  *   lse_delta: scratch fp32 [B*Hq, nMt*128, 2]   (nMt = ceil(Sq/128))
  *   dq_accum : scratch fp32 [B*Hq, nMt*128, 128]; zeroed by this call
- * Both scratch buffers are caller-allocated; fba_bwd_scratch_bytes() gives their sizes.
+ * Both scratch buffers are caller-allocated; fba_bwd_scratch_bytes() gives their sizes.  o, dq and the scratch buffers are
+ * 16-byte aligned, like the tensors that a tensor map covers (any other pointer: FBA_ERR_BAD_ARG).
  */
 int fba_bwd_scratch_bytes(int B, int Hq, int Sq, uint64_t* lse_delta_bytes,
                           uint64_t* dq_accum_bytes);
