@@ -817,7 +817,8 @@ __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, 
             for (int sh = 16; sh > 0; sh >>= 1) l += __shfl_xor_sync(0xffffffffu, l, sh);
             lse = top + log2f(l);
         }
-        if (lane == 0) s_lse[hq] = lse;
+        // A head without a finite score has no probabilities, as in its output: all differences are to be -inf then.
+        if (lane == 0) s_lse[hq] = lse == -INFINITY ? INFINITY : lse;
     }
     __syncthreads();
 #pragma unroll

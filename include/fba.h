@@ -369,7 +369,8 @@ int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, con
  * Rows outside what a query sees are not read: whatever they hold, NaN included, does not matter.
  * e4m3: a row stands for its bytes' values times its scale.
  * accumulate != 0 (window 0, lse not NULL, at most 16 query heads a kv head): weight[slot] += the sum of the slot's
- * probabilities over the query heads of its kv head, in a fixed order.
+ * probabilities over the query heads of its kv head, in a fixed order.  A head whose visible scores are all -inf has no
+ * probabilities: zeros, lse = -inf, and nothing is added for it.
  * The tiles of all sequences are divided evenly over the SMs; parts of one sequence are joined by a second kernel
  * through `workspace` (256-byte aligned, fba_paged_decode_workspace_bytes()).  Results do not depend on the order in which
  * CTAs run.  They may differ in the last bit with the other sequences' lengths, which move the seams.

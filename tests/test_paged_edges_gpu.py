@@ -1,7 +1,10 @@
 """GPU: arguments and values at the ends of what the paged cache's entry points take, against the 64-bit oracle."""
+import math
+
 import pytest
 import torch
 
+from oracle import window_oracle as orc
 from tests.paged_util import make, to_gpu
 from tests.test_paged_gpu import check, queries
 
@@ -20,3 +23,35 @@ def test_sinks_that_cover_everything(lens, sinks, window, e4m3):
     q, n = queries(len(lens), 8, 3), torch.tensor(lens, dtype=torch.int32).cuda()
     o, lse = fba.paged_decode_attn(q.cuda(), to_gpu(pools), table.cuda(), n, window, sinks, need_lse=True)
     check(q, pools, table, lens, o, lse)
+
+
+@pytest.mark.parametrize("lens,Hkv", [([40], 2), ([900, 30], 2), ([3000], 2), ([1100 + i for i in range(60)], 8)])
+def test_heads_without_a_finite_score_add_nothing(lens, Hkv):
+    """Keys of -inf under queries that are positive there: no probabilities, zeros, lse of -inf, and weights as they were;
+    where only some keys are, the others share what there is.  In one part, in several, in several of many rows."""
+    import flex_block_attn_b200 as fba
+
+    page = 32
+    pools, table = make(lens, Hkv, page, track=True, seed=21)
+    q = queries(len(lens), 2 * Hkv, 5)
+    q[..., 0] = q[..., 0].abs() + 1
+    for b, n in enumerate(lens):
+        for j in range(n):   # all keys of kv head 1, every third one of kv head 0
+            row = int(table[b, j // page]), slice(None), j % page
+            pools["k"][row][1, 0] = -math.inf
+            if j % 3 == 1:
+                pools["k"][row][0, 0] = -math.inf
+    cache, n = to_gpu(pools), torch.tensor(lens, dtype=torch.int32).cuda()
+    o, lse = fba.paged_decode_attn(q.cuda(), cache, table.cuda(), n, need_lse=True, accumulate=True)
+    assert not o[:, 2:4].any() and (lse[:, 2:4] == -math.inf).all()
+    assert torch.isfinite(o.float()).all() and torch.isfinite(lse[:, :2]).all()
+    got = cache.weight.cpu()
+    for b, m in enumerate(lens):
+        new, was = (orc.rows_of(x, table[b], m, 0).double() for x in (got, pools["weight"]))
+        none = torch.arange(m) % 3 == 1
+        assert torch.equal(new[none], was[none])
+        # two heads' probabilities; a score is a sum of 128 products, off by at most dq, a weight by two fp32 roundings
+        k = orc.rows_of(pools["k"], table[b], m, 0).double()[~none]
+        dq = 128 * 2.0**-23 * 128**-0.5 * float(q[b].double().norm(dim=-1).max()) * float(k.norm(dim=-1).max())
+        assert (new >= was).all() and abs(float((new - was).sum()) - 2) <= 2 * (2 * dq + 1e-6) + 2.0**-23 * float((new + 1).sum())
+        assert torch.equal(*(orc.rows_of(x, table[b], m, 1) for x in (got, pools["weight"])))
