@@ -55,10 +55,10 @@ class _StatusMonitor:
         self._mapped_np = self.mapped.numpy()
 
     def poll_mapped(self) -> None:
-        """Raise if a kernel has reported into the words in host memory."""
-        if self._mapped_np[0]:
-            if not _capturing():
-                torch.cuda.synchronize(self.device)   # all of the words are there
+        """Raise if a kernel has reported into the words in host memory; during a capture leave that to a later call, as it
+        may neither wait for the rest of the words nor record anything into the graph."""
+        if self._mapped_np[0] and not _capturing():
+            torch.cuda.synchronize(self.device)   # all of the words are there
             self.raise_from(self.mapped.tolist())
 
     def after_call(self) -> None:

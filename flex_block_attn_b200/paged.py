@@ -4,8 +4,8 @@ No counterpart in the reference.  A pool of pages holds the keys and values of a
 ``s % page_size`` of page ``block_table[b, s // page_size]``.  Page tables and lengths are read on the device, so the calls
 neither synchronise nor depend on host copies of them, and may be captured into a graph (after one call on the device
 outside of a capture).  A page number or length that the cache does not have is left out by the kernels and raised by
-``check_status()`` (or by the first attention call after it that sees it); a page that a call writes (keys, weights or
-positions) must stand in the tables once only, pages that are only read may be shared.
+``check_status()``, or by the first call after it, outside of a capture, that sees it; a page that a call writes (keys,
+weights or positions) must stand in the tables once only, pages that are only read may be shared.
 """
 from __future__ import annotations
 

@@ -55,3 +55,32 @@ def test_heads_without_a_finite_score_add_nothing(lens, Hkv):
         dq = 128 * 2.0**-23 * 128**-0.5 * float(q[b].double().norm(dim=-1).max()) * float(k.norm(dim=-1).max())
         assert (new >= was).all() and abs(float((new - was).sum()) - 2) <= 2 * (2 * dq + 1e-6) + 2.0**-23 * float((new + 1).sum())
         assert torch.equal(*(orc.rows_of(x, table[b], m, 1) for x in (got, pools["weight"])))
+
+
+def test_a_report_ahead_of_a_capture_is_raised_behind_it():
+    """The call that is captured neither raises it nor records a clearing of the device's status words."""
+    import flex_block_attn_b200 as fba
+    from flex_block_attn_b200 import interface
+
+    pools, table = make([80], 1, 16, seed=3)
+    q, cache, n = queries(1, 2, 3).cuda(), to_gpu(pools), torch.tensor([80], dtype=torch.int32).cuda()
+    good, broken = table.cuda(), table.clone()
+    broken[0, 2] = 77
+    graph = torch.cuda.CUDAGraph()
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("FBA_CHECK_STATUS", "0")
+        m.setenv("FBA_POISON_OUTPUTS", "0")
+        fba.paged_decode_attn(q, cache, good, n)
+        fba.paged_decode_attn(q, cache, broken.cuda(), n)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            o = fba.paged_decode_attn(q, cache, good, n)
+        words = interface._monitor(q.device).buf
+        words[0] = 1
+        graph.replay()
+        assert words.tolist() == [1] + [0] * 7
+        words.zero_()
+        check(q.cpu(), pools, table, [80], o, None)
+        with pytest.raises(RuntimeError, match="page number 77"):
+            fba.check_status()
+        fba.check_status()

@@ -1,0 +1,45 @@
+"""CPU: what the status monitor does with reports of the kernels, on words that no kernel wrote."""
+import pytest
+import torch
+
+from flex_block_attn_b200 import interface
+
+
+@pytest.fixture
+def monitor(monkeypatch):
+    """A monitor without a device; ``monitor.capturing`` says whether the stream is being captured."""
+    mon = interface._StatusMonitor.__new__(interface._StatusMonitor)
+    mon.device, mon.pending, mon.capturing = torch.device("cpu"), False, False
+    mon.buf, mon.host, mon.mapped = (torch.zeros(8, dtype=torch.int32) for _ in range(3))
+    mon._mapped_np = mon.mapped.numpy()
+    mon.event = type("Done", (), {"query": lambda self: True})()
+    monkeypatch.setattr(interface, "_capturing", lambda: mon.capturing)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda device=None: None)
+    return mon
+
+
+PAGE = [2, 0, 0, 3, 0, 0, 77, 0]
+WAIT = [1, 2, 13, 5, 6, 7, 100, 0]
+
+
+def put(words, values):
+    words.copy_(torch.tensor(values, dtype=torch.int32))
+
+
+def test_a_report_is_raised_once(monitor):
+    monitor.poll_mapped()
+    put(monitor.mapped, PAGE)
+    with pytest.raises(RuntimeError, match="page number 77 for sequence 3"):
+        monitor.poll_mapped()
+    monitor.poll_mapped()
+
+
+def test_a_report_waits_for_the_end_of_a_capture(monitor):
+    """Nothing is raised, cleared or read while it may still be incomplete, and nothing recorded into the graph."""
+    put(monitor.mapped, PAGE)
+    monitor.capturing = True
+    monitor.poll_mapped()
+    assert monitor.mapped.tolist() == PAGE
+    monitor.capturing = False
+    with pytest.raises(RuntimeError, match="page number 77"):
+        monitor.poll_mapped()
