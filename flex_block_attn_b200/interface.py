@@ -59,7 +59,7 @@ class _StatusMonitor:
         may neither wait for the rest of the words nor record anything into the graph."""
         if self._mapped_np[0] and not _capturing():
             torch.cuda.synchronize(self.device)   # all of the words are there
-            self.raise_from(self.mapped.tolist())
+            self.raise_from(self.mapped)
 
     def after_call(self) -> None:
         if _capturing():   # a replay writes the words; check_status() or a later call sees them
@@ -73,12 +73,14 @@ class _StatusMonitor:
         if self.pending and not _capturing() and self.event.query():
             self.pending = False
             if int(self.host[0]) != 0:
-                self.raise_from(self.host.tolist())
+                self.raise_from(self.host, self.buf)
 
-    def raise_from(self, words) -> None:
-        self.buf.zero_()
-        self.host.zero_()
-        self.mapped.zero_()
+    @staticmethod
+    def raise_from(report: torch.Tensor, *copies: torch.Tensor) -> None:
+        """Raise what the words say, and clear them and their copies, but no others."""
+        words = report.tolist()
+        for x in (report, *copies):
+            x.zero_()
         if words[0] != 1:
             raise RuntimeError(
                 "flex_block_attn_b200: a paged cache was given the "

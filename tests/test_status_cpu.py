@@ -43,3 +43,28 @@ def test_a_report_waits_for_the_end_of_a_capture(monitor):
     monitor.capturing = False
     with pytest.raises(RuntimeError, match="page number 77"):
         monitor.poll_mapped()
+
+
+def test_a_report_in_one_set_of_words_does_not_clear_the_other(monitor):
+    """The block operator's (device words and their mirror) and those in host memory."""
+    put(monitor.mapped, PAGE)
+    put(monitor.buf, WAIT)
+    with pytest.raises(RuntimeError, match="page number 77"):
+        monitor.poll_mapped()
+    assert monitor.buf.tolist() == WAIT and not monitor.mapped.any()
+    put(monitor.host, WAIT)
+    put(monitor.mapped, PAGE)
+    monitor.pending = True
+    with pytest.raises(RuntimeError, match=r"wait timed out.*block=\(5,6\)"):
+        monitor.poll()
+    assert not monitor.buf.any() and not monitor.host.any() and monitor.mapped.tolist() == PAGE
+    with pytest.raises(RuntimeError, match="page number 77"):
+        monitor.poll_mapped()
+
+
+def test_a_timeout_in_the_words_in_host_memory(monitor):
+    """The window kernels report there."""
+    put(monitor.mapped, WAIT)
+    with pytest.raises(RuntimeError, match="kernel=2 role=13"):
+        monitor.poll_mapped()
+    assert not monitor.mapped.any()
