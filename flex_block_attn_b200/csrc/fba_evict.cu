@@ -448,7 +448,8 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     int rc = paged_args("fba_paged_evict", cache, B, &c);
     if (rc != FBA_OK) return rc;
     if (!seq_lens || !out_lens || !status) return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: null pointer argument");
-    if (out_lens == seq_lens) return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: out_lens must not be seq_lens");
+    if (lens_overlap(out_lens, seq_lens, B) || lens_overlap(out_lens, next_positions, B))
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: out_lens must not overlap seq_lens or next_positions");
     if (!c.weight) return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: the cache has no weights");
     if (budget <= 0 || sinks < 0 || recent < 0 || static_cast<long long>(sinks) + recent > budget)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: budget must be positive, and sinks + recent at most budget");

@@ -884,8 +884,8 @@ extern "C" int fba_paged_append(const fba_paged_t* cache, const void* k, const v
     if (rc != FBA_OK) return rc;
     if (!k || !v || !k_strides || !v_strides || !seq_lens || !status)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: null pointer argument");
-    if (out_lens && out_lens == seq_lens)
-        return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: out_lens must not be seq_lens");
+    if (lens_overlap(out_lens, seq_lens, B) || lens_overlap(out_lens, new_lens, B) || lens_overlap(out_lens, positions, B))
+        return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: out_lens must not overlap seq_lens, new_lens or positions");
     if (T <= 0) return set_error(FBA_ERR_BAD_ARG, "fba_paged_append: non-positive size");
     if (static_cast<long long>(T) * c.Hkv > 1 << 30)   // rows, and rows plus a grid's, are counted in 31 bits
         return set_error(FBA_ERR_TOO_LARGE, "fba_paged_append: more than 2^30 rows of a sequence");

@@ -352,10 +352,10 @@ typedef struct fba_paged {
  * Write new tokens behind the sequences' ends: token t < new_lens[b] (NULL: T) of sequence b goes to slot
  * seq_lens[b] + t.  k, v: bf16, element (b, h, t, d) at b * stride[0] + h * stride[1] + t * stride[2] + d, strides in
  * elements and multiples of 8, bases 16-byte aligned.  e4m3: per row scale = max(max|x| * fp32(1/448), 2^-126) (1 for an
- * all-zero row, NaN for a row with a NaN or an infinity), byte = e4m3(x * (1 / scale)), round to nearest even.  With weight / position: 0 and positions[b] + t
- * (NULL: the slot).  out_lens (NULL, or int32 [B], not seq_lens itself) receives seq_lens[b] + new_lens[b].  Tokens that do not fit
- * into the table's row are left out, with the report above, and not counted; so are all tokens of a sequence whose length
- * is out of range.
+ * all-zero row, NaN for a row with a NaN or an infinity), byte = e4m3(x * (1 / scale)), round to nearest even.  A
+ * weight becomes 0, a position positions[b] + t (NULL: the slot).  out_lens (NULL, or int32 [B], which must not overlap seq_lens,
+ * new_lens or positions) receives seq_lens[b] + new_lens[b].  Tokens that do not fit into the table's row are left out, with
+ * the report above, and not counted; so are all tokens of a sequence whose length is out of range.
  */
 int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, const int64_t* k_strides,
                      const int64_t* v_strides, int B, int T, const int32_t* seq_lens, const int32_t* new_lens,
@@ -386,7 +386,7 @@ int fba_paged_decode(const fba_paged_t* cache, const void* q, const int64_t* q_s
  * that come first by (weight, slot), among those that are not protected.  Protected are tokens with position < sinks and
  * those with position >= next_positions[b] - recent (NULL: n - recent); sinks + recent <= budget.  A NaN weight counts as
  * the largest.  (Should more than `budget` positions be protected all the same, the lowest slots of them leave.)
- * out_lens[b] (not seq_lens itself) = min(n, budget).
+ * out_lens[b] = min(n, budget); it must not overlap seq_lens or next_positions.
  *   out_table NULL: in place.  A token that stays keeps its slot if that is below the budget; the others that stay go, in
  *     slot order, to the slots below the budget that came free, in slot order.  Slots from the budget on keep what they
  *     hold.  The slots are in no order of positions afterwards; attention does not depend on it.
