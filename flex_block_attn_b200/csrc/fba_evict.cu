@@ -453,6 +453,7 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     if (!c.weight) return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: the cache has no weights");
     if (budget <= 0 || sinks < 0 || recent < 0 || static_cast<long long>(sinks) + recent > budget)
         return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: budget must be positive, and sinks + recent at most budget");
+    if (out_table == c.table) return set_error(FBA_ERR_BAD_ARG, "fba_paged_evict: out_table must not be the cache's table");
     const int list = evict_list(c.page_size, c.max_pages, budget);
     if (out_table && (out_pages <= 0 || static_cast<long long>(out_pages) * c.page_size < list ||
                       static_cast<long long>(out_pages) * c.page_size >= 1 << 30))

@@ -37,3 +37,11 @@ def test_evict_refuses_lengths_over_its_inputs(lib, name, B, offset):  # noqa: F
     rc = lib.fba_paged_evict(struct(**TRACK), B, ctypes.c_void_p(4096), 20, 0, 0, ctypes.c_void_p(8192), None, 0,
                              ctypes.c_void_p(at[name] + offset), some, 2**30, some, None)
     assert rc == -1 and b"out_lens must not overlap" in lib.fba_last_error()
+
+
+def test_evict_refuses_its_own_table_as_the_new_one(lib):  # noqa: F811
+    """Rows would be written over others that are still to be read."""
+    some, table = ctypes.c_void_p(256), ctypes.c_void_p(4096)
+    rc = lib.fba_paged_evict(struct(**TRACK, table=4096), 1, some, 20, 0, 0, None, table, 3, ctypes.c_void_p(512), some, 2**30,
+                             some, None)
+    assert rc == -1 and b"out_table must not be the cache's table" in lib.fba_last_error()
