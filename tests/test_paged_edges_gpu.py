@@ -84,3 +84,48 @@ def test_a_report_ahead_of_a_capture_is_raised_behind_it():
         with pytest.raises(RuntimeError, match="page number 77"):
             fba.check_status()
         fba.check_status()
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("lens,Hkv", [([700, 64, 0], 2), ([20 * i for i in range(60)], 8)])
+def test_a_graph_of_many_steps(lens, Hkv, e4m3):
+    """Steps with no other kernel in between, in memory that later steps use again: each reads the lengths and rows of the
+    step before it, and none later ones."""
+    import flex_block_attn_b200 as fba
+
+    steps, page, B = 12, 32, len(lens)
+    pools, table = make([n + steps for n in lens], Hkv, page, e4m3, seed=31)
+    g = torch.Generator().manual_seed(32)
+    q, k, v = (torch.randn((steps, B, h, 1, 128), generator=g).bfloat16() for h in (2 * Hkv, Hkv, Hkv))
+    for b, n in enumerate(lens):   # the rows that the steps write
+        for i in range(steps):
+            at = int(table[b, (n + i) // page]), slice(None), (n + i) % page
+            for name, x in (("k", k), ("v", v)):
+                if e4m3:
+                    pools[name][at], pools[name + "_scale"][at] = orc.quantize_rows(x[i, b, :, 0])
+                else:
+                    pools[name][at] = x[i, b, :, 0]
+    cache = to_gpu(pools)
+    for name in pools:   # not there yet
+        x = getattr(cache, name)
+        for b, n in enumerate(lens):
+            for i in range(steps):
+                x[int(table[b, (n + i) // page]), :, (n + i) % page] = 0x7F if x.dtype == torch.uint8 else math.nan
+    tab, start, dev = table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), [x.cuda() for x in (q, k, v)]
+    fba.paged_decode_attn(dev[0][0, :, :, 0].contiguous(), cache, tab, start)
+    torch.cuda.synchronize()
+    graph, outs = torch.cuda.CUDAGraph(), []
+    with pytest.MonkeyPatch.context() as m:
+        m.setenv("FBA_POISON_OUTPUTS", "0")
+        with torch.cuda.graph(graph):
+            n = start
+            for i in range(steps):
+                n = fba.append_kv(cache, dev[1][i], dev[2][i], tab, n)
+                outs.append(fba.paged_decode_attn(dev[0][i, :, :, 0], cache, tab, n, need_lse=True))
+    for _ in range(2):
+        for o, lse in outs:
+            o.fill_(math.nan), lse.fill_(math.nan)
+        graph.replay()
+    for i, (o, lse) in enumerate(outs):
+        check(q[i, :, :, 0], pools, table, [x + i + 1 for x in lens], o, lse)
+    fba.check_status()
