@@ -114,6 +114,7 @@ struct BwdParams {
     WindowSplit wsplit;    //   which tiles' steps are divided
     int Sq, n_bhk;         //   kv heads in all
     int heads_at_once;     //   kv heads whose tiles take turns in the grid
+    float ds_scale;        //   `scale` as dS is multiplied by it: 0 where no query has a choice of keys
 };
 
 // ------------------------------------------------------------------------------------------
@@ -632,7 +633,8 @@ fba_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__
         const int row = quad * 32 + lane;  // epilogue: row inside the tile == TMEM lane
         const uint32_t lane_base = static_cast<uint32_t>(quad * 32) << 16;
         const float c = p.scale * kLog2e;
-        const float2 sc2 = make_float2(p.scale, p.scale);
+        const float ds_scale = kWindow ? p.ds_scale : p.scale;
+        const float2 sc2 = make_float2(ds_scale, ds_scale);
         const int mbit0 = 8 * (quad >> 1);  // key-half part of the mask bit index
         const int q4 = lane & 3;
         // Address of this lane's row of the 8 x 8 dS^T matrices (stmatrix): swizzled chunk of query columns 8 (lane / 8) ..
@@ -1273,7 +1275,11 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     if ((rc = make_tmap_bf16(&tm_do, dout, Sq, n_bhq, 128)) != FBA_OK) return rc;
     if ((rc = make_tmap_bf16(&tm_dk, dk, Skv, n_bhk, 128)) != FBA_OK) return rc;
     if ((rc = make_tmap_bf16(&tm_dv, dv, Skv, n_bhk, 128)) != FBA_OK) return rc;
-    if ((rc = launch_prep(o, o_rest, dout, lse, lse_delta, dq_accum, Sq, n_bhq, softmax_scale, true, stream)) != FBA_OK) return rc;
+    // A query that sees one key has a probability of 1 whatever its score: dP and delta are equal, and their difference would
+    // be what two orders of summation leave, 1e-7 where the gradient is 0.  Where that is so for every query (a window of 1
+    // without sinks, a single key) dS is multiplied by 0 instead of the scale.
+    const float ds_scale = win.window == 1 && (win.sinks == 0 || Skv == 1) ? 0.f : softmax_scale;
+    if ((rc = launch_prep(o, o_rest, dout, lse, lse_delta, dq_accum, Sq, n_bhq, ds_scale, true, stream)) != FBA_OK) return rc;
 
     BwdParams p = {};
     p.ld = reinterpret_cast<const float2*>(lse_delta);
@@ -1283,6 +1289,7 @@ extern "C" int fba_window_bwd(const void* q, const void* k, const void* v, const
     p.Hq = Hq;
     p.Hkv = Hkv;
     p.scale = softmax_scale;
+    p.ds_scale = ds_scale;
     p.partial = partial;
     p.n_ntiles = n_ntiles;
     p.win = win;
