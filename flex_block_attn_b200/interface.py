@@ -100,8 +100,7 @@ def _monitor(device: torch.device) -> _StatusMonitor:
     if mon is None:
         if _capturing():   # the words must not live in a graph's memory
             raise RuntimeError("flex_block_attn_b200: make one call on this device before a stream capture")
-        mon = _StatusMonitor(torch.device("cuda", key))
-        _monitors[key] = mon
+        mon = _monitors.setdefault(key, _StatusMonitor(torch.device("cuda", key)))   # another thread's, if that was first
     return mon
 
 

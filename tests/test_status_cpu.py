@@ -68,3 +68,25 @@ def test_a_timeout_in_the_words_in_host_memory(monitor):
     with pytest.raises(RuntimeError, match="kernel=2 role=13"):
         monitor.poll_mapped()
     assert not monitor.mapped.any()
+
+
+def test_threads_that_call_first_share_one_monitor(monkeypatch):
+    """Words that nobody looks at again would lose what kernels report there."""
+    import threading
+
+    both = threading.Barrier(2, timeout=10)
+
+    class Slow:
+        def __init__(self, device):
+            both.wait()
+
+    monkeypatch.setattr(interface, "_StatusMonitor", Slow)
+    monkeypatch.setattr(interface, "_monitors", {})
+    monkeypatch.setattr(interface, "_capturing", lambda: False)
+    got = []
+    threads = [threading.Thread(target=lambda: got.append(interface._monitor(torch.device("cuda", 0)))) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert len(got) == 2 and got[0] is got[1] is interface._monitors[0]
