@@ -12,7 +12,8 @@
 //   4. the rows on the lists are copied, by a second kernel where there can be many.
 // In place, the i-th staying token behind slot `budget` goes to the i-th slot that came free before it: only as many rows
 // move as tokens leave from there, and no row is both read and written.  Where one token is too many, as at every step of
-// serving within a budget, the smallest key is all there is to find: 128 heads of 2049 slots take 10 us, 16 with lists.
+// serving within a budget, the smallest key is all there is to find: 128 heads of 2049 slots take 5.3 us behind other work, 9
+// by themselves and 10 with a cold L2; with two too many, which takes the lists, 8.7, 13 and 14.
 // What bounds it: the rows copied, and with few rows the latency of the steps before.
 #include <math.h>
 #include <stdio.h>
@@ -117,7 +118,8 @@ __device__ __forceinline__ void copy_rows(const PagedDev& c, const EvictParams& 
     }
 }
 
-// kCtas: CTAs a head, one cluster.
+// kCtas: CTAs a head, one cluster.  1024 threads leave 64 registers each, and 68 to 76 bytes are spilled; with 512 threads
+// many heads took longer (126 -> 130, 99 -> 110 us).
 template <int kCtas>
 __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev c, const EvictParams p) {
     extern __shared__ __align__(16) uint32_t keys[];
@@ -404,8 +406,8 @@ __global__ void __launch_bounds__(kEvThreads) paged_evict_kernel(const PagedDev 
 }
 
 // The copies, a warp per 32 entries of a head's lists.
-// Seven CTAs an SM have 72 registers a thread; eight, of 64, spill: 32 heads of 4096 rows 48 us instead of 46, 512 of 2048
-// 247 instead of 228.
+// Seven CTAs an SM have 72 registers a thread (20 bytes spilled); eight, of 64, spill more: 32 heads of 4096 rows 48 us instead
+// of 46, 512 of 2048 247 instead of 228.
 constexpr int kMoveWarps = 4;
 template <bool e4m3>
 __global__ void __launch_bounds__(kMoveWarps * 32, 7) paged_move_kernel(const PagedDev c, const EvictParams p) {
@@ -480,7 +482,9 @@ extern "C" int fba_paged_evict(const fba_paged_t* cache, int B, const int32_t* s
     p.list = list;
     // The keys of a CTA's slots stay in shared memory beside the histogram, with a cluster of up to 8 CTAs if need be; a
     // cluster also where there are idle SMs and long stretches to go through (32 heads of up to 32768 slots, selection and
-    // copies: 80 us with one CTA a head, 64 with two, 55 with four; with the loads of step 2 in parallel 46).
+    // copies: 80 us with one CTA a head, 64 with two, 55 with four; with the loads of step 2 in parallel 46).  All of it for
+    // what the table has room for, as the host does not know the lengths: 128 heads of 2049 slots, one too many, take 5.5 us
+    // in tables for 2112, 8 for 16384, 21 for 131072.
     constexpr long long kMostKeys = 200 * 1024 / 4;
     const long long cap = static_cast<long long>(c.max_pages) * c.page_size;
     int ctas = 1;

@@ -98,10 +98,12 @@ __global__ void __launch_bounds__(256) paged_append_kernel(const PagedDev c, con
 
 // ------------------------------------------------------------------------------------------ decode
 //
-// The rows of a (sequence, kv head) are taken 16 at a time ("tiles", which never straddle a page).  All tiles of all
-// sequences form one list, which is cut into equal pieces, one per CTA; a CTA's piece may cover parts of several rows
-// ("row": sequence, kv head, group of at most 8 * NT of its query heads), and a row may be cut over several CTAs, whose
-// partial results (running maximum, sum, unnormalised output) a second kernel joins.
+// The rows of a (sequence, kv head) are taken 16 at a time ("tiles", which never straddle a page).  They are cut up in one of
+// two ways (decode_plan has the rule), for every "row": sequence, kv head, group of at most 8 * NT of its query heads.
+//   Many rows: each is cut into the same number of equal parts, one or more, with a CTA for each.
+//   Few rows: all tiles of all rows form one list, which is cut into equal pieces, one per CTA; a piece may cover parts of
+//   several rows, and a row may be cut over several pieces.
+// The partial results of a row (running maximum, sum, unnormalised output) are joined by a second kernel.
 //
 // In a CTA the four warps take the tiles in turn, each with a ring of its own in shared memory that cp.async fills several
 // tiles ahead, across the seams between rows; rows that the query does not see are filled with zeros instead of being
@@ -772,7 +774,9 @@ __device__ __forceinline__ void join(const PagedDev& c, const DecodeParams& p, i
 }
 
 // Adds the probabilities to the weights, from the scores and the parts' sums: a block of the join's launch for each stretch of
-// kWeighSlots slots.  What does not depend on the sums is under way before they are looked at.
+// kWeighSlots slots.  What does not depend on the sums is under way before they are looked at.  The host does not know the
+// lengths: there are blocks, and room for scores, for all that the table has room for (16 sequences of 2049 tokens, 32 heads
+// on 8: 34 us with the decode in tables for 2112 slots, 35 for 16384, 65 for 131072).
 constexpr int kWeighSlots = 256;
 template <int NT, int kWarps>
 __device__ __forceinline__ void weigh(const PagedDev& c, const DecodeParams& p, int b, int h, int stretch) {
@@ -925,7 +929,9 @@ DecodePlan decode_plan(int B, int Hq, int Hkv, int page_size, int max_pages, boo
     // The order in which CTAs end evens out lengths and SMs, and a row in one part needs no join.  Few rows: the list of all
     // tiles in as many pieces as are resident at a time.  Us, list -> rows: 256 sequences of 600 tokens and 8 kv heads 126 ->
     // 100, of 1 - 1000 126 -> 84, 64 of 2048 95 -> 83 (1 part), of 512 - 8192 182 -> 170 (3 parts); e4m3, 64 of 1 - 2048 63 ->
-    // 41, of 2048 58 -> 68.  Rows that barely fill the chip: 40 sequences of 1500 50 -> 54.
+    // 41, of 2048 58 -> 68 (the rule counts two CTAs an SM for both types, though three of e4m3 fit: 512 rows end in a wave
+    // that is mostly empty).  Rows that barely fill the chip: 40 sequences of 1500 50 -> 54.  `tiles` is what the table has
+    // room for, so the cut, and with it the last bits, follow from its width.
     // (The list in two, three and four waves: 64 sequences of 512 - 8192 183 -> 179, 178, 177; two long e4m3 ones 101 ->
     // 105, 109, 115: a CTA's start and end cost a few us.)
     const long long resident = 148 * (d.nt == 1 && e4m3 ? 3 : 2), four_waves = 4 * 2 * 148;

@@ -170,7 +170,8 @@ def paged_decode_attn(q: torch.Tensor, cache: PagedKVCache, block_table: torch.T
         block_table: int32 [B, max_pages]; seq_lens: int32 [B], the new token counted
         window, sinks: as for ``sliding_window_attn_func``; only the pages that hold visible tokens are read
         accumulate: add to ``cache.weight`` the probability that each token received, summed over the query heads of
-            its kv head (no window; at most 16 query heads per kv head)
+            its kv head (no window; at most 16 query heads per kv head).  Takes 4 bytes of scratch per query head and
+            slot that the table has room for: pass a table of the pages in use, not of the most there may be
 
     Returns o, bf16 [B, heads, 128] (and the log-sum-exp, fp32 [B, heads], with ``need_lse``).  A sequence of length 0
     gives zeros and -inf.  Not differentiable.
@@ -220,6 +221,8 @@ def evict_kv(cache: PagedKVCache, block_table: torch.Tensor, seq_lens: torch.Ten
     Every kv head drops, of its n tokens, the n - budget with the least ``cache.weight`` (of equal ones the lowest slots)
     that are not protected: the first ``sinks`` positions and the last ``recent`` ones stay (sinks + recent <= budget).
     ``next_positions``: int32 [B], how many tokens the sequences have seen; None = seq_lens (never cut before).
+    The weights are what ``paged_decode_attn(..., accumulate=True)`` and the caller have put there; ``append_kv`` starts
+    with 0, so a prompt that is cut before anything was accumulated loses its first unprotected tokens.
 
     In place, the staying tokens behind the budget move to the slots that came free before it: the slots are then in no
     order of positions (``cache.position`` keeps them), the pages from ``ceil(budget / page_size)`` on are free, and

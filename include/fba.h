@@ -372,9 +372,15 @@ int fba_paged_append(const fba_paged_t* cache, const void* k, const void* v, con
  * accumulate != 0 (window 0, lse not NULL, at most 16 query heads a kv head): weight[slot] += the sum of the slot's
  * probabilities over the query heads of its kv head, in a fixed order.  A head whose visible scores are all -inf has no
  * probabilities: zeros, lse = -inf, and nothing is added for it.
- * The tiles of all sequences are divided evenly over the SMs; parts of one sequence are joined by a second kernel
- * through `workspace` (256-byte aligned, fba_paged_decode_workspace_bytes()).  Results do not depend on the order in which
- * CTAs run.  They may differ in the last bit with the other sequences' lengths, which move the seams.
+ * Where there are many rows (sequence, kv head, group of 8 or 16 query heads) each is cut into the same number of equal
+ * parts, a CTA for each; where there are few, the tiles of all rows are divided evenly over the SMs.  Parts of a row are joined
+ * by a second kernel through `workspace` (256-byte aligned, fba_paged_decode_workspace_bytes()).  Results do not depend on
+ * the order in which CTAs run.  The seams depend on B, Hq, Hkv and max_pages * page_size, and with few rows on the other
+ * sequences' lengths, too: where these differ, results may in the last bit.
+ * The host does not know the lengths, so that workspace and launches follow from what the table has room for.  With
+ * accumulation the workspace holds B * Hq * max_pages * page_size floats (64 sequences of 32 heads with room for 131072
+ * slots: 1 GiB), and wide tables take time: a caller whose sequences are short, as behind an eviction, passes a table of the
+ * pages in use.
  */
 int fba_paged_decode_workspace_bytes(int B, int Hq, int Hkv, int page_size, int max_pages, int e4m3, int accumulate,
                                      uint64_t* bytes);
@@ -393,6 +399,9 @@ int fba_paged_decode(const fba_paged_t* cache, const void* q, const int64_t* q_s
  *     hold.  The slots are in no order of positions afterwards; attention does not depend on it.
  *   out_table int32 [B, out_pages]: the tokens that stay are copied in slot order to slots 0, 1, ... of that table (all n
  *     where n <= budget), whose pages must not be among those that `table` names; the source is left as it is.
+ * Weights are what the caller and fba_paged_decode's accumulation put there: tokens just appended have 0, so that a prompt cut
+ * before anything was accumulated loses its lowest slots that are not protected.  Time follows from the table's width as well
+ * as from the lengths (see fba_paged_decode).
  * K, V, scales, weights and positions move together.  workspace: 4-byte aligned, fba_paged_evict_workspace_bytes() bytes.
  * The result does not depend on timing.
  */
