@@ -71,7 +71,8 @@ int launch_chained(void (*kernel)(Params...), dim3 grid, int threads, size_t sme
 
 // Whether two arrays of B lengths or positions share memory: what one CTA of a sequence writes, others may still have to read.
 inline bool lens_overlap(const int32_t* x, const int32_t* y, int B) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y), n = sizeof(int32_t) * static_cast<uintptr_t>(B);
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x), b = reinterpret_cast<uintptr_t>(y);
+    const uintptr_t n = sizeof(int32_t) * static_cast<uintptr_t>(B);
     return x && y && a < b + n && b < a + n;
 }
 

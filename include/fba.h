@@ -308,10 +308,10 @@ int fba_bwd_split(const void* q, const void* k, const void* v, const void* o, co
  * Backward: scratch buffers as fba_bwd's (fba_bwd_scratch_bytes; dq_accum is zeroed by the call); o, dq, lse_delta and
  * dq_accum are 16-byte aligned.  `partial`, 16-byte aligned, of fba_window_partial_bytes() bytes, at most 74 MB (0: NULL is
  * accepted), holds the fp32 dK / dV of key tiles with long lists (sinks, which every query sees; all tiles where there are
- * few kv heads, unless the window leaves the first of them to no query), whose steps are divided over several CTAs.  dK and dV have the same bits in every call with the same
- * sizes; a call on part of the batch or of the kv heads may divide other tiles and differ in the last bit.  dQ is summed in
- * scheduling order, like fba_bwd's.  Where no query sees more than one key (window 1 without sinks, Skv 1) dQ and dK are
- * exact zeros.
+ * few kv heads, unless the window leaves the first of them to no query), whose steps are divided over several CTAs.  dK and
+ * dV have the same bits in every call with the same sizes; a call on part of the batch or of the kv heads may divide other
+ * tiles and differ in the last bit.  dQ is summed in scheduling order, like fba_bwd's.  Where no query sees more than one
+ * key (window 1 without sinks, Skv 1) dQ and dK are exact zeros.
  */
 int fba_window_fwd(const void* q, const void* k, const void* v, void* o, float* lse, void* o_rest, int B, int Hq, int Hkv,
                    int Sq, int Skv, int window, int sinks, float softmax_scale, uint32_t* status, void* stream);
